@@ -142,6 +142,108 @@ int kve_attn_plan(const int32_t* block_tables, const int32_t* seq_rows, const in
                   void* plan, size_t plan_bytes, void* stream);
 
 /*
+ * Trees of drafted tokens. The q_len new tokens of a sequence are the nodes of a
+ * tree instead of a chain: node 0 the last emitted token, node t a draft that
+ * continues node parents[t] < t. Node t's K/V sits at slot start + t like a
+ * chain's (kve_kv_write, kve_rope_kv_write), its rotary position is start +
+ * depth[t]. No counterpart in the reference, whose drafts are chains
+ * (kvengine/speculative.py:111-215).
+ */
+#define KVE_TREE_MAX_NODES 64
+
+/*
+ * kve_tree_masks: masks[i][t] (int64 [num_seqs, nodes]) = bit j set where node j
+ * is node t or stands above it; depths[i][t] (int32) = nodes above t. parents:
+ * int32 [num_seqs, nodes], nodes <= KVE_TREE_MAX_NODES; a parent outside [0, t)
+ * counts as none (-1 by convention). node_counts: per-sequence node count (NULL:
+ * all `nodes`); nodes past it get mask 0 and depth 0. Either output may be NULL.
+ */
+int kve_tree_masks(const int32_t* parents, const int32_t* node_counts, int num_seqs, int nodes,
+                   int64_t* masks, int32_t* depths, void* stream);
+
+/*
+ * kve_paged_tree_attn: kve_paged_verify_attn (same arguments, layouts, plan,
+ * workspace and summation orders) where query t sees keys 0 .. start_pos[row]-1
+ * and, of the new tokens, those j <= t whose bit j of masks[i][t] is set (bits
+ * above t are ignored: a parent stands before its children). masks: int64
+ * [num_seqs, q_len] (kve_tree_masks), q_len <= KVE_TREE_MAX_NODES. A row that sees
+ * no key at all is zeros. What a key that a row does not see holds, infinities and
+ * NaN too, never reaches that row. scale > 0. The masks of a chain (bits 0..t) give
+ * kve_paged_verify_attn's bits.
+ */
+int kve_paged_tree_attn(const void* q, const void* k_pool, const void* v_pool,
+                        const int64_t* masks, const int32_t* block_tables,
+                        const int32_t* seq_rows, const int32_t* start_pos, const int32_t* q_lens,
+                        int num_seqs, int q_len, int num_q_heads, int num_kv_heads, int head_dim,
+                        int block_size, int max_blocks, int num_rows, int num_blocks, int max_ctx,
+                        int unit_blocks, int key_waves, float scale, int dtype, const void* plan,
+                        void* out, void* workspace, size_t workspace_bytes, int layout,
+                        void* stream);
+
+/*
+ * kve_tree_accept: the walk of each sequence's tree by the target's picks, from
+ * node 0: the child whose token is the pick at the current node (the lowest such
+ * node) is accepted and walked to; where there is none, the pick is emitted.
+ * The tree's form of kve_accept (kvengine/speculative.py:169-197): with a chain's
+ * parents, tokens = [last token, drafts] and the same preds it gives the same
+ * n_acc, emitted and keep_lens.
+ * tokens, preds: [num_seqs, nodes] (preds[i][t]: the target's token after node t);
+ * parents, node_counts as for kve_tree_masks
+ * n_acc [num_seqs]: accepted nodes below node 0
+ * emitted [num_seqs, nodes]: their tokens, then the pick after the last one, then -1
+ * path [num_seqs, nodes]: the nodes walked, node 0 first, then -1
+ * keep_lens[i] = start + 1 + n_acc[i], where start = lens[row] - node count: the
+ *      length to roll back to (kve_rollback), lens including the whole tree
+ * k_pool, v_pool (both or neither): [num_layers, ...] pools of contiguous layers;
+ *      the K/V of path[j] moves to slot start + j in every layer, so that the
+ *      accepted tokens are consecutive. Slots past keep_lens are left as they are.
+ * A sequence of no nodes has n_acc 0, emitted and path -1 and keeps its length. Where
+ * two entries of seq_rows name one row, only the first one's K/V is moved.
+ * lens may be NULL without pools and keep_lens.
+ */
+int kve_tree_accept(const int32_t* tokens, const int32_t* parents, const int32_t* preds,
+                    const int32_t* node_counts, const int32_t* lens, int num_rows,
+                    const int32_t* seq_rows, int num_seqs, int nodes, int32_t* n_acc,
+                    int32_t* emitted, int32_t* path, int32_t* keep_lens, void* k_pool,
+                    void* v_pool, const int32_t* block_tables, int num_layers, int num_kv_heads,
+                    int head_dim, int block_size, int max_blocks, int num_blocks, int dtype,
+                    void* stream);
+
+/*
+ * kve_sample_verify: verification of drafted tokens by rejection sampling (decoding
+ * at a temperature; kve_accept is the greedy form). With p_j, q_j the softmax of
+ * the target's and the draft's logits over T at position j, draft x_j is accepted
+ * while u_accept[j] * q_j(x_j) < p_j(x_j); the token after the accepted ones is the
+ * lowest id i whose running sum r_0 + .. + r_i exceeds u_sample * sum(r), with
+ * r = max(p_j - q_j, 0) at the first rejected j (p_j itself where that has no mass) and
+ * r = p_k where every draft was accepted. So emitted tokens are distributed as the
+ * target's own samples, for uniform numbers in [0, 1). All in 64 bits: a token is a
+ * place among V running sums, and 32-bit ones would move one draw in a hundred.
+ * target: [num_seqs, k + 1, V] logits, draft: [num_seqs, k, V] or NULL (drafts that were
+ *      not sampled: q_j is one at x_j), both `dtype`, with element strides per
+ *      sequence and position (any alignment of the type)
+ * drafts [num_seqs, k] (an id outside [0, V) is rejected), u_accept [num_seqs, k] float,
+ *      u_sample [num_seqs] float; k = 0 samples one token per sequence
+ * temperatures [num_seqs] float, or NULL: `temperature` for all; where T is not
+ *      positive and finite, n_acc is 0 and emitted -1
+ * n_acc [num_seqs]; emitted [num_seqs, k + 1]: accepted drafts, the sampled token, then
+ *      -1. A position whose logits have no distribution (NaN, +inf, all -inf) rejects its
+ *      draft and emits -1.
+ * keep_lens[i] = lens[row] - k + n_acc[i] as for kve_accept (NULL: not wanted)
+ * workspace: kve_sample_workspace_bytes(...) bytes, 16-byte aligned; no
+ *      initialisation needed
+ */
+size_t kve_sample_workspace_bytes(int num_seqs, int k, int vocab, int dtype);
+
+int kve_sample_verify(const void* target, int64_t target_seq_stride, int64_t target_pos_stride,
+                      const void* draft, int64_t draft_seq_stride, int64_t draft_pos_stride,
+                      const int32_t* drafts, const float* u_accept, const float* u_sample,
+                      const float* temperatures, float temperature, const int32_t* lens,
+                      int num_rows, const int32_t* seq_rows, int num_seqs, int k, int vocab,
+                      int dtype, int32_t* n_acc, int32_t* emitted, int32_t* keep_lens,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Scatter the new K/V rows of one layer into their paged slots.
  *
  * Replaces PagedSequenceCache.slot_indices + write's index_copy_

@@ -48,6 +48,11 @@ EXPORTS = (
     "kve_small_pass",
     "kve_f32_pass",
     "kve_f32_pass_bytes",
+    "kve_tree_masks",
+    "kve_paged_tree_attn",
+    "kve_tree_accept",
+    "kve_sample_workspace_bytes",
+    "kve_sample_verify",
 )
 
 DTYPE_F32 = 0
@@ -100,6 +105,13 @@ _SIGS = {
                          I, I, I, I, I, P, P, SZ, P, F, P, P]),
     "kve_small_pass": (I, [P, P, I, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, I,
                            I, I, P, P, SZ, P, F, P, I, P]),
+    "kve_tree_masks": (I, [P, P, I, I, P, P, P]),
+    "kve_paged_tree_attn": (I, [P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, I, F, I, P,
+                                P, P, SZ, I, P]),
+    "kve_tree_accept": (I, [P, P, P, P, P, I, P, I, I, P, P, P, P, P, P, P, I, I, I, I, I, I, I, P]),
+    "kve_sample_workspace_bytes": (SZ, [I, I, I, I]),
+    "kve_sample_verify": (I, [P, I64, I64, P, I64, I64, P, P, P, P, F, P, I, P, I, I, I, I, P, P, P,
+                              P, SZ, P]),
 }
 
 

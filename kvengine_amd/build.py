@@ -20,7 +20,7 @@ ARCH = "gfx950"
 
 SOURCES = ["kve_runtime.hip", "kve_attn.hip", "kve_kvcache.hip", "kve_lmhead.hip",
            "kve_layer.hip", "kve_linear.hip", "kve_f32.hip",
-           "kve_pass.hip"]
+           "kve_pass.hip", "kve_tree.hip", "kve_sample.hip"]
 
 # Per-file flags: the fused layer and projection kernels must round every
 # product and sum like the torch ops they replace, so no multiply-add

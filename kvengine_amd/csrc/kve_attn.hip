@@ -56,6 +56,15 @@
 // product of a row of ones with the same hi and lo P^T on the matrix cores
 // instead of VALU adds.
 
+//
+// Trees (TREE, kve_paged_tree_attn): the new tokens are the nodes of a tree of
+// drafts, node t at cache slot start + t, and query t sees the history and those
+// nodes whose bit its mask has. A parent stands before its children, so the keys a
+// query can see end at its own slot as in the causal case: plan, units, loads and
+// folds are the same, and only the tiles that reach the tree test a bit per key
+// (eight keys' bits are one shift of the mask) instead of comparing positions. A
+// chain's masks give the causal kernel's bits.
+
 #include "kve_common.h"
 #include "kve_gemm.h"
 
@@ -89,6 +98,7 @@ struct AttnArgs {
   const int32_t* seq_rows;
   const int32_t* start_pos;
   const int32_t* q_lens;
+  const uint64_t* masks;  // tree launches: [num_seqs][Tq] nodes that each query sees (else null)
   int32_t* plan;   // written by the plan kernel, read by the attention and merge kernels
   float* part_o;   // [slot][Hkv][ROWS][D]: unit states of split items
   float* part_ml;  // [slot][Hkv][ROWS][2]: (max, sum) per row
@@ -506,9 +516,10 @@ __global__ __launch_bounds__(kPlanThreads) void attn_plan_kernel(AttnArgs a) {
 struct UnitInfo {
   int kvh, b, kt0, kt1, pslot, srow, start, R, r, Lk, qlim;
   bool active;  // the wave's row tile has rows below R
+  uint64_t vis;  // trees: bit j set where the row sees the key at start + j
 };
 
-template <int NT>
+template <int NT, bool TREE>
 __device__ __forceinline__ UnitInfo unit_info(const AttnArgs& a, int rec, int u, int nt, int lr) {
   UnitInfo x;
   x.kvh = u % a.Hkv;
@@ -527,7 +538,59 @@ __device__ __forceinline__ UnitInfo unit_info(const AttnArgs& a, int rec, int u,
   const int row_end = min(x.R, row0 + 16 * NT);
   x.Lk = x.start + div_g(row_end - 1, a) + 1;  // keys visible to the row group
   x.qlim = x.r < x.R ? x.start + div_g(x.r, a) : -1;
+  x.vis = 0;
+  if constexpr (TREE) {
+    // bits above the query's own node are no ancestors: the plan's tile count
+    // (keys up to the group's last query) then holds for every tree
+    if (x.r < x.R) {
+      const int t = x.qlim - x.start;
+      x.vis = a.masks[static_cast<size_t>(x.b) * a.Tq + t] & (~0ull >> (63 - t));
+    }
+  }
   return x;
+}
+
+// Trees: which of the n (<= 8) keys from key k0 on a row sees, bit i for key
+// k0 + i: the committed history [0, start) whole, of the tree the nodes in vis.
+__device__ __forceinline__ uint32_t tree_bits(uint64_t vis, int k0, int start) {
+  const int sh = k0 - start;  // the first key's node
+  if (sh >= 0) return sh < 64 ? static_cast<uint32_t>(vis >> sh) : 0u;
+  return sh > -8 ? (static_cast<uint32_t>(vis) << -sh) | ((1u << -sh) - 1u) : 0xffu;
+}
+
+// Trees: a row must not take up an infinity or NaN in the V of a node that it
+// does not see, and the matrix product would make 0 * inf = NaN of it. V is
+// therefore taken without its non-finite values from the pair (32 keys) that
+// holds `start` on, and where a wave dropped any, the rows that see such a key get
+// it added here: p * inf and p * NaN of a p > 0 are the value itself. Never entered
+// while the cache is finite.
+template <int D, bool BF16>
+__device__ __forceinline__ void add_nonfinite(const AttnArgs& a, const UnitInfo& x, int lg,
+                                              f32x4 (&acc)[D / 16]) {
+  using elem_t = std::conditional_t<BF16, uint16_t, float>;
+  const int32_t* table = a.tables + static_cast<size_t>(x.srow) * a.max_blocks;
+  const int first = max(x.kt0 * 16, x.start - 31), end = min(x.Lk, x.kt1 * 16);
+#pragma unroll
+  for (int dt = 0; dt < D / 16; ++dt) {
+    // (one channel group's keys at a time, so that this path takes none of the
+    // registers that the bursts need: keys outermost spilled 140 at D = 128)
+    f32x4 add = {0, 0, 0, 0};
+#pragma unroll 1
+    for (int key = first; key < end; ++key) {
+      const bool sees = key < x.start || (x.vis >> (key - x.start) & 1);
+      const int blk = safe_block(table[key / a.bs], a.num_blocks);
+      const elem_t* vp = static_cast<const elem_t*>(a.v) + key % a.bs +
+                         ((static_cast<size_t>(blk) * a.Hkv + x.kvh) * D + dt * 16 + 4 * lg) * a.bs;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float v;
+        if constexpr (BF16) v = bf16_to_f32(vp[i * a.bs]);
+        else v = vp[i * a.bs];
+        add[i] += sees && (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u ? v : 0.0f;
+      }
+    }
+    acc[dt] += add;
+  }
 }
 
 // End of a unit: the KW key waves' states are folded in wave order through
@@ -536,7 +599,7 @@ __device__ __forceinline__ UnitInfo unit_info(const AttnArgs& a, int rec, int u,
 // rows: the normalised output for an item of one unit, else the unit's state
 // for verify_attn_merge_kernel. Every wave of the workgroup calls it (KW > 1
 // has barriers). Lane (lr, lg) holds O^T[channel dt*16 + 4*lg + i][row lr].
-template <int D, bool BF16, int NT, int KW>
+template <int D, bool BF16, int NT, int KW, bool TREE>
 __device__ __forceinline__ void finish_unit(const AttnArgs& a, const UnitInfo& x, int* sm, int nt,
                                             int kw, int l, float m_run, float lt,
                                             f32x4 (&acc)[D / 16]) {
@@ -572,7 +635,7 @@ __device__ __forceinline__ void finish_unit(const AttnArgs& a, const UnitInfo& x
   if (x.pslot < 0) {
     const int t_out = div_g(x.r, a);
     const int orow = x.b * a.Tq + t_out, ocol = (x.kvh * a.G + x.r - t_out * a.G) * D + 4 * lg;
-    const float inv = 1.0f / lt;
+    const float inv = TREE && lt == 0.0f ? 0.0f : 1.0f / lt;  // a row that sees no key: zeros
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       const f32x4 y = acc[dt] * inv;
@@ -606,7 +669,7 @@ __device__ __forceinline__ void finish_unit(const AttnArgs& a, const UnitInfo& x
 // fold reuses.
 
 // fp32: each key wave loads its bursts into registers (two bursts in flight).
-template <int D, int NT, bool BS16, int KW>
+template <int D, int NT, bool BS16, int KW, bool TREE>
 __global__ __launch_bounds__(64 * NT * KW) void verify_attn_f32_kernel(AttnArgs a) {
   constexpr int NPRE = burst_tiles<D, false>();
   constexpr int DT = D / 16;
@@ -629,7 +692,7 @@ __global__ __launch_bounds__(64 * NT * KW) void verify_attn_f32_kernel(AttnArgs 
   nunits = __builtin_amdgcn_readfirstlane(min(nunits, a.max_units)) * a.Hkv;
   for (int u = blockIdx.x; u < nunits; u += gridDim.x) {
     if (u != static_cast<int>(blockIdx.x)) rec = recs[static_cast<size_t>(u / a.Hkv) * kRecInts + l];
-    const UnitInfo x = unit_info<NT>(a, rec, u, nt, lr);
+    const UnitInfo x = unit_info<NT, TREE>(a, rec, u, nt, lr);
     if (KW == 1 && !x.active) continue;  // (key waves still meet at the fold)
     const int kt0 = x.kt0, kt1 = x.kt1, kvh = x.kvh, start = x.start, Lk = x.Lk, qlim = x.qlim;
     const int32_t* table = a.tables + static_cast<size_t>(x.srow) * a.max_blocks;
@@ -645,6 +708,7 @@ __global__ __launch_bounds__(64 * NT * KW) void verify_attn_f32_kernel(AttnArgs 
     }
 
     float m_run = kNegBig, l_run = 0.0f;
+    bool dropped = false;  // trees: a non-finite V was left out (add_nonfinite)
     f32x4 acc[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0, 0, 0, 0};
@@ -687,13 +751,35 @@ __global__ __launch_bounds__(64 * NT * KW) void verify_attn_f32_kernel(AttnArgs 
           else zero_v(fr[j]);
         }
       }
+      if constexpr (TREE) {
+#pragma unroll
+        for (int j = 0; j < NPRE; ++j) {
+          if (r0 + j >= kt1 || (r0 + j) * 16 + 15 < start) continue;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool inf = (__float_as_uint(fr[j].v[dt][i]) & 0x7f800000u) == 0x7f800000u;
+              dropped |= inf;
+              fr[j].v[dt][i] = inf ? 0.0f : fr[j].v[dt][i];
+            }
+          }
+        }
+      }
       // one online-softmax step over the burst (see verify_attn_bf16_kernel)
       float smax = -INFINITY;
 #pragma unroll
       for (int j = 0; j < NPRE; ++j) {
         const int kt = r0 + j;
         if (kt >= kt1) break;
-        if (kt * 16 + 15 > start) {
+        if constexpr (TREE) {
+          if (kt * 16 + 15 >= start) {
+            const uint32_t bits = tree_bits(x.vis, kt * 16 + 4 * lg, start);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (!(bits >> i & 1)) sc[j][i] = -INFINITY;
+          }
+        } else if (kt * 16 + 15 > start) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (kt * 16 + 4 * lg + i > qlim) sc[j][i] = -INFINITY;
@@ -740,7 +826,10 @@ __global__ __launch_bounds__(64 * NT * KW) void verify_attn_f32_kernel(AttnArgs 
         consume(fb, r0 + BSTEP);
       }
     }
-    finish_unit<D, false, NT, KW>(a, x, sm_dyn, nt, kw, l, m_run, sum_across_groups(l_run), acc);
+    if constexpr (TREE) {
+      if (__any(dropped)) add_nonfinite<D, false>(a, x, lg, acc);
+    }
+    finish_unit<D, false, NT, KW, TREE>(a, x, sm_dyn, nt, kw, l, m_run, sum_across_groups(l_run), acc);
   }
 }
 
@@ -755,7 +844,7 @@ __global__ __launch_bounds__(64 * NT * KW) void verify_attn_f32_kernel(AttnArgs 
 // two such workgroups share a CU only at four waves per SIMD (measured: at
 // 151 registers the second one waited for the first to finish). The register
 // path keeps two bursts in registers and takes what it needs.
-template <int D, int NT, bool BS16, int KW>
+template <int D, int NT, bool BS16, int KW, bool TREE>
 __global__ __launch_bounds__(64 * NT * KW)
 __attribute__((amdgpu_waves_per_eu(NT >= 2 && NT * KW <= 6 ? 4 : 1))) void verify_attn_bf16_kernel(AttnArgs a) {
   constexpr int NPRE = burst_tiles<D, true>();
@@ -789,7 +878,7 @@ __attribute__((amdgpu_waves_per_eu(NT >= 2 && NT * KW <= 6 ? 4 : 1))) void verif
   nunits = __builtin_amdgcn_readfirstlane(min(nunits, a.max_units)) * a.Hkv;
   for (int u = blockIdx.x; u < nunits; u += gridDim.x) {
     if (u != static_cast<int>(blockIdx.x)) rec = recs[static_cast<size_t>(u / a.Hkv) * kRecInts + l];
-    const UnitInfo x = unit_info<NT>(a, rec, u, nt, lr);
+    const UnitInfo x = unit_info<NT, TREE>(a, rec, u, nt, lr);
     // A row tile wholly past q_len has nothing to compute; with K/V staged in
     // LDS the wave still takes its share of the loads and barriers.
     if (!DMAKV && KW == 1 && !x.active) continue;  // (key waves still meet at the fold)
@@ -798,7 +887,8 @@ __attribute__((amdgpu_waves_per_eu(NT >= 2 && NT * KW <= 6 ? 4 : 1))) void verif
     const int klim = min(x.qlim, kt1 * 16 - 1);
     // a pair whose last key passes `edge` needs the mask (wave-uniform test;
     // every real row sees keys up to start)
-    const int edge = min(x.start, kt1 * 16 - 1);
+    // (trees: the history is seen whole, every pair that reaches the tree is tested)
+    const int edge = min(TREE ? x.start - 1 : x.start, kt1 * 16 - 1);
     // V keys from vlim on are zeroed: stale slots past the history, tiles past the unit
     const int vlim = min(x.Lk, kt1 * 16);
     const int32_t* table = a.tables + static_cast<size_t>(x.srow) * a.max_blocks;
@@ -815,6 +905,7 @@ __attribute__((amdgpu_waves_per_eu(NT >= 2 && NT * KW <= 6 ? 4 : 1))) void verif
     }
 
     float m_run = kNegBig;
+    bool dropped = false;  // trees: a non-finite V was left out (add_nonfinite)
     f32x4 acc[DT], lsum = {0, 0, 0, 0};  // every lane of a row holds its row's sum
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0, 0, 0, 0};
@@ -848,11 +939,13 @@ __attribute__((amdgpu_waves_per_eu(NT >= 2 && NT * KW <= 6 ? 4 : 1))) void verif
       for (int p = 0; p < NP; ++p) {
         const int kt = r0 + 2 * p;
         if (kt * 16 + 31 > edge) {
+          const int k0 = kt * 16 + 8 * lg;
+          const uint32_t bits = TREE && k0 < kt1 * 16 ? tree_bits(x.vis, k0, x.start) : 0u;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (kt * 16 + 8 * lg + 4 * h + i > klim) sc[p][h][i] = -INFINITY;
+              if (TREE ? !(bits >> (4 * h + i) & 1) : k0 + 4 * h + i > klim) sc[p][h][i] = -INFINITY;
           }
         }
       }
@@ -912,6 +1005,16 @@ __attribute__((amdgpu_waves_per_eu(NT >= 2 && NT * KW <= 6 ? 4 : 1))) void verif
         for (int dt = 0; dt < DT; ++dt) {
           u32x4 v = vget(p, dt);
           if (vz) v &= keep;
+          if constexpr (TREE) {
+            if ((r0 + 2 * p) * 16 + 31 >= x.start) {
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                const bool lo = (v[w] & 0x7f80u) == 0x7f80u, hi = (v[w] & 0x7f800000u) == 0x7f800000u;
+                dropped |= lo || hi;
+                v[w] &= (lo ? 0xffff0000u : ~0u) & (hi ? 0x0000ffffu : ~0u);
+              }
+            }
+          }
           acc[dt] = mfma16x16x32_bf16(v, ph, acc[dt]);
           acc[dt] = mfma16x16x32_bf16(v, pl, acc[dt]);
         }
@@ -1131,7 +1234,10 @@ __attribute__((amdgpu_waves_per_eu(NT >= 2 && NT * KW <= 6 ? 4 : 1))) void verif
       }
       barrier_after_vm<0>();  // the buffers are rewritten by the fold or the next unit
     }
-    finish_unit<D, true, NT, KW>(a, x, sm_dyn, nt, kw, l, m_run, lsum[0], acc);
+    if constexpr (TREE) {
+      if (__any(dropped)) add_nonfinite<D, true>(a, x, lg, acc);
+    }
+    finish_unit<D, true, NT, KW, TREE>(a, x, sm_dyn, nt, kw, l, m_run, lsum[0], acc);
   }
 }
 
@@ -1201,7 +1307,7 @@ __global__ __launch_bounds__(64 * NT) void verify_attn_merge_kernel(AttnArgs a) 
       x[0] = live ? x2[0] : x[0];
     }
   }
-  const float inv = 1.0f / L;
+  const float inv = a.masks && L == 0.0f ? 0.0f : 1.0f / L;  // (a tree row that sees no key)
   const f32x4 y = x[0] * inv;
   const int r = row0 + rr;
   const int t = div_g(r, a), h = kvh * a.G + r - t * a.G;
@@ -1398,7 +1504,7 @@ static int merge_batch(long long workgroups, int max_item_units) {
   return max_item_units <= 10 ? 4 : 8;
 }
 
-template <int D, bool BF16, int NT, int KW>
+template <int D, bool BF16, int NT, int KW, bool TREE>
 static int launch_attn_t(const AttnArgs& a, const AttnCfg& p, hipStream_t st, bool bs16) {
   auto go = [&](auto kernel) {
     const int rc = grant_lds(kernel, p.lds, "kve_paged_verify_attn");
@@ -1411,11 +1517,11 @@ static int launch_attn_t(const AttnArgs& a, const AttnCfg& p, hipStream_t st, bo
   };
   int rc;
   if constexpr (BF16)
-    rc = bs16 ? go(verify_attn_bf16_kernel<D, NT, true, KW>)
-              : go(verify_attn_bf16_kernel<D, NT, false, KW>);
+    rc = bs16 ? go(verify_attn_bf16_kernel<D, NT, true, KW, TREE>)
+              : go(verify_attn_bf16_kernel<D, NT, false, KW, TREE>);
   else
-    rc = bs16 ? go(verify_attn_f32_kernel<D, NT, true, KW>)
-              : go(verify_attn_f32_kernel<D, NT, false, KW>);
+    rc = bs16 ? go(verify_attn_f32_kernel<D, NT, true, KW, TREE>)
+              : go(verify_attn_f32_kernel<D, NT, false, KW, TREE>);
   if (rc) return rc;
   // histories longer than one unit: merge their units' states (only launched
   // when max_ctx allows more than one unit per history)
@@ -1432,11 +1538,11 @@ static int launch_attn_t(const AttnArgs& a, const AttnCfg& p, hipStream_t st, bo
 
 // Instantiated (row tiles, key waves): (1, 1), (1, 2), (1, 4), (1, 8), (2-4, 1),
 // (2-4, 2), (2-3, 4), (6, 1), (6, 2), (8, 1).
-template <int D, bool BF16>
+template <int D, bool BF16, bool TREE>
 static int launch_attn_nt(const AttnArgs& a, const AttnCfg& p, hipStream_t st, bool bs16) {
   const int NT = p.NT, KW = p.KW;
 #define KVE_ATTN_CASE(nt, kw) \
-  if (NT == nt && KW == kw) return launch_attn_t<D, BF16, nt, kw>(a, p, st, bs16);
+  if (NT == nt && KW == kw) return launch_attn_t<D, BF16, nt, kw, TREE>(a, p, st, bs16);
   KVE_ATTN_CASE(1, 8)
   KVE_ATTN_CASE(1, 4)
   KVE_ATTN_CASE(1, 2)
@@ -1572,33 +1678,31 @@ extern "C" int kve_attn_plan(const int32_t* block_tables, const int32_t* seq_row
   return check_launch("kve_attn_plan");
 }
 
-extern "C" int kve_paged_verify_attn(const void* q, const void* k_pool, const void* v_pool,
-                                     const int32_t* block_tables, const int32_t* seq_rows,
-                                     const int32_t* start_pos, const int32_t* q_lens, int num_seqs,
-                                     int q_len, int num_q_heads, int num_kv_heads, int head_dim,
-                                     int block_size, int max_blocks, int num_rows, int num_blocks,
-                                     int max_ctx, int unit_blocks, int key_waves, float scale,
-                                     int dtype, const void* plan, void* out, void* workspace,
-                                     size_t workspace_bytes, int layout, void* stream) {
-  clear_error();
-  if (num_seqs == 0) return KVE_OK;
-  KVE_REQUIRE(q && k_pool && v_pool && out, "kve_paged_verify_attn: null pointer argument");
+// The attention launches of a pass's layer; masks: a tree launch's (else null).
+static int paged_attn(const char* name, const uint64_t* masks, const void* q, const void* k_pool,
+                      const void* v_pool, const int32_t* block_tables, const int32_t* seq_rows,
+                      const int32_t* start_pos, const int32_t* q_lens, int num_seqs, int q_len,
+                      int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                      int max_blocks, int num_rows, int num_blocks, int max_ctx, int unit_blocks,
+                      int key_waves, float scale, int dtype, const void* plan, void* out,
+                      void* workspace, size_t workspace_bytes, int layout, void* stream) {
+  KVE_REQUIRE(q && k_pool && v_pool && out, "%s: null pointer argument", name);
   KVE_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) |
                 reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) &
                15) == 0,
-              "kve_paged_verify_attn: q, out, k_pool and v_pool must be 16-byte aligned");
+              "%s: q, out, k_pool and v_pool must be 16-byte aligned", name);
   AttnArgs a{};
   AttnCfg p;
-  int rc = attn_setup(a, p, "kve_paged_verify_attn", block_tables, seq_rows, start_pos, q_lens,
+  int rc = attn_setup(a, p, name, block_tables, seq_rows, start_pos, q_lens,
                       num_seqs, q_len, num_q_heads, num_kv_heads, head_dim, block_size, max_blocks,
                       num_rows, num_blocks, max_ctx, unit_blocks, key_waves, dtype);
   if (rc) return rc;
   const size_t need = attn_ws_bytes(p, plan == nullptr);
   if (need) {
     KVE_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
-                "kve_paged_verify_attn: workspace required (256-byte aligned)");
+                "%s: workspace required (256-byte aligned)", name);
     if (workspace_bytes < need) {
-      set_error("kve_paged_verify_attn: workspace %zu bytes, need %zu", workspace_bytes, need);
+      set_error("%s: workspace %zu bytes, need %zu", name, workspace_bytes, need);
       return KVE_EWORKSPACE;
     }
   }
@@ -1611,7 +1715,7 @@ extern "C" int kve_paged_verify_attn(const void* q, const void* k_pool, const vo
     if (rc) return rc;
   } else {
     KVE_REQUIRE((reinterpret_cast<uintptr_t>(plan) & 15) == 0,
-                "kve_paged_verify_attn: plan must be 16-byte aligned");
+                "%s: plan must be 16-byte aligned", name);
     a.plan = static_cast<int32_t*>(const_cast<void*>(plan));
   }
   a.part_ml = p.max_split ? reinterpret_cast<float*>(ws) : nullptr;
@@ -1622,18 +1726,60 @@ extern "C" int kve_paged_verify_attn(const void* q, const void* k_pool, const vo
   KVE_REQUIRE(layout == KVE_LAYOUT_ROWS ||
                   (layout == KVE_LAYOUT_BLOCKED && dtype == KVE_DTYPE_BF16 &&
                    (num_q_heads * head_dim) % 32 == 0),
-              "kve_paged_verify_attn: layout %d with dtype %d", layout, dtype);
+              "%s: layout %d with dtype %d", name, layout, dtype);
   a.out = out;
   a.out_blocked = layout == KVE_LAYOUT_BLOCKED ? 1 : 0;
   a.scale_log2 = scale * 1.4426950408889634f;
+  a.masks = masks;
   const bool bs16 = block_size == 16;
-  if (dtype == KVE_DTYPE_BF16) {
-    rc = head_dim == 64 ? launch_attn_nt<64, true>(a, p, st, bs16)
-                        : launch_attn_nt<128, true>(a, p, st, bs16);
-  } else {
-    rc = head_dim == 64 ? launch_attn_nt<64, false>(a, p, st, bs16)
-                        : launch_attn_nt<128, false>(a, p, st, bs16);
-  }
+  const auto launch = [&](auto bf16, auto tree) {
+    constexpr bool BF16 = decltype(bf16)::value, TREE = decltype(tree)::value;
+    return head_dim == 64 ? launch_attn_nt<64, BF16, TREE>(a, p, st, bs16)
+                          : launch_attn_nt<128, BF16, TREE>(a, p, st, bs16);
+  };
+  const std::true_type yes{};
+  const std::false_type no{};
+  if (dtype == KVE_DTYPE_BF16) rc = masks ? launch(yes, yes) : launch(yes, no);
+  else rc = masks ? launch(no, yes) : launch(no, no);
   if (rc) return rc;
-  return check_launch("kve_paged_verify_attn");
+  return check_launch(name);
+}
+
+extern "C" int kve_paged_verify_attn(const void* q, const void* k_pool, const void* v_pool,
+                                     const int32_t* block_tables, const int32_t* seq_rows,
+                                     const int32_t* start_pos, const int32_t* q_lens, int num_seqs,
+                                     int q_len, int num_q_heads, int num_kv_heads, int head_dim,
+                                     int block_size, int max_blocks, int num_rows, int num_blocks,
+                                     int max_ctx, int unit_blocks, int key_waves, float scale,
+                                     int dtype, const void* plan, void* out, void* workspace,
+                                     size_t workspace_bytes, int layout, void* stream) {
+  clear_error();
+  if (num_seqs == 0) return KVE_OK;
+  return paged_attn("kve_paged_verify_attn", nullptr, q, k_pool, v_pool, block_tables, seq_rows,
+                    start_pos, q_lens, num_seqs, q_len, num_q_heads, num_kv_heads, head_dim,
+                    block_size, max_blocks, num_rows, num_blocks, max_ctx, unit_blocks, key_waves,
+                    scale, dtype, plan, out, workspace, workspace_bytes, layout, stream);
+}
+
+extern "C" int kve_paged_tree_attn(const void* q, const void* k_pool, const void* v_pool,
+                                   const int64_t* masks, const int32_t* block_tables,
+                                   const int32_t* seq_rows, const int32_t* start_pos,
+                                   const int32_t* q_lens, int num_seqs, int q_len, int num_q_heads,
+                                   int num_kv_heads, int head_dim, int block_size, int max_blocks,
+                                   int num_rows, int num_blocks, int max_ctx, int unit_blocks,
+                                   int key_waves, float scale, int dtype, const void* plan,
+                                   void* out, void* workspace, size_t workspace_bytes, int layout,
+                                   void* stream) {
+  clear_error();
+  if (num_seqs == 0) return KVE_OK;
+  KVE_REQUIRE(masks && (reinterpret_cast<uintptr_t>(masks) & 7) == 0,
+              "kve_paged_tree_attn: masks must be an 8-byte aligned buffer");
+  KVE_REQUIRE(q_len <= KVE_TREE_MAX_NODES, "kve_paged_tree_attn: %d nodes, at most %d", q_len,
+              KVE_TREE_MAX_NODES);
+  KVE_REQUIRE(scale > 0.0f, "kve_paged_tree_attn: scale %g", static_cast<double>(scale));
+  return paged_attn("kve_paged_tree_attn", reinterpret_cast<const uint64_t*>(masks), q, k_pool,
+                    v_pool, block_tables, seq_rows, start_pos, q_lens, num_seqs, q_len, num_q_heads,
+                    num_kv_heads, head_dim, block_size, max_blocks, num_rows, num_blocks, max_ctx,
+                    unit_blocks, key_waves, scale, dtype, plan, out, workspace, workspace_bytes,
+                    layout, stream);
 }

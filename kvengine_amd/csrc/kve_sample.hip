@@ -1,0 +1,681 @@
+// Verification of drafted tokens by rejection sampling from given uniform numbers
+// (kve_sample_verify; the sampled counterpart of the greedy accept of
+// kvengine/speculative.py:169-197).
+//
+// The mathematics. p = softmax(target / T), q = softmax(draft / T) at each drafted
+// position; draft x stands while u q(x) < p(x). At the first that falls the token is
+// drawn from r = max(p - q, 0), else, after the last draft, from p, by inversion: the
+// lowest id whose running sum exceeds u * sum(r).
+//
+// Everything is in 64 bits. The drawn id is a place among up to 150 000 running sums,
+// and an error of e in the sums moves a draw with a probability of about 2 V e: 32-bit
+// exponentials (6e-8) would answer one or two draws in a hundred differently from the
+// definition, 64-bit ones none. A 64-bit FMA costs a wave the same four cycles here as
+// an unpacked 32-bit one, so the price is the polynomial's length.
+//
+// Launches, each a dependency of the next over the whole vocabulary:
+//  stats   every (row, chunk): maximum and sum of 2^((l - max) c), c = log2(e) / T,
+//          the chunk held in registers between the two
+//  rest    every (sequence, chunk), where drafts have probabilities: the rows' chunks
+//          joined, the accept tests, and the chunk's sum of r at the deciding position
+//          (one row of each side, again)
+//  pick    every sequence: the chunk that holds the drawn place, then its elements
+// The stats launch reads all logits once and bounds the call; the others re-read one
+// position's rows, or one chunk.
+
+#include "kve_common.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace kve {
+
+// The deciding position of a sequence: r = 2^((l - mp) c) of the target alone (both
+// false; `skip`, a rejected draft of no distribution, left out) or max(p - q, 0).
+struct SamplePick {
+  double ip, iq;  // 1 / sum over the row, of the target and the draft
+  float mp, mq;   // row maxima
+  int n_acc, skip;  // skip: id left out, or -1
+};
+
+struct SampleArgs {
+  const void *target, *draft;
+  int64_t ts, tp, ds, dp;  // element strides per sequence and position
+  const int32_t* drafts;
+  const float *u_accept, *u_sample, *temps;
+  float temp;
+  const int32_t *lens, *seq_rows;
+  int num_rows, B, k, V, rows, chunks;  // rows per sequence: k + 1 target, then k draft
+  int32_t *n_acc, *emitted, *keep;
+  double* sums;   // [B][rows][chunks]: sum of the chunk relative to its maximum
+  float* maxes;   // [B][rows][chunks]
+  double* rest;   // [B][chunks]: sum of r over the chunk
+  SamplePick* picks;  // [B]
+};
+
+constexpr int kStatThreads = 256;
+constexpr int kPickThreads = 1024;
+
+// log2(e) / T, or 0 where T is not positive and finite (the sequence has no answer)
+__device__ __forceinline__ double sample_rate(const SampleArgs& a, int b) {
+  const float t = a.temps ? a.temps[b] : a.temp;
+  return t > 0.0f && t < INFINITY ? 1.4426950408889634074 / static_cast<double>(t) : 0.0;
+}
+
+// 2^y = 2^n 2^f with n = round(y), f = y - n: the polynomial of degree 10 that meets 2^f
+// at the eleven Chebyshev points of [-1/2, 1/2], within 3e-16 of it; 2^0 is 1 exactly, so
+// that equal logits give exactly equal sums.
+__device__ __forceinline__ double exp2_poly(double f) {
+  double p = 7.072585949269223e-09;
+  p = fma(p, f, 1.0208690299958306e-07);
+  p = fma(p, f, 1.321544258792169e-06);
+  p = fma(p, f, 1.5252657260200837e-05);
+  p = fma(p, f, 0.0001540353044173605);
+  p = fma(p, f, 0.0013333558230164974);
+  p = fma(p, f, 0.009618129107606888);
+  p = fma(p, f, 0.05550410866444772);
+  p = fma(p, f, 0.24022650695910097);
+  p = fma(p, f, 0.69314718055995);
+  return fma(p, f, 1.0);
+}
+
+// The weight 2^((l - m) c) of a logit against a maximum m (center() of it), for every
+// value: 0 where it underflows and at -inf, NaN where l or m is NaN or m is +inf.
+__device__ __forceinline__ double weight(float l, double m, double rate) {
+  // the product rounded on its own: an exponent far below any is then a whole number,
+  // where a fused y - round(y) would be the product's rounding error, which may be large
+#pragma clang fp contract(off)
+  const double y = (static_cast<double>(l) - m) * rate;
+  const double n = __builtin_rint(y);
+  const double w = __builtin_amdgcn_ldexp(exp2_poly(y - n), static_cast<int>(fmax(n, -4096.0)));
+  return l == -INFINITY ? 0.0 : w;
+}
+
+// The same bits where (l - m) c is known to lie in [-1000, 0]: the rounding and the
+// power of two by adding 1.5 * 2^52, whose low word then holds n, in place of the
+// slower rounding, conversion and scaling instructions.
+__device__ __forceinline__ double weight_near(float l, double m, double rate) {
+#pragma clang fp contract(off)
+  constexpr double kShift = 6755399441055744.0;
+  const double y = (static_cast<double>(l) - m) * rate;
+  const double t = y + kShift;
+  const uint64_t p = __builtin_bit_cast(uint64_t, exp2_poly(y - (t - kShift)));
+  const uint32_t n = static_cast<uint32_t>(__builtin_bit_cast(uint64_t, t));
+  return __builtin_bit_cast(double, p + (static_cast<uint64_t>(n << 20) << 32));
+}
+constexpr double kNear = -1000.0;
+
+// What weights are taken against: a maximum of -inf (no mass) counts as 0.
+__device__ __forceinline__ double center(float m) {
+  return m == -INFINITY ? 0.0 : static_cast<double>(m);
+}
+
+// (v_maximum / v_minimum: a NaN stays, so that it reaches the sums)
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float min_nan(float a, float b) { return __builtin_elementwise_minimum(a, b); }
+
+// over the 16 lanes of a row
+__device__ __forceinline__ float row_max(float v) {
+  v = max_nan(v, dpp_mov<0xB1>(v));
+  v = max_nan(v, dpp_mov<0x4E>(v));
+  v = max_nan(v, dpp_mov<0x141>(v));
+  return max_nan(v, dpp_mov<0x140>(v));
+}
+__device__ __forceinline__ double row_sum(double v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+  v = row_max(v);
+  const uint32_t u = __float_as_uint(v);
+  const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  v = max_nan(__uint_as_float(h[0]), __uint_as_float(h[1]));
+  const uint32_t w = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+  return max_nan(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ double wave_sum64(double v) {
+  v = row_sum(v);
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+template <typename E>
+__device__ __forceinline__ float to_f32(E v) {
+  if constexpr (std::is_same_v<E, float>) return v;
+  else return bf16_to_f32(v);
+}
+
+template <typename E>
+constexpr int kVec = 16 / sizeof(E);
+
+// A 16-byte vector of logits from element i0 on, of a row of V; those past the end are
+// -inf. Rows may start at any element (an odd vocabulary): gfx950 reads vectors at the
+// type's alignment.
+template <typename E>
+__device__ __forceinline__ void load_logits(const E* row, int i0, int V, float (&x)[kVec<E>]) {
+  constexpr int N = kVec<E>;
+  struct __attribute__((packed, aligned(sizeof(E)))) Vec { E v[N]; };
+  if (i0 + N <= V) {
+    const Vec t = *reinterpret_cast<const Vec*>(row + i0);
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = to_f32(t.v[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = i0 + e < V ? to_f32(row[i0 + e]) : -INFINITY;
+  }
+}
+
+template <typename E>
+__device__ __forceinline__ const E* logits_row(const SampleArgs& a, int b, int r) {
+  return r <= a.k ? static_cast<const E*>(a.target) + b * a.ts + r * a.tp
+                  : static_cast<const E*>(a.draft) + b * a.ds + (r - a.k - 1) * a.dp;
+}
+
+// Grid: sequences x rows x chunks, chunks fastest. NV 16-byte vectors a thread.
+template <typename E, int NV>
+__global__ __launch_bounds__(kStatThreads) void sample_stats_kernel(SampleArgs a) {
+  constexpr int N = kVec<E>;
+  __shared__ float sm_max[kStatThreads / 64];
+  __shared__ double sm_sum[kStatThreads / 64];
+  const int tid = threadIdx.x, w = tid >> 6;
+  const int br = blockIdx.x / a.chunks, ch = blockIdx.x - br * a.chunks;
+  const int b = br / a.rows, r = br - b * a.rows;
+  const E* row = logits_row<E>(a, b, r);
+  const double rate = sample_rate(a, b);
+  float x[NV][N];
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+    load_logits<E>(row, (ch * NV + v) * kStatThreads * N + tid * N, a.V, x[v]);
+  float m = x[0][0], lo = x[0][0];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      m = max_nan(m, x[v][e]);
+      lo = min_nan(lo, x[v][e]);
+    }
+  }
+  m = wave_max(m);
+  if ((tid & 63) == 0) sm_max[w] = m;
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < kStatThreads / 64; ++q) m = max_nan(m, sm_max[q]);
+  const double c = center(m);
+  double s = 0.0;
+  if (__all((static_cast<double>(lo) - c) * rate >= kNear)) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) s += weight_near(x[v][e], c, rate);
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) s += weight(x[v][e], c, rate);
+    }
+  }
+  s = wave_sum64(s);
+  if ((tid & 63) == 0) sm_sum[w] = s;
+  __syncthreads();
+  if (tid == 0) {
+    for (int q = 1; q < kStatThreads / 64; ++q) s += sm_sum[q];
+    a.maxes[blockIdx.x] = m;
+    a.sums[blockIdx.x] = s;
+  }
+}
+
+// A chunk's sum against its row's maximum (center mc) instead of its own. A chunk of no
+// mass holds 0, one with a NaN in it that.
+__device__ __forceinline__ double chunk_sum(double s, float m, double mc, double rate) {
+  return m == -INFINITY ? s : s * weight(m, mc, rate);
+}
+
+// The deciding position of sequence b, by a whole workgroup: every row's chunks joined
+// (16 lanes a row), then the drafts' tests; the lowest that fails decides. sm: rows
+// doubles, then rows floats.
+template <typename E, int THREADS>
+__device__ __forceinline__ SamplePick decide(const SampleArgs& a, int b, double rate, double* sm_s,
+                                             int* sm_acc) {
+  float* sm_m = reinterpret_cast<float*>(sm_s + a.rows);
+  const int tid = threadIdx.x, l16 = tid & 15;
+  const auto test = [&](int j, int x, float lp, float lq, float u) {
+    bool ok = false;
+    if (x >= 0 && x < a.V) {
+      const double p = weight(lp, center(sm_m[j]), rate) / sm_s[j];
+      const int r = a.k + 1 + j;
+      const double q = a.draft ? weight(lq, center(sm_m[r]), rate) / sm_s[r] : 1.0;
+      ok = static_cast<double>(u) * q < p;
+    }
+    if (!ok) atomicMin(sm_acc, j);
+  };
+  const auto fetch = [&](int j, int& x, float& lp, float& lq, float& u) {
+    x = a.drafts[static_cast<size_t>(b) * a.k + j];
+    u = a.u_accept[static_cast<size_t>(b) * a.k + j];
+    lp = lq = 0.0f;
+    if (x >= 0 && x < a.V) {
+      lp = to_f32(logits_row<E>(a, b, j)[x]);
+      if (a.draft) lq = to_f32(logits_row<E>(a, b, a.k + 1 + j)[x]);
+    }
+  };
+  // (asked for before the statistics arrive)
+  int x0 = -1;
+  float lp0 = 0, lq0 = 0, u0 = 0;
+  if (tid < a.k) fetch(tid, x0, lp0, lq0, u0);
+  if (tid == 0) *sm_acc = a.k;
+  for (int r = tid >> 4; r < a.rows; r += THREADS / 16) {
+    const size_t at = (static_cast<size_t>(b) * a.rows + r) * a.chunks;
+    // the first chunks of the lanes stay in registers: 32 chunks are a vocabulary of
+    // 262144 at full chunk size
+    constexpr int KEEP = 2;
+    float m[KEEP], M = -INFINITY;
+    double s[KEEP], S = 0.0;
+#pragma unroll
+    for (int q = 0; q < KEEP; ++q) {
+      const int c = q * 16 + l16;
+      m[q] = c < a.chunks ? a.maxes[at + c] : -INFINITY;
+      s[q] = c < a.chunks ? a.sums[at + c] : 0.0;
+      M = max_nan(M, m[q]);
+    }
+    for (int c = KEEP * 16 + l16; c < a.chunks; c += 16) M = max_nan(M, a.maxes[at + c]);
+    M = row_max(M);
+    const double mc = center(M);
+#pragma unroll
+    for (int q = 0; q < KEEP; ++q) S += chunk_sum(s[q], m[q], mc, rate);
+    for (int c = KEEP * 16 + l16; c < a.chunks; c += 16)
+      S += chunk_sum(a.sums[at + c], a.maxes[at + c], mc, rate);
+    S = row_sum(S);
+    if (l16 == 0) {
+      sm_s[r] = S;
+      sm_m[r] = M;
+    }
+  }
+  __syncthreads();
+  if (tid < a.k) test(tid, x0, lp0, lq0, u0);
+  for (int j = tid + THREADS; j < a.k; j += THREADS) {
+    fetch(j, x0, lp0, lq0, u0);
+    test(j, x0, lp0, lq0, u0);
+  }
+  __syncthreads();
+  const int j = rate > 0.0 ? *sm_acc : 0;
+  const bool both = a.draft && j < a.k;
+  SamplePick p;
+  p.n_acc = j;
+  p.mp = sm_m[j];
+  p.ip = 1.0 / sm_s[j];
+  p.mq = both ? sm_m[a.k + 1 + j] : 0.0f;
+  p.iq = both ? 1.0 / sm_s[a.k + 1 + j] : 0.0;
+  p.skip = !a.draft && j < a.k ? a.drafts[static_cast<size_t>(b) * a.k + j] : -1;
+  return p;
+}
+
+// r of the N ids from i0 on at the deciding position; ids past the vocabulary have 0.
+template <typename E>
+__device__ __forceinline__ void rest_weights(const SampleArgs& a, const SamplePick& p, bool both,
+                                             const float (&lp)[kVec<E>], const float (&lq)[kVec<E>],
+                                             int i0, double rate, double (&r)[kVec<E>]) {
+  // both products rounded, so that equal probabilities leave exactly nothing
+#pragma clang fp contract(off)
+  const double mp = center(p.mp), mq = center(p.mq);
+#pragma unroll
+  for (int e = 0; e < kVec<E>; ++e) {
+    const double w = weight(lp[e], mp, rate);
+    if (both) {
+      const double d = w * p.ip - weight(lq[e], mq, rate) * p.iq;
+      r[e] = d > 0.0 ? d : 0.0 * d;  // (a NaN stays)
+    } else {
+      r[e] = i0 + e == p.skip ? 0.0 : w;
+    }
+    // past the end both logits are -inf; 0 * (1 / sum) of a row without mass is not 0
+    if (i0 + e >= a.V) r[e] = 0.0;
+  }
+}
+
+// Grid: sequences x chunks, chunks fastest (drafts with probabilities only).
+template <typename E, int NV>
+__global__ __launch_bounds__(kStatThreads) void sample_rest_kernel(SampleArgs a) {
+  constexpr int N = kVec<E>;
+  extern __shared__ double sm_rows[];
+  __shared__ double sm_sum[kStatThreads / 64];
+  __shared__ int sm_acc;
+  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63;
+  const int b = blockIdx.x / a.chunks, ch = blockIdx.x - b * a.chunks;
+  const double rate = sample_rate(a, b);
+  const SamplePick p = decide<E, kStatThreads>(a, b, rate, sm_rows, &sm_acc);
+  const bool both = p.n_acc < a.k;
+  if (!both) {
+    // every draft stands: the chunk's sum is what the stats launch left
+    if (tid == 0) {
+      const size_t at = (static_cast<size_t>(b) * a.rows + a.k) * a.chunks + ch;
+      a.rest[blockIdx.x] = chunk_sum(a.sums[at], a.maxes[at], center(p.mp), rate);
+      if (ch == 0) a.picks[b] = p;
+    }
+    return;
+  }
+  const E* tr = logits_row<E>(a, b, p.n_acc);
+  const E* dr = logits_row<E>(a, b, a.k + 1 + p.n_acc);
+  float x[NV][N], y[NV][N];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int i0 = (ch * NV + v) * kStatThreads * N + tid * N;
+    load_logits<E>(tr, i0, a.V, x[v]);
+    load_logits<E>(dr, i0, a.V, y[v]);
+  }
+  double s = 0.0;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    double r[N];
+    rest_weights<E>(a, p, true, x[v], y[v], (ch * NV + v) * kStatThreads * N + tid * N, rate, r);
+#pragma unroll
+    for (int e = 0; e < N; ++e) s += r[e];
+  }
+  s = wave_sum64(s);
+  if (l == 0) sm_sum[w] = s;
+  __syncthreads();
+  if (tid == 0) {
+    for (int q = 1; q < kStatThreads / 64; ++q) s += sm_sum[q];
+    a.rest[blockIdx.x] = s;
+    if (ch == 0) a.picks[b] = p;
+  }
+}
+
+// Exclusive prefix of a value over the workgroup's threads, and the total.
+template <int THREADS>
+__device__ __forceinline__ double block_prefix(double v, double* sm, int tid, double& total) {
+  const int l = tid & 63, w = tid >> 6;
+  double inc = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double up = __shfl_up(inc, o);
+    if (l >= o) inc += up;
+  }
+  if (l == 63) sm[w] = inc;
+  __syncthreads();
+  double before = 0.0;
+  total = 0.0;
+#pragma unroll
+  for (int q = 0; q < THREADS / 64; ++q) {
+    if (q == w) before = total;
+    total += sm[q];
+  }
+  __syncthreads();
+  return before + inc - v;
+}
+
+// Grid: sequences. A chunk is `per` ids.
+template <typename E>
+__global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a, int per) {
+  constexpr int N = kVec<E>, T = kPickThreads;
+  extern __shared__ double sm_rows[];
+  __shared__ double sm[T / 64], sm_ahead, sm_skip;
+  __shared__ int sm_acc, sm_at, sm_last;
+  const int tid = threadIdx.x, b = blockIdx.x;
+  const double rate = sample_rate(a, b);
+  SamplePick p = a.draft ? a.picks[b] : decide<E, T>(a, b, rate, sm_rows, &sm_acc);
+  bool both = a.draft && p.n_acc < a.k;
+  const double u = a.u_sample[b];
+  const size_t prow = (static_cast<size_t>(b) * a.rows + p.n_acc) * a.chunks;
+  const E* tr = logits_row<E>(a, b, p.n_acc);
+  const E* dr = both ? logits_row<E>(a, b, a.k + 1 + p.n_acc) : tr;
+  const double mc = center(p.mp);
+
+  // the chunk that an id left out lies in is summed again without it (taking its weight
+  // off the sum would leave that sum's rounding error, of any size against the rest)
+  const bool skips = p.skip >= 0 && p.skip < a.V;
+  const int skip_chunk = skips ? p.skip / per : -1;
+  if (skips) {
+    double s = 0.0, all;
+    for (int i0 = skip_chunk * per + tid * N; i0 < min((skip_chunk + 1) * per, a.V); i0 += T * N) {
+      float x[N];
+      double r[N];
+      load_logits<E>(tr, i0, a.V, x);
+      rest_weights<E>(a, p, false, x, x, i0, rate, r);
+#pragma unroll
+      for (int e = 0; e < N; ++e) s += r[e];
+    }
+    block_prefix<T>(s, sm, tid, all);
+    if (tid == 0) sm_skip = all;
+    __syncthreads();
+  }
+  // plain: p itself, where p - q or p without the draft leaves nothing
+  const auto sum_of = [&](int c, bool plain) {
+    if (c >= a.chunks) return 0.0;
+    if (both && !plain) return a.rest[static_cast<size_t>(b) * a.chunks + c];
+    if (c == skip_chunk && !plain) return sm_skip;
+    return chunk_sum(a.sums[prow + c], a.maxes[prow + c], mc, rate);
+  };
+  const auto total_of = [&](bool plain) {
+    double t = 0.0, all;
+    for (int c = tid; c < a.chunks; c += T) t += sum_of(c, plain);
+    block_prefix<T>(t, sm, tid, all);
+    return all;
+  };
+  double R = total_of(false);
+  bool plain = false;
+  if (R == 0.0 && (both || skips)) {
+    plain = true;
+    R = total_of(true);
+  }
+  int32_t token = -1;
+  if (rate > 0.0 && R > 0.0) {
+    const double place = u * R;
+    // the first chunk whose running sum passes the place, and the sum ahead of it; the
+    // last chunk of any mass where rounding lets none pass
+    if (tid == 0) {
+      sm_at = a.chunks;
+      sm_last = -1;
+    }
+    __syncthreads();
+    double carry = 0.0;
+    for (int c0 = 0; c0 < a.chunks; c0 += T) {
+      const double v = sum_of(c0 + tid, plain);
+      double all;
+      const double before = carry + block_prefix<T>(v, sm, tid, all);
+      if (v > 0.0) {
+        atomicMax(&sm_last, c0 + tid);
+        if (before + v > place) atomicMin(&sm_at, c0 + tid);
+      }
+      __syncthreads();
+      const int c = sm_at < a.chunks ? sm_at : sm_last;
+      if (c == c0 + tid) sm_ahead = before;
+      carry += all;
+      if (sm_at < a.chunks) break;
+    }
+    __syncthreads();
+    const int c = sm_at < a.chunks ? sm_at : sm_last;
+    const double ahead = sm_ahead;
+    __syncthreads();
+    if (tid == 0) {
+      sm_at = a.V;
+      sm_last = -1;
+    }
+    __syncthreads();
+    if (plain) {
+      both = false;
+      p.skip = -1;
+    }
+    double run = ahead;
+    for (int base = c * per; base < (c + 1) * per; base += T * N) {
+      const int i0 = base + tid * N;
+      float x[N], y[N];
+      double r[N], mine = 0.0, all;
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[e] = y[e] = -INFINITY;
+      if (i0 < (c + 1) * per) {
+        load_logits<E>(tr, i0, a.V, x);
+        if (both) load_logits<E>(dr, i0, a.V, y);
+      }
+      rest_weights<E>(a, p, both, x, y, i0, rate, r);
+#pragma unroll
+      for (int e = 0; e < N; ++e) mine += r[e];
+      double at = run + block_prefix<T>(mine, sm, tid, all);
+      int first = a.V, last = -1;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        at += r[e];
+        if (r[e] > 0.0) {
+          last = i0 + e;
+          if (at > place && first == a.V) first = i0 + e;
+        }
+      }
+      if (first < a.V) atomicMin(&sm_at, first);
+      if (last >= 0) atomicMax(&sm_last, last);
+      run += all;
+    }
+    __syncthreads();
+    token = sm_at < a.V ? sm_at : sm_last;
+  }
+  for (int j = tid; j <= a.k; j += T) {
+    const int32_t d = j < a.k ? a.drafts[static_cast<size_t>(b) * a.k + j] : -1;
+    a.emitted[static_cast<size_t>(b) * (a.k + 1) + j] =
+        j < p.n_acc ? d : j == p.n_acc ? token : -1;
+  }
+  if (tid == 0) {
+    a.n_acc[b] = p.n_acc;
+    if (a.keep) {
+      const int row = a.seq_rows ? a.seq_rows[b] : b;
+      a.keep[b] = row >= 0 && row < a.num_rows ? a.lens[row] - a.k + p.n_acc : 0;
+    }
+  }
+}
+
+// Vectors a thread: chunks of 8192 logits, smaller ones where those leave compute
+// units without a workgroup.
+static int sample_vectors(long long rows, int V, int vec) {
+  const int most = 8192 / (kStatThreads * vec);
+  for (int nv = most; nv > 1; nv /= 2)
+    if (rows * cdiv(V, nv * kStatThreads * vec) >= 512) return nv;
+  return 1;
+}
+
+struct SampleCfg {
+  int rows, nv, chunks;
+  size_t sums, maxes, rest, picks, bytes;  // offsets of the workspace's parts
+};
+
+static SampleCfg sample_cfg(int B, int k, int V, int dtype, bool draft) {
+  SampleCfg c{};
+  const int vec = dtype == KVE_DTYPE_BF16 ? 8 : 4;
+  c.rows = draft ? 2 * k + 1 : k + 1;
+  c.nv = sample_vectors(static_cast<long long>(B) * c.rows, V, vec);
+  c.chunks = cdiv(V, c.nv * kStatThreads * vec);
+  const size_t parts = static_cast<size_t>(B) * c.rows * c.chunks;
+  size_t at = 0;
+  const auto take = [&](size_t n) {
+    const size_t was = at;
+    at += (n + 15) & ~static_cast<size_t>(15);
+    return was;
+  };
+  c.sums = take(parts * sizeof(double));
+  c.maxes = take(parts * sizeof(float));
+  c.rest = take(static_cast<size_t>(B) * c.chunks * sizeof(double));
+  c.picks = take(static_cast<size_t>(B) * sizeof(SamplePick));
+  c.bytes = at;
+  return c;
+}
+
+template <typename E, int NV>
+static void launch_sample(const SampleArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((sample_stats_kernel<E, NV>), dim3(a.B * a.rows * a.chunks),
+                     dim3(kStatThreads), 0, st, a);
+  const size_t lds = static_cast<size_t>(a.rows) * (sizeof(double) + sizeof(float));
+  if (a.draft)
+    hipLaunchKernelGGL((sample_rest_kernel<E, NV>), dim3(a.B * a.chunks), dim3(kStatThreads), lds, st,
+                       a);
+  hipLaunchKernelGGL(sample_pick_kernel<E>, dim3(a.B), dim3(kPickThreads), lds, st, a,
+                     NV * kStatThreads * kVec<E>);
+}
+
+}  // namespace kve
+
+using namespace kve;
+
+// Drafts a sequence may have (their rows' statistics share a workgroup's LDS).
+constexpr int kSampleMaxDrafts = 1024;
+
+extern "C" size_t kve_sample_workspace_bytes(int num_seqs, int k, int vocab, int dtype) {
+  if (num_seqs <= 0 || k < 0 || k > kSampleMaxDrafts || vocab <= 0 ||
+      (dtype != KVE_DTYPE_BF16 && dtype != KVE_DTYPE_F32))
+    return 0;
+  return std::max(sample_cfg(num_seqs, k, vocab, dtype, true).bytes,
+                  sample_cfg(num_seqs, k, vocab, dtype, false).bytes);
+}
+
+extern "C" int kve_sample_verify(const void* target, int64_t target_seq_stride,
+                                 int64_t target_pos_stride, const void* draft,
+                                 int64_t draft_seq_stride, int64_t draft_pos_stride,
+                                 const int32_t* drafts, const float* u_accept,
+                                 const float* u_sample, const float* temperatures,
+                                 float temperature, const int32_t* lens, int num_rows,
+                                 const int32_t* seq_rows, int num_seqs, int k, int vocab,
+                                 int dtype, int32_t* n_acc, int32_t* emitted, int32_t* keep_lens,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (num_seqs == 0) return KVE_OK;
+  KVE_REQUIRE(target && u_sample && n_acc && emitted && (k == 0 || (drafts && u_accept)),
+              "kve_sample_verify: null pointer argument");
+  KVE_REQUIRE(num_seqs > 0 && k >= 0 && k <= kSampleMaxDrafts && vocab > 0 && vocab <= (1 << 30),
+              "kve_sample_verify: %d sequences, k = %d (at most %d), vocabulary %d", num_seqs, k,
+              kSampleMaxDrafts, vocab);
+  KVE_REQUIRE(dtype == KVE_DTYPE_BF16 || dtype == KVE_DTYPE_F32, "kve_sample_verify: dtype %d",
+              dtype);
+  KVE_REQUIRE(temperatures || (temperature > 0.0f && temperature < INFINITY),
+              "kve_sample_verify: temperature %g", static_cast<double>(temperature));
+  KVE_REQUIRE(!keep_lens || (lens && num_rows > 0), "kve_sample_verify: keep_lens needs lens");
+  const size_t esz = dtype == KVE_DTYPE_BF16 ? 2 : 4;
+  KVE_REQUIRE(((reinterpret_cast<uintptr_t>(target) | reinterpret_cast<uintptr_t>(draft)) &
+               (esz - 1)) == 0,
+              "kve_sample_verify: logits are not aligned to their type");
+  const SampleCfg c = sample_cfg(num_seqs, k, vocab, dtype, draft != nullptr && k > 0);
+  KVE_REQUIRE(static_cast<long long>(num_seqs) * c.rows * c.chunks < (1ll << 31),
+              "kve_sample_verify: %d x %d rows of %d too large for one launch", num_seqs, c.rows,
+              vocab);
+  KVE_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
+              "kve_sample_verify: workspace required (16-byte aligned)");
+  if (workspace_bytes < c.bytes) {
+    set_error("kve_sample_verify: workspace %zu bytes, need %zu", workspace_bytes, c.bytes);
+    return KVE_EWORKSPACE;
+  }
+  char* ws = static_cast<char*>(workspace);
+  SampleArgs a{};
+  a.target = target;
+  a.draft = k > 0 ? draft : nullptr;
+  a.ts = target_seq_stride;
+  a.tp = target_pos_stride;
+  a.ds = draft_seq_stride;
+  a.dp = draft_pos_stride;
+  a.drafts = drafts;
+  a.u_accept = u_accept;
+  a.u_sample = u_sample;
+  a.temps = temperatures;
+  a.temp = temperature;
+  a.lens = lens;
+  a.seq_rows = seq_rows;
+  a.num_rows = num_rows;
+  a.B = num_seqs;
+  a.k = k;
+  a.V = vocab;
+  a.rows = c.rows;
+  a.chunks = c.chunks;
+  a.n_acc = n_acc;
+  a.emitted = emitted;
+  a.keep = keep_lens;
+  a.sums = reinterpret_cast<double*>(ws + c.sums);
+  a.maxes = reinterpret_cast<float*>(ws + c.maxes);
+  a.rest = reinterpret_cast<double*>(ws + c.rest);
+  a.picks = reinterpret_cast<SamplePick*>(ws + c.picks);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == KVE_DTYPE_BF16) {
+    if (c.nv == 4) launch_sample<uint16_t, 4>(a, st);
+    else if (c.nv == 2) launch_sample<uint16_t, 2>(a, st);
+    else launch_sample<uint16_t, 1>(a, st);
+  } else {
+    if (c.nv == 8) launch_sample<float, 8>(a, st);
+    else if (c.nv == 4) launch_sample<float, 4>(a, st);
+    else if (c.nv == 2) launch_sample<float, 2>(a, st);
+    else launch_sample<float, 1>(a, st);
+  }
+  return check_launch("kve_sample_verify");
+}

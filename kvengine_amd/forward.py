@@ -80,11 +80,13 @@ class LayerAttention:
     """The paged verify-attention launches of one forward pass: one work plan
     (kve_attn_plan) shared by every layer, and the summation order `attn` =
     (unit_blocks, key_waves) of kve_paged_verify_attn ((0, 0): chosen per
-    launch; fixed values make a row's result independent of the batch)."""
+    launch; fixed values make a row's result independent of the batch). tree: the
+    (masks, depths) of a pass over trees (kernels.tree_masks)."""
 
     def __init__(self, kv: DeviceKV, rows, B: int, T: int, Hq: int, max_ctx: int, q_lens,
-                 dtype, attn: tuple[int, int] = (0, 0)):
+                 dtype, attn: tuple[int, int] = (0, 0), tree=None):
         self.kv, self.rows, self.q_lens, self.max_ctx = kv, rows, q_lens, max_ctx
+        self.masks = None if tree is None else tree[0]
         self.unit_blocks, self.key_waves = attn
         _, NB, Hkv, bs, D = kv.k.shape
         self.plan = kernels.attn_plan(kv.tables, kv.lens, B, T, Hq, Hkv, D, bs, NB, max_ctx, dtype,
@@ -93,6 +95,12 @@ class LayerAttention:
 
     def __call__(self, q, li: int, scale: float, out=None, blocked: bool = False):
         kv = self.kv
+        if self.masks is not None:
+            return kernels.paged_tree_attn(q, kv.k[li], kv.v[li], kv.tables, kv.lens, self.max_ctx,
+                                           self.masks, seq_rows=self.rows, q_lens=self.q_lens,
+                                           scale=scale, unit_blocks=self.unit_blocks,
+                                           key_waves=self.key_waves, plan=self.plan, out=out,
+                                           blocked=blocked)
         return kernels.paged_verify_attn(q, kv.k[li], kv.v[li], kv.tables, kv.lens, self.max_ctx,
                                          seq_rows=self.rows, q_lens=self.q_lens, scale=scale,
                                          unit_blocks=self.unit_blocks, key_waves=self.key_waves,
@@ -184,7 +192,8 @@ def _small_fusable(model, rows: int) -> bool:
 def forward_hidden(model, input_ids: torch.Tensor, kv: DeviceKV, rows: torch.Tensor, max_ctx: int,
                    q_lens: torch.Tensor | None = None, attn_order: tuple[int, int] = (0, 0),
                    fused: bool | None = None, gemm_rows: int | None = None,
-                   blocked_out: bool = False) -> torch.Tensor:
+                   blocked_out: bool = False,
+                   tree: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
     """Final-normed hidden states [B, T, H] for `input_ids` [B, T] (device int64).
 
     Row i of the batch is table/length row rows[i]; its tokens land at positions
@@ -206,7 +215,20 @@ def forward_hidden(model, input_ids: torch.Tensor, kv: DeviceKV, rows: torch.Ten
     blocked_out: return the final hidden states as the [B*T, H] blocked matrix
     (kernels.to_blocked layout, rows padded to 16) for a blocked LM head; only
     where blocked_forward(model, input_ids.numel(), gemm_rows) holds.
+
+    tree: the T tokens of a sequence are the nodes of a tree of drafts, (masks,
+    depths) of kernels.tree_masks: node t's K/V lands at slot kv.lens + t, its
+    rotary position is kv.lens + depth, and it attends to the history and the
+    nodes above it. The passes that issue their layers by one host call
+    (kernels.small_pass, kernels.f32_pass) take chains only: trees run the
+    split-K layer, or the library GEMMs where that does not fit. After the commit
+    kernels.tree_accept picks the path and makes its K/V consecutive.
     """
+    if tree is not None:
+        masks, depths = tree
+        if masks.shape != input_ids.shape or depths.shape != input_ids.shape:
+            raise ValueError(f"tree masks {tuple(masks.shape)} and depths {tuple(depths.shape)} "
+                             f"do not match the tokens {tuple(input_ids.shape)}")
     if fused is None:
         fused = _fusable(model)
     n = input_ids.numel()
@@ -215,27 +237,25 @@ def forward_hidden(model, input_ids: torch.Tensor, kv: DeviceKV, rows: torch.Ten
             raise ValueError("blocked_out needs the blocked split-K layer (blocked_forward)")
     if fused and gemm_rows is not None and n <= gemm_rows and _wide_ok(model, gemm_rows):
         return _forward_splitk(model, input_ids, kv, rows, max_ctx, q_lens, attn_order, wide=True,
-                               blocked_out=blocked_out)
+                               blocked_out=blocked_out, tree=tree)
     if fused:
-        if _small_fusable(model, n):
-            if _small_path(model, n) == "splitk":
+        if _small_fusable(model, n) and (tree is None or _splitk_ok(model, n)):
+            if tree is not None or _small_path(model, n) == "splitk":
                 return _forward_splitk(model, input_ids, kv, rows, max_ctx, q_lens, attn_order,
-                                       blocked_out=blocked_out)
+                                       blocked_out=blocked_out, tree=tree)
             return _forward_small(model, input_ids, kv, rows, max_ctx, q_lens, attn_order)
         if _wide_ok(model, n) and (n <= SPLITK_MAX_ROWS or _plain_tokens(model, input_ids)):
             return _forward_splitk(model, input_ids, kv, rows, max_ctx, q_lens, attn_order, wide=True,
-                                   blocked_out=blocked_out)
-        if _f32_ok(model, n) and _plain_tokens(model, input_ids):
+                                   blocked_out=blocked_out, tree=tree)
+        if tree is None and _f32_ok(model, n) and _plain_tokens(model, input_ids):
             return _forward_f32(model, input_ids, kv, rows, max_ctx, q_lens, attn_order)
-        return _forward_fused(model, input_ids, kv, rows, max_ctx, q_lens, attn_order)
+        return _forward_fused(model, input_ids, kv, rows, max_ctx, q_lens, attn_order, tree)
     inner = model.model
     B, T = input_ids.shape
     hidden = inner.embed_tokens(input_ids)
-    start = kv.lens.index_select(0, rows).to(torch.long)
-    positions = start[:, None] + torch.arange(T, device=input_ids.device)[None, :]
-    cos, sin = inner.rotary_emb(hidden, positions, max_ctx)
+    cos, sin = inner.rotary_emb(hidden, _positions(kv, rows, T, tree), max_ctx)
     layer_attn = LayerAttention(kv, rows, B, T, _q_heads(model, kv), max_ctx, q_lens, kv.k.dtype,
-                                attn_order)
+                                attn_order, tree)
     for layer in inner.layers:
         attn = layer.self_attn
         if getattr(attn, "sliding_window", None) is not None:
@@ -327,20 +347,26 @@ def _wide_ok(model, rows: int) -> bool:
     return all(n % 128 == 0 for n in outs) and all(k % 64 == 0 for k in ins)
 
 
-def _forward_fused(model, input_ids, kv: DeviceKV, rows, max_ctx, q_lens, attn_order):
+def _positions(kv: DeviceKV, rows, T: int, tree=None) -> torch.Tensor:
+    """Rotary positions [B, T] of a pass's tokens: a tree's node at its depth."""
+    start = kv.lens.index_select(0, rows).to(torch.long)
+    if tree is not None:
+        return start[:, None] + tree[1]
+    return start[:, None] + torch.arange(T, device=start.device)[None, :]
+
+
+def _forward_fused(model, input_ids, kv: DeviceKV, rows, max_ctx, q_lens, attn_order, tree=None):
     inner = model.model
     layers = inner.layers
     B, T = input_ids.shape
     splitk = _splitk_ok(model, B * T)
     residual = inner.embed_tokens(input_ids)
-    start = kv.lens.index_select(0, rows).to(torch.long)
-    positions = start[:, None] + torch.arange(T, device=input_ids.device)[None, :]
-    cos, sin = inner.rotary_emb(residual, positions, max_ctx)
+    cos, sin = inner.rotary_emb(residual, _positions(kv, rows, T, tree), max_ctx)
     cos, sin = cos.contiguous(), sin.contiguous()
     first = layers[0].input_layernorm
     h = kernels.rmsnorm(residual, first.weight, first.variance_epsilon)
     layer_attn = LayerAttention(kv, rows, B, T, _q_heads(model, kv), max_ctx, q_lens, kv.k.dtype,
-                                attn_order)
+                                attn_order, tree)
     for i, layer in enumerate(layers):
         attn = layer.self_attn
         if getattr(attn, "sliding_window", None) is not None:
@@ -633,7 +659,7 @@ def blocked_forward(model, n: int, gemm_rows: int | None = None) -> bool:
 
 
 def _forward_splitk(model, input_ids, kv: DeviceKV, rows, max_ctx, q_lens, attn_order,
-                    wide: bool = False, blocked_out: bool = False):
+                    wide: bool = False, blocked_out: bool = False, tree=None):
     """Six launches per layer: QKV (+bias, RoPE, KV write), attention (+ its
     split merge), o_proj + residual (whole columns per workgroup), gate/up with
     the RMSNorm in its prologue + SiLU*up, down_proj k-slices, residual add +
@@ -653,12 +679,15 @@ def _forward_splitk(model, input_ids, kv: DeviceKV, rows, max_ctx, q_lens, attn_
     blk = _has_blocked(model)
     fused_o = not wide and SPLITK_FUSED_O and n <= SPLITK_FUSED_O_ROWS
     residual, cos, sin = _prologue(model, input_ids, kv, rows, max_ctx)
+    if tree is not None:  # the prologue's angles are a chain's
+        cos, sin = inner.rotary_emb(residual, _positions(kv, rows, T, tree), max_ctx)
+        cos, sin = cos.contiguous(), sin.contiguous()
     slots = kernels.kv_slots(kv.tables, kv.lens, B, T, kv.block_size, kv.k.shape[1], seq_rows=rows,
                              q_lens=q_lens)
     first = layers[0].input_layernorm
     xn = kernels.rmsnorm(residual, first.weight, first.variance_epsilon, blocked=blk)
     layer_attn = LayerAttention(kv, rows, B, T, _q_heads(model, kv), max_ctx, q_lens, kv.k.dtype,
-                                attn_order)
+                                attn_order, tree)
     for i, layer in enumerate(layers):
         attn = layer.self_attn
         if getattr(attn, "sliding_window", None) is not None:

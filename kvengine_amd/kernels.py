@@ -877,3 +877,209 @@ def linear_rows(x: torch.Tensor, weight: torch.Tensor, mode: int, out: torch.Ten
                              int(mode), _layout(blocked), _stream(x.device))
     _lib.check(rc, "kve_linear_rows")
     return out
+
+
+# ---- trees of drafted tokens, sampled verification ------------------------------
+
+TREE_MAX_NODES = 64
+
+
+def _check_on(t: torch.Tensor | None, name: str, dtype, shape: tuple, dev) -> None:
+    if t is None:
+        return
+    _need(t.dtype is dtype and tuple(t.shape) == shape and t.device == dev and t.is_contiguous(),
+          f"{name} must be contiguous {dtype} {list(shape)} on {dev}, "
+          f"got {t.dtype} {list(t.shape)} on {t.device}")
+
+
+def _check_tree(parents: torch.Tensor, q_lens: torch.Tensor | None) -> tuple[int, int]:
+    _need(parents.dim() == 2 and parents.is_cuda, "parents must be [B, nodes] on the GPU")
+    B, n = parents.shape
+    _need(1 <= n <= TREE_MAX_NODES, f"{n} nodes per tree, 1 to {TREE_MAX_NODES}")
+    _check_on(parents, "parents", torch.int32, (B, n), parents.device)
+    _check_on(q_lens, "q_lens", torch.int32, (B,), parents.device)
+    return B, n
+
+
+def tree_masks(parents: torch.Tensor, q_lens: torch.Tensor | None = None):
+    """Trees of drafted tokens, parents [B, n] int32 (node 0 the last emitted token,
+    parents[:, 0] = -1, parents[:, t] < t, n <= TREE_MAX_NODES) -> (masks [B, n]
+    int64: bit j of masks[b, t] set where node j is node t or above it, depths
+    [B, n] int32: nodes above t, so start + depth is node t's rotary position).
+    q_lens [B]: nodes per tree (those past it get mask 0). A parent outside [0, t)
+    counts as none."""
+    B, n = _check_tree(parents, q_lens)
+    dev = parents.device
+    masks = torch.empty(B, n, dtype=torch.int64, device=dev)
+    depths = torch.empty(B, n, dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        rc = _lib.lib().kve_tree_masks(parents.data_ptr(), _ptr(q_lens), B, n, masks.data_ptr(),
+                                       depths.data_ptr(), _stream(dev))
+    _lib.check(rc, "kve_tree_masks")
+    return masks, depths
+
+
+def paged_tree_attn(q: torch.Tensor, k_layer: torch.Tensor, v_layer: torch.Tensor,
+                    block_tables: torch.Tensor, start_pos: torch.Tensor, max_ctx: int,
+                    masks: torch.Tensor, seq_rows: torch.Tensor | None = None,
+                    q_lens: torch.Tensor | None = None, scale: float | None = None,
+                    unit_blocks: int = 0, key_waves: int = 0, plan: AttnPlan | None = None,
+                    out: torch.Tensor | None = None, ws: torch.Tensor | None = None,
+                    blocked: bool = False) -> torch.Tensor:
+    """paged_verify_attn where the T new tokens of a sequence are the nodes of a tree
+    (node t at slot start_pos + t): query t sees the committed keys and, of the tree,
+    the nodes j <= t whose bit masks[b, t] has (tree_masks). masks [B, T] int64, T <=
+    TREE_MAX_NODES; the other arguments, the plan (attn_plan) and the result as there.
+    A row that sees no key is zeros; a chain's masks give paged_verify_attn's bits.
+    The workspace is this call's own (ws: a buffer of attn_workspace_bytes instead),
+    so captured graphs share none."""
+    _need(q.dim() == 4 and q.is_contiguous() and q.is_cuda, "q must be contiguous [B, T, Hq, D]")
+    dev = q.device
+    B, T, Hq, D = q.shape
+    _need(T <= TREE_MAX_NODES, f"{T} nodes per tree, at most {TREE_MAX_NODES}")
+    _check_on(masks, "masks", torch.int64, (B, T), dev)
+    _need(k_layer.dim() == 4 and v_layer.dim() == 4, "k/v layer must be 4-d")
+    NB, Hkv, bs, Dk = k_layer.shape
+    _need(Dk == D and tuple(v_layer.shape) == (NB, Hkv, D, bs),
+          f"pool shapes k{tuple(k_layer.shape)} v{tuple(v_layer.shape)} do not match q D={D}")
+    _need(k_layer.is_contiguous() and v_layer.is_contiguous() and k_layer.device == dev
+          and v_layer.device == dev, f"k/v layer must be contiguous on {dev}")
+    _need(k_layer.dtype == q.dtype == v_layer.dtype, "q/k/v dtype mismatch")
+    _need(Hkv > 0 and Hq % Hkv == 0, f"{Hq} q heads not a multiple of {Hkv} kv heads")
+    max_blocks, num_rows = _attn_checks(block_tables, start_pos, seq_rows, q_lens, B, bs, max_ctx,
+                                        dev)
+    if plan is not None:
+        _need(plan.key == _attn_key(B, T, Hq, Hkv, D, bs, max_ctx, unit_blocks, key_waves, q.dtype)
+              and plan.buf.device == dev,
+              "attention plan was built for another shape, configuration or device")
+    if blocked:
+        _need(q.dtype == torch.bfloat16 and (Hq * D) % 32 == 0, "blocked out is bf16, Hq*D % 32")
+        if out is None:
+            out = blocked_matrix(B * T, Hq * D, dev)
+        _need(out.dtype == q.dtype and out.device == dev and out.is_contiguous()
+              and out.numel() >= blocked_rows(B * T) * Hq * D, "bad blocked out")
+    elif out is None:
+        out = torch.empty_like(q)
+    else:
+        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == dev
+              and out.is_contiguous(), "bad out")
+    scale = D ** -0.5 if scale is None else float(scale)
+    _need(scale > 0.0, f"scale {scale} must be positive")
+    if B == 0 or T == 0:
+        return out
+    nbytes = attn_workspace_bytes(B, T, Hq, Hkv, D, bs, max_ctx, unit_blocks, key_waves, q.dtype)
+    if ws is None:
+        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+    _need(ws.numel() * ws.element_size() >= nbytes and ws.device == dev,
+          "attention workspace too small")
+    with torch.cuda.device(dev):
+        rc = _lib.lib().kve_paged_tree_attn(
+            q.data_ptr(), k_layer.data_ptr(), v_layer.data_ptr(), masks.data_ptr(),
+            block_tables.data_ptr(), _ptr(seq_rows), start_pos.data_ptr(), _ptr(q_lens), B, T, Hq,
+            Hkv, D, bs, max_blocks, num_rows, NB, int(max_ctx), int(unit_blocks), int(key_waves),
+            scale, _dtype_code(q), None if plan is None else plan.buf.data_ptr(), out.data_ptr(),
+            ws.data_ptr(), ws.numel() * ws.element_size(), _layout(blocked), _stream(dev))
+    _lib.check(rc, "kve_paged_tree_attn")
+    return out
+
+
+def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, preds: torch.Tensor, kv=None,
+                seq_rows: torch.Tensor | None = None, q_lens: torch.Tensor | None = None):
+    """The walk of trees by the target's picks (accept's form for trees): from node 0 to
+    the child whose token is the pick at the current node, lowest node first.
+    tokens, parents, preds [B, n] int32 (preds[b, t]: the target's token after node t,
+    from lmhead_argmax or sample_verify) -> (n_acc [B], emitted [B, n]: the accepted
+    nodes' tokens, then the pick after the last, then -1, path [B, n]: the nodes walked
+    from node 0 on, then -1, keep [B] or None).
+    kv (a DeviceKV whose lens hold the whole trees): in every layer the K/V of the
+    accepted nodes move to consecutive slots behind the committed history, and keep is
+    the length to roll back to (rollback). seq_rows: table rows (default 0 .. B-1); of
+    two entries with one row the first moves it."""
+    B, n = _check_tree(parents, q_lens)
+    dev = parents.device
+    _check_on(tokens, "tokens", torch.int32, (B, n), dev)
+    _check_on(preds, "preds", torch.int32, (B, n), dev)
+    _check_on(seq_rows, "seq_rows", torch.int32, (B,), dev)
+    out = torch.empty(2, B, n, dtype=torch.int32, device=dev)
+    ints = torch.empty(2, B, dtype=torch.int32, device=dev)
+    emitted, path, n_acc, keep = out[0], out[1], ints[0], None
+    pools, sizes, lens, rows = (None, None, None), (0, 0, 0, 0, 0, 0, 0), None, 0
+    if kv is not None:
+        keep = ints[1]
+        L, NB, Hkv, bs, D = kv.k.shape
+        _need(tuple(kv.v.shape) == (L, NB, Hkv, D, bs) and kv.k.dtype == kv.v.dtype
+              and kv.k.is_contiguous() and kv.v.is_contiguous() and kv.k.device == dev
+              and kv.v.device == dev, "pools must be contiguous [L, NB, Hkv, bs, D] / [.., D, bs]")
+        lens, rows = kv.lens, kv.lens.numel()
+        _check_i32(lens, "lens", dev)
+        _check_i32(kv.tables, "tables", dev)
+        _need(kv.tables.dim() == 2 and kv.tables.shape[0] == rows, "one length per table row")
+        _need(seq_rows is not None or rows >= B, "too few table rows")
+        pools = (kv.k.data_ptr(), kv.v.data_ptr(), kv.tables.data_ptr())
+        sizes = (L, Hkv, D, bs, kv.tables.shape[1], NB, _dtype_code(kv.k))
+    with torch.cuda.device(dev):
+        rc = _lib.lib().kve_tree_accept(
+            tokens.data_ptr(), parents.data_ptr(), preds.data_ptr(), _ptr(q_lens), _ptr(lens),
+            rows, _ptr(seq_rows), B, n, n_acc.data_ptr(), emitted.data_ptr(), path.data_ptr(),
+            _ptr(keep), *pools, *sizes, _stream(dev))
+    _lib.check(rc, "kve_tree_accept")
+    return n_acc, emitted, path, keep
+
+
+def sample_verify(target_logits: torch.Tensor, drafts: torch.Tensor, u_accept: torch.Tensor,
+                  u_sample: torch.Tensor, draft_logits: torch.Tensor | None = None,
+                  temperature: float | torch.Tensor = 1.0, lens: torch.Tensor | None = None,
+                  seq_rows: torch.Tensor | None = None):
+    """Verification of drafted tokens by rejection sampling (accept's form for decoding
+    at a temperature). target_logits [B, k+1, V], draft_logits [B, k, V] of one dtype
+    (bf16 or float32; vocabulary contiguous, the other strides free), drafts [B, k] int32
+    sampled from the draft's softmax at the same temperature; None: drafts that were not
+    sampled (a greedy draft, a tree's node). u_accept [B, k], u_sample [B] float32 uniform
+    in [0, 1). temperature: a positive number, or [B] float32. k = 0 samples one token per
+    sequence. -> (n_acc [B], emitted [B, k+1]: accepted drafts, the sampled token, then -1,
+    keep [B] = lens - k + n_acc, or None without lens). Draws are exact: 64-bit sums."""
+    _need(target_logits.dim() == 3 and target_logits.is_cuda, "target_logits must be [B, k+1, V]")
+    dev = target_logits.device
+    B, k1, V = target_logits.shape
+    k = k1 - 1
+    _need(k >= 0 and V >= 1, f"target_logits {list(target_logits.shape)}")
+    _need(target_logits.stride(2) == 1 or V == 1, "logits need a contiguous vocabulary")
+    _check_on(drafts, "drafts", torch.int32, (B, k), dev)
+    _check_on(u_accept, "u_accept", torch.float32, (B, k), dev)
+    _check_on(u_sample, "u_sample", torch.float32, (B,), dev)
+    ds = (0, 0)
+    if draft_logits is not None:
+        _need(tuple(draft_logits.shape) == (B, k, V) and draft_logits.dtype == target_logits.dtype
+              and draft_logits.device == dev and (draft_logits.stride(2) == 1 or V == 1),
+              f"draft_logits must be {target_logits.dtype} {[B, k, V]} on {dev} with a contiguous "
+              f"vocabulary")
+        ds = draft_logits.stride()[:2]
+    temps = None
+    if isinstance(temperature, torch.Tensor):
+        temps, temperature = temperature, 1.0
+        _check_on(temps, "temperature", torch.float32, (B,), dev)
+    else:
+        temperature = float(temperature)
+        _need(0.0 < temperature < float("inf"), f"temperature {temperature} must be positive")
+    _check_i32(lens, "lens", dev)
+    _check_on(seq_rows, "seq_rows", torch.int32, (B,), dev)
+    num_rows = 0 if lens is None else lens.numel()
+    _need(lens is None or seq_rows is not None or num_rows >= B, "too few length rows")
+    code = _dtype_code(target_logits)
+    n_acc = torch.empty(B, dtype=torch.int32, device=dev)
+    emitted = torch.empty(B, k1, dtype=torch.int32, device=dev)
+    keep = None if lens is None else torch.empty(B, dtype=torch.int32, device=dev)
+    if B == 0:
+        return n_acc, emitted, keep
+    lib = _lib.lib()
+    nbytes = lib.kve_sample_workspace_bytes(B, k, V, code)
+    _need(nbytes > 0, f"{k} drafts per sequence are too many")
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        rc = lib.kve_sample_verify(
+            target_logits.data_ptr(), *target_logits.stride()[:2], _ptr(draft_logits), *ds,
+            drafts.data_ptr(), u_accept.data_ptr(), u_sample.data_ptr(), _ptr(temps), temperature,
+            _ptr(lens), num_rows, _ptr(seq_rows), B, k, V, code, n_acc.data_ptr(),
+            emitted.data_ptr(), _ptr(keep), ws.data_ptr(), nbytes, _stream(dev))
+    _lib.check(rc, "kve_sample_verify")
+    return n_acc, emitted, keep
