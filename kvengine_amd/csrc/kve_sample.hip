@@ -14,8 +14,8 @@
 // an unpacked 32-bit one, so the price is the polynomial's length.
 //
 // Launches, each a dependency of the next over the whole vocabulary:
-//  stats   every (row, chunk): maximum and sum of 2^((l - max) c), c = log2(e) / T,
-//          the chunk held in registers between the two
+//  stats   every (row, chunk of 2048 logits), a chunk per wave: maximum and sum of
+//          2^((l - max) c), c = log2(e) / T, the chunk held in registers between the two
 //  rest    every (sequence, chunk), where drafts have probabilities: the rows' chunks
 //          joined, the accept tests, and the chunk's sum of r at the deciding position
 //          (one row of each side, again)
@@ -53,8 +53,9 @@ struct SampleArgs {
   SamplePick* picks;  // [B]
 };
 
-constexpr int kStatThreads = 256;
-constexpr int kPickThreads = 1024;
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kChunk = 2048;  // logits: 32 per lane of a wave, 8 per thread of a workgroup
 
 // log2(e) / T, or 0 where T is not positive and finite (the sequence has no answer)
 __device__ __forceinline__ double sample_rate(const SampleArgs& a, int b) {
@@ -62,20 +63,19 @@ __device__ __forceinline__ double sample_rate(const SampleArgs& a, int b) {
   return t > 0.0f && t < INFINITY ? 1.4426950408889634074 / static_cast<double>(t) : 0.0;
 }
 
-// 2^y = 2^n 2^f with n = round(y), f = y - n: the polynomial of degree 10 that meets 2^f
-// at the eleven Chebyshev points of [-1/2, 1/2], within 3e-16 of it; 2^0 is 1 exactly, so
-// that equal logits give exactly equal sums.
+// 2^y = 2^n 2^f with n = round(y), f = y - n: 1 + f q(f), q the polynomial of degree 8
+// that meets (2^f - 1) / f at the nine Chebyshev points of [-1/2, 1/2]. Within 4e-14
+// of 2^f, and 2^0 is 1 exactly, so that equal logits give exactly equal sums.
 __device__ __forceinline__ double exp2_poly(double f) {
-  double p = 7.072585949269223e-09;
-  p = fma(p, f, 1.0208690299958306e-07);
-  p = fma(p, f, 1.321544258792169e-06);
-  p = fma(p, f, 1.5252657260200837e-05);
-  p = fma(p, f, 0.0001540353044173605);
-  p = fma(p, f, 0.0013333558230164974);
-  p = fma(p, f, 0.009618129107606888);
-  p = fma(p, f, 0.05550410866444772);
-  p = fma(p, f, 0.24022650695910097);
-  p = fma(p, f, 0.69314718055995);
+  double p = 1.0203121063391729e-07;
+  p = fma(p, f, 1.3255224878668817e-06);
+  p = fma(p, f, 1.525268684626772e-05);
+  p = fma(p, f, 0.00015403455852453838);
+  p = fma(p, f, 0.0013333558179043112);
+  p = fma(p, f, 0.009618129159402558);
+  p = fma(p, f, 0.055504108664760424);
+  p = fma(p, f, 0.2402265069581299);
+  p = fma(p, f, 0.6931471805599453);
   return fma(p, f, 1.0);
 }
 
@@ -91,19 +91,17 @@ __device__ __forceinline__ double weight(float l, double m, double rate) {
   return l == -INFINITY ? 0.0 : w;
 }
 
-// The same bits where (l - m) c is known to lie in [-1000, 0]: the rounding and the
-// power of two by adding 1.5 * 2^52, whose low word then holds n, in place of the
-// slower rounding, conversion and scaling instructions.
-__device__ __forceinline__ double weight_near(float l, double m, double rate) {
-#pragma clang fp contract(off)
-  constexpr double kShift = 6755399441055744.0;
-  const double y = (static_cast<double>(l) - m) * rate;
-  const double t = y + kShift;
-  const uint64_t p = __builtin_bit_cast(uint64_t, exp2_poly(y - (t - kShift)));
-  const uint32_t n = static_cast<uint32_t>(__builtin_bit_cast(uint64_t, t));
-  return __builtin_bit_cast(double, p + (static_cast<uint64_t>(n << 20) << 32));
-}
+// The same where (l - m) c is known to lie in [kNear, 0]: the rounding and the power of
+// two come from adding 1.5 * 2^52, whose low word then holds n, in place of the slower
+// rounding, conversion and scaling instructions.
 constexpr double kNear = -1000.0;
+__device__ __forceinline__ double weight_near(float l, double m, double rate) {
+  constexpr double kShift = 6755399441055744.0;
+  const double d = static_cast<double>(l) - m;
+  const double t = fma(d, rate, kShift);
+  const double p = exp2_poly(fma(d, rate, kShift - t));
+  return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
+}
 
 // What weights are taken against: a maximum of -inf (no mass) counts as 0.
 __device__ __forceinline__ double center(float m) {
@@ -150,21 +148,40 @@ __device__ __forceinline__ float to_f32(E v) {
 template <typename E>
 constexpr int kVec = 16 / sizeof(E);
 
-// A 16-byte vector of logits from element i0 on, of a row of V; those past the end are
-// -inf. Rows may start at any element (an odd vocabulary): gfx950 reads vectors at the
-// type's alignment.
+// A 16-byte vector of logits as stored, from element i0 on, of a row of V; those past the
+// end are -inf. Rows may start at any element (an odd vocabulary): gfx950 reads vectors
+// at the type's alignment.
+template <typename E>
+__device__ __forceinline__ u32x4 load_raw(const E* row, int i0, int V) {
+  constexpr int N = kVec<E>;
+  struct __attribute__((packed, aligned(sizeof(E)))) Vec { u32x4 v; };
+  if (i0 + N <= V) return reinterpret_cast<const Vec*>(row + i0)->v;
+  u32x4 x;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if constexpr (N == 4) {
+      x[w] = i0 + w < V ? __float_as_uint(row[i0 + w]) : 0xff800000u;
+    } else {
+      const uint32_t lo = i0 + 2 * w < V ? row[i0 + 2 * w] : 0xff80u;
+      const uint32_t hi = i0 + 2 * w + 1 < V ? row[i0 + 2 * w + 1] : 0xff80u;
+      x[w] = lo | hi << 16;
+    }
+  }
+  return x;
+}
+
+// Logit e of such a vector.
+template <typename E>
+__device__ __forceinline__ float logit(const u32x4& x, int e) {
+  if constexpr (kVec<E> == 4) return __uint_as_float(x[e]);
+  else return __uint_as_float(e & 1 ? x[e >> 1] & 0xffff0000u : x[e >> 1] << 16);
+}
+
 template <typename E>
 __device__ __forceinline__ void load_logits(const E* row, int i0, int V, float (&x)[kVec<E>]) {
-  constexpr int N = kVec<E>;
-  struct __attribute__((packed, aligned(sizeof(E)))) Vec { E v[N]; };
-  if (i0 + N <= V) {
-    const Vec t = *reinterpret_cast<const Vec*>(row + i0);
+  const u32x4 raw = load_raw<E>(row, i0, V);
 #pragma unroll
-    for (int e = 0; e < N; ++e) x[e] = to_f32(t.v[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e) x[e] = i0 + e < V ? to_f32(row[i0 + e]) : -INFINITY;
-  }
+  for (int e = 0; e < kVec<E>; ++e) x[e] = logit<E>(raw, e);
 }
 
 template <typename E>
@@ -173,57 +190,76 @@ __device__ __forceinline__ const E* logits_row(const SampleArgs& a, int b, int r
                   : static_cast<const E*>(a.draft) + b * a.ds + (r - a.k - 1) * a.dp;
 }
 
-// Grid: sequences x rows x chunks, chunks fastest. NV 16-byte vectors a thread.
-template <typename E, int NV>
-__global__ __launch_bounds__(kStatThreads) void sample_stats_kernel(SampleArgs a) {
-  constexpr int N = kVec<E>;
-  __shared__ float sm_max[kStatThreads / 64];
-  __shared__ double sm_sum[kStatThreads / 64];
-  const int tid = threadIdx.x, w = tid >> 6;
-  const int br = blockIdx.x / a.chunks, ch = blockIdx.x - br * a.chunks;
-  const int b = br / a.rows, r = br - b * a.rows;
-  const E* row = logits_row<E>(a, b, r);
-  const double rate = sample_rate(a, b);
-  float x[NV][N];
+// A lane's share of a chunk as stored: logits ch * kChunk + v * 64 * N + lane * N ...
+template <typename E>
+struct Piece {
+  static constexpr int N = kVec<E>, NV = kChunk / (64 * N);
+  u32x4 x[NV];
+  __device__ __forceinline__ void load(const E* row, int ch, int l, int V) {
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
-    load_logits<E>(row, (ch * NV + v) * kStatThreads * N + tid * N, a.V, x[v]);
-  float m = x[0][0], lo = x[0][0];
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      m = max_nan(m, x[v][e]);
-      lo = min_nan(lo, x[v][e]);
-    }
+    for (int v = 0; v < NV; ++v) x[v] = load_raw<E>(row, (ch * NV + v) * 64 * N + l * N, V);
   }
-  m = wave_max(m);
-  if ((tid & 63) == 0) sm_max[w] = m;
-  __syncthreads();
-#pragma unroll
-  for (int q = 0; q < kStatThreads / 64; ++q) m = max_nan(m, sm_max[q]);
-  const double c = center(m);
-  double s = 0.0;
-  if (__all((static_cast<double>(lo) - c) * rate >= kNear)) {
+  // Vector v from here on only: without it the compiler converts every logit of the
+  // chunk ahead of the sums (120 registers, four waves a SIMD).
+  __device__ __forceinline__ void hide(int v) { __asm__ volatile("" : "+v"(x[v])); }
+};
+
+// Every wave takes chunks (sequences x rows x chunks, chunks fastest) wave, wave +
+// waves of the grid, ..., the next one loading while one is summed.
+template <typename E>
+__global__ __launch_bounds__(kThreads) void sample_stats_kernel(SampleArgs a) {
+  constexpr int N = Piece<E>::N, NV = Piece<E>::NV;
+  const int l = threadIdx.x & 63;
+  const int total = a.B * a.rows * a.chunks, step = gridDim.x * kWaves;
+  int i = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (i >= total) return;
+  Piece<E> t;
+  int b = 0;
+  const auto load = [&](int at) {
+    const int br = at / a.chunks;
+    b = br / a.rows;
+    t.load(logits_row<E>(a, b, br - b * a.rows), at - br * a.chunks, l, a.V);
+  };
+  load(i);
+  for (;;) {
+    Piece<E> x = t;
+    const double rate = sample_rate(a, b);
+    const int next = i + step;
+    if (next < total) load(next);
+    float m = logit<E>(x.x[0], 0), lo = m;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) s += weight_near(x[v][e], c, rate);
+      for (int e = 0; e < N; ++e) {
+        m = max_nan(m, logit<E>(x.x[v], e));
+        lo = min_nan(lo, logit<E>(x.x[v], e));
+      }
     }
-  } else {
+    m = wave_max(m);
+    const double c = center(m);
+    double s = 0.0;
+    if (__all((static_cast<double>(lo) - c) * rate >= kNear)) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
+      for (int v = 0; v < NV; ++v) {
+        x.hide(v);
 #pragma unroll
-      for (int e = 0; e < N; ++e) s += weight(x[v][e], c, rate);
+        for (int e = 0; e < N; ++e) s += weight_near(logit<E>(x.x[v], e), c, rate);
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        x.hide(v);
+#pragma unroll
+        for (int e = 0; e < N; ++e) s += weight(logit<E>(x.x[v], e), c, rate);
+      }
     }
-  }
-  s = wave_sum64(s);
-  if ((tid & 63) == 0) sm_sum[w] = s;
-  __syncthreads();
-  if (tid == 0) {
-    for (int q = 1; q < kStatThreads / 64; ++q) s += sm_sum[q];
-    a.maxes[blockIdx.x] = m;
-    a.sums[blockIdx.x] = s;
+    s = wave_sum64(s);
+    if (l == 0) {
+      a.maxes[i] = m;
+      a.sums[i] = s;
+    }
+    if (next >= total) return;
+    i = next;
   }
 }
 
@@ -236,7 +272,7 @@ __device__ __forceinline__ double chunk_sum(double s, float m, double mc, double
 // The deciding position of sequence b, by a whole workgroup: every row's chunks joined
 // (16 lanes a row), then the drafts' tests; the lowest that fails decides. sm: rows
 // doubles, then rows floats.
-template <typename E, int THREADS>
+template <typename E>
 __device__ __forceinline__ SamplePick decide(const SampleArgs& a, int b, double rate, double* sm_s,
                                              int* sm_acc) {
   float* sm_m = reinterpret_cast<float*>(sm_s + a.rows);
@@ -265,11 +301,10 @@ __device__ __forceinline__ SamplePick decide(const SampleArgs& a, int b, double 
   float lp0 = 0, lq0 = 0, u0 = 0;
   if (tid < a.k) fetch(tid, x0, lp0, lq0, u0);
   if (tid == 0) *sm_acc = a.k;
-  for (int r = tid >> 4; r < a.rows; r += THREADS / 16) {
+  for (int r = tid >> 4; r < a.rows; r += kThreads / 16) {
     const size_t at = (static_cast<size_t>(b) * a.rows + r) * a.chunks;
-    // the first chunks of the lanes stay in registers: 32 chunks are a vocabulary of
-    // 262144 at full chunk size
-    constexpr int KEEP = 2;
+    // the lanes' first chunks stay in registers: 80 are a vocabulary of 163840
+    constexpr int KEEP = 5;
     float m[KEEP], M = -INFINITY;
     double s[KEEP], S = 0.0;
 #pragma unroll
@@ -294,7 +329,7 @@ __device__ __forceinline__ SamplePick decide(const SampleArgs& a, int b, double 
   }
   __syncthreads();
   if (tid < a.k) test(tid, x0, lp0, lq0, u0);
-  for (int j = tid + THREADS; j < a.k; j += THREADS) {
+  for (int j = tid + kThreads; j < a.k; j += kThreads) {
     fetch(j, x0, lp0, lq0, u0);
     test(j, x0, lp0, lq0, u0);
   }
@@ -333,56 +368,48 @@ __device__ __forceinline__ void rest_weights(const SampleArgs& a, const SamplePi
   }
 }
 
-// Grid: sequences x chunks, chunks fastest (drafts with probabilities only).
-template <typename E, int NV>
-__global__ __launch_bounds__(kStatThreads) void sample_rest_kernel(SampleArgs a) {
-  constexpr int N = kVec<E>;
+// Grid: sequences x groups of kWaves chunks, a chunk per wave (drafts with
+// probabilities only).
+template <typename E>
+__global__ __launch_bounds__(kThreads) void sample_rest_kernel(SampleArgs a) {
+  constexpr int N = Piece<E>::N, NV = Piece<E>::NV;
   extern __shared__ double sm_rows[];
-  __shared__ double sm_sum[kStatThreads / 64];
   __shared__ int sm_acc;
-  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63;
-  const int b = blockIdx.x / a.chunks, ch = blockIdx.x - b * a.chunks;
+  const int l = threadIdx.x & 63, groups = cdiv(a.chunks, kWaves);
+  const int b = blockIdx.x / groups;
+  const int ch = (blockIdx.x - b * groups) * kWaves + (threadIdx.x >> 6);
   const double rate = sample_rate(a, b);
-  const SamplePick p = decide<E, kStatThreads>(a, b, rate, sm_rows, &sm_acc);
-  const bool both = p.n_acc < a.k;
-  if (!both) {
-    // every draft stands: the chunk's sum is what the stats launch left
-    if (tid == 0) {
-      const size_t at = (static_cast<size_t>(b) * a.rows + a.k) * a.chunks + ch;
-      a.rest[blockIdx.x] = chunk_sum(a.sums[at], a.maxes[at], center(p.mp), rate);
-      if (ch == 0) a.picks[b] = p;
-    }
-    return;
-  }
-  const E* tr = logits_row<E>(a, b, p.n_acc);
-  const E* dr = logits_row<E>(a, b, a.k + 1 + p.n_acc);
-  float x[NV][N], y[NV][N];
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const int i0 = (ch * NV + v) * kStatThreads * N + tid * N;
-    load_logits<E>(tr, i0, a.V, x[v]);
-    load_logits<E>(dr, i0, a.V, y[v]);
-  }
+  const SamplePick p = decide<E>(a, b, rate, sm_rows, &sm_acc);
+  if (ch == 0 && l == 0) a.picks[b] = p;
+  if (ch >= a.chunks) return;
   double s = 0.0;
+  if (p.n_acc < a.k) {
+    Piece<E> x, y;
+    x.load(logits_row<E>(a, b, p.n_acc), ch, l, a.V);
+    y.load(logits_row<E>(a, b, a.k + 1 + p.n_acc), ch, l, a.V);
 #pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    double r[N];
-    rest_weights<E>(a, p, true, x[v], y[v], (ch * NV + v) * kStatThreads * N + tid * N, rate, r);
+    for (int v = 0; v < NV; ++v) {
+      float lp[N], lq[N];
+      double r[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) s += r[e];
+      for (int e = 0; e < N; ++e) {
+        lp[e] = logit<E>(x.x[v], e);
+        lq[e] = logit<E>(y.x[v], e);
+      }
+      rest_weights<E>(a, p, true, lp, lq, (ch * NV + v) * 64 * N + l * N, rate, r);
+#pragma unroll
+      for (int e = 0; e < N; ++e) s += r[e];
+    }
+    s = wave_sum64(s);
+  } else {
+    // every draft stands: the chunk's sum is what the stats launch left
+    const size_t at = (static_cast<size_t>(b) * a.rows + a.k) * a.chunks + ch;
+    s = chunk_sum(a.sums[at], a.maxes[at], center(p.mp), rate);
   }
-  s = wave_sum64(s);
-  if (l == 0) sm_sum[w] = s;
-  __syncthreads();
-  if (tid == 0) {
-    for (int q = 1; q < kStatThreads / 64; ++q) s += sm_sum[q];
-    a.rest[blockIdx.x] = s;
-    if (ch == 0) a.picks[b] = p;
-  }
+  if (l == 0) a.rest[static_cast<size_t>(b) * a.chunks + ch] = s;
 }
 
 // Exclusive prefix of a value over the workgroup's threads, and the total.
-template <int THREADS>
 __device__ __forceinline__ double block_prefix(double v, double* sm, int tid, double& total) {
   const int l = tid & 63, w = tid >> 6;
   double inc = v;
@@ -396,7 +423,7 @@ __device__ __forceinline__ double block_prefix(double v, double* sm, int tid, do
   double before = 0.0;
   total = 0.0;
 #pragma unroll
-  for (int q = 0; q < THREADS / 64; ++q) {
+  for (int q = 0; q < kWaves; ++q) {
     if (q == w) before = total;
     total += sm[q];
   }
@@ -404,59 +431,73 @@ __device__ __forceinline__ double block_prefix(double v, double* sm, int tid, do
   return before + inc - v;
 }
 
-// Grid: sequences. A chunk is `per` ids.
+// Grid: sequences.
 template <typename E>
-__global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a, int per) {
-  constexpr int N = kVec<E>, T = kPickThreads;
+__global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
+  constexpr int N = kVec<E>, NV = kChunk / (kThreads * N);  // a thread's ids are consecutive
   extern __shared__ double sm_rows[];
-  __shared__ double sm[T / 64], sm_ahead, sm_skip;
+  __shared__ double sm[kWaves], sm_ahead;
   __shared__ int sm_acc, sm_at, sm_last;
   const int tid = threadIdx.x, b = blockIdx.x;
   const double rate = sample_rate(a, b);
-  SamplePick p = a.draft ? a.picks[b] : decide<E, T>(a, b, rate, sm_rows, &sm_acc);
+  SamplePick p = a.draft ? a.picks[b] : decide<E>(a, b, rate, sm_rows, &sm_acc);
   bool both = a.draft && p.n_acc < a.k;
-  const double u = a.u_sample[b];
+  const double u = a.u_sample[b], mc = center(p.mp);
   const size_t prow = (static_cast<size_t>(b) * a.rows + p.n_acc) * a.chunks;
   const E* tr = logits_row<E>(a, b, p.n_acc);
   const E* dr = both ? logits_row<E>(a, b, a.k + 1 + p.n_acc) : tr;
-  const double mc = center(p.mp);
+
+  // r of this thread's ids of chunk c
+  const auto ids_of = [&](int c, int v) { return c * kChunk + (tid * NV + v) * N; };
+  const auto weights_of = [&](int c, double (&r)[NV][N]) {
+    float x[NV][N], y[NV][N];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      load_logits<E>(tr, ids_of(c, v), a.V, x[v]);
+      if (both) load_logits<E>(dr, ids_of(c, v), a.V, y[v]);
+    }
+    double mine = 0.0;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      rest_weights<E>(a, p, both, x[v], both ? y[v] : x[v], ids_of(c, v), rate, r[v]);
+#pragma unroll
+      for (int e = 0; e < N; ++e) mine += r[v][e];
+    }
+    return mine;
+  };
 
   // the chunk that an id left out lies in is summed again without it (taking its weight
   // off the sum would leave that sum's rounding error, of any size against the rest)
   const bool skips = p.skip >= 0 && p.skip < a.V;
-  const int skip_chunk = skips ? p.skip / per : -1;
+  const int skip_chunk = skips ? p.skip / kChunk : -1;
+  double skip_sum = 0.0;
   if (skips) {
-    double s = 0.0, all;
-    for (int i0 = skip_chunk * per + tid * N; i0 < min((skip_chunk + 1) * per, a.V); i0 += T * N) {
-      float x[N];
-      double r[N];
-      load_logits<E>(tr, i0, a.V, x);
-      rest_weights<E>(a, p, false, x, x, i0, rate, r);
-#pragma unroll
-      for (int e = 0; e < N; ++e) s += r[e];
-    }
-    block_prefix<T>(s, sm, tid, all);
-    if (tid == 0) sm_skip = all;
-    __syncthreads();
+    double r[NV][N];
+    block_prefix(weights_of(skip_chunk, r), sm, tid, skip_sum);
   }
   // plain: p itself, where p - q or p without the draft leaves nothing
   const auto sum_of = [&](int c, bool plain) {
     if (c >= a.chunks) return 0.0;
     if (both && !plain) return a.rest[static_cast<size_t>(b) * a.chunks + c];
-    if (c == skip_chunk && !plain) return sm_skip;
+    if (c == skip_chunk && !plain) return skip_sum;
     return chunk_sum(a.sums[prow + c], a.maxes[prow + c], mc, rate);
   };
-  const auto total_of = [&](bool plain) {
-    double t = 0.0, all;
-    for (int c = tid; c < a.chunks; c += T) t += sum_of(c, plain);
-    block_prefix<T>(t, sm, tid, all);
-    return all;
-  };
-  double R = total_of(false);
   bool plain = false;
+  double first_sum = sum_of(tid, false), first_before, R = 0.0;  // the first kThreads chunks
+  const auto total_of = [&]() {
+    first_before = block_prefix(first_sum, sm, tid, R);
+    if (a.chunks > kThreads) {
+      double t = 0.0, more;
+      for (int c = tid + kThreads; c < a.chunks; c += kThreads) t += sum_of(c, plain);
+      block_prefix(t, sm, tid, more);
+      R += more;
+    }
+  };
+  total_of();
   if (R == 0.0 && (both || skips)) {
     plain = true;
-    R = total_of(true);
+    first_sum = sum_of(tid, true);
+    total_of();
   }
   int32_t token = -1;
   if (rate > 0.0 && R > 0.0) {
@@ -469,65 +510,56 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a,
     }
     __syncthreads();
     double carry = 0.0;
-    for (int c0 = 0; c0 < a.chunks; c0 += T) {
-      const double v = sum_of(c0 + tid, plain);
-      double all;
-      const double before = carry + block_prefix<T>(v, sm, tid, all);
-      if (v > 0.0) {
-        atomicMax(&sm_last, c0 + tid);
-        if (before + v > place) atomicMin(&sm_at, c0 + tid);
+    int c = -1;
+    for (int c0 = 0; c0 < a.chunks; c0 += kThreads) {
+      double v = first_sum, before = first_before, all = 0.0;
+      if (a.chunks > kThreads) {
+        v = sum_of(c0 + tid, plain);
+        before = carry + block_prefix(v, sm, tid, all);
+      }
+      const uint64_t some = __ballot(v > 0.0), past = __ballot(v > 0.0 && before + v > place);
+      if ((tid & 63) == 0) {
+        const int w0 = c0 + tid;
+        if (some) atomicMax(&sm_last, w0 + 63 - __builtin_clzll(some));
+        if (past) atomicMin(&sm_at, w0 + __builtin_ctzll(past));
       }
       __syncthreads();
-      const int c = sm_at < a.chunks ? sm_at : sm_last;
+      c = sm_at < a.chunks ? sm_at : sm_last;
       if (c == c0 + tid) sm_ahead = before;
       carry += all;
       if (sm_at < a.chunks) break;
     }
     __syncthreads();
-    const int c = sm_at < a.chunks ? sm_at : sm_last;
-    const double ahead = sm_ahead;
-    __syncthreads();
     if (tid == 0) {
       sm_at = a.V;
       sm_last = -1;
     }
-    __syncthreads();
     if (plain) {
       both = false;
       p.skip = -1;
     }
-    double run = ahead;
-    for (int base = c * per; base < (c + 1) * per; base += T * N) {
-      const int i0 = base + tid * N;
-      float x[N], y[N];
-      double r[N], mine = 0.0, all;
+    double r[NV][N], all;
+    double at = block_prefix(weights_of(c, r), sm, tid, all) + sm_ahead;
+    int first = a.V, last = -1;
 #pragma unroll
-      for (int e = 0; e < N; ++e) x[e] = y[e] = -INFINITY;
-      if (i0 < (c + 1) * per) {
-        load_logits<E>(tr, i0, a.V, x);
-        if (both) load_logits<E>(dr, i0, a.V, y);
-      }
-      rest_weights<E>(a, p, both, x, y, i0, rate, r);
-#pragma unroll
-      for (int e = 0; e < N; ++e) mine += r[e];
-      double at = run + block_prefix<T>(mine, sm, tid, all);
-      int first = a.V, last = -1;
+    for (int v = 0; v < NV; ++v) {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        at += r[e];
-        if (r[e] > 0.0) {
-          last = i0 + e;
-          if (at > place && first == a.V) first = i0 + e;
+        at += r[v][e];
+        if (r[v][e] > 0.0) {
+          last = ids_of(c, v) + e;
+          if (at > place && first == a.V) first = last;
         }
       }
-      if (first < a.V) atomicMin(&sm_at, first);
-      if (last >= 0) atomicMax(&sm_last, last);
-      run += all;
     }
+    // (ids grow with the lane)
+    const uint64_t some = __ballot(last >= 0), past = __ballot(first < a.V);
+    if (some && (tid & 63) == 63 - __builtin_clzll(some)) atomicMax(&sm_last, last);
+    if (past && (tid & 63) == __builtin_ctzll(past)) atomicMin(&sm_at, first);
     __syncthreads();
     token = sm_at < a.V ? sm_at : sm_last;
   }
-  for (int j = tid; j <= a.k; j += T) {
+  for (int j = tid; j <= a.k; j += kThreads) {
     const int32_t d = j < a.k ? a.drafts[static_cast<size_t>(b) * a.k + j] : -1;
     a.emitted[static_cast<size_t>(b) * (a.k + 1) + j] =
         j < p.n_acc ? d : j == p.n_acc ? token : -1;
@@ -541,26 +573,18 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a,
   }
 }
 
-// Vectors a thread: chunks of 8192 logits, smaller ones where those leave compute
-// units without a workgroup.
-static int sample_vectors(long long rows, int V, int vec) {
-  const int most = 8192 / (kStatThreads * vec);
-  for (int nv = most; nv > 1; nv /= 2)
-    if (rows * cdiv(V, nv * kStatThreads * vec) >= 512) return nv;
-  return 1;
-}
+// Workgroups of the stats launch that the chip holds at once (8 per compute unit).
+constexpr int kStatGrid = 2048;
 
 struct SampleCfg {
-  int rows, nv, chunks;
+  int rows, chunks;
   size_t sums, maxes, rest, picks, bytes;  // offsets of the workspace's parts
 };
 
-static SampleCfg sample_cfg(int B, int k, int V, int dtype, bool draft) {
+static SampleCfg sample_cfg(int B, int k, int V, bool draft) {
   SampleCfg c{};
-  const int vec = dtype == KVE_DTYPE_BF16 ? 8 : 4;
   c.rows = draft ? 2 * k + 1 : k + 1;
-  c.nv = sample_vectors(static_cast<long long>(B) * c.rows, V, vec);
-  c.chunks = cdiv(V, c.nv * kStatThreads * vec);
+  c.chunks = cdiv(V, kChunk);
   const size_t parts = static_cast<size_t>(B) * c.rows * c.chunks;
   size_t at = 0;
   const auto take = [&](size_t n) {
@@ -576,16 +600,15 @@ static SampleCfg sample_cfg(int B, int k, int V, int dtype, bool draft) {
   return c;
 }
 
-template <typename E, int NV>
+template <typename E>
 static void launch_sample(const SampleArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((sample_stats_kernel<E, NV>), dim3(a.B * a.rows * a.chunks),
-                     dim3(kStatThreads), 0, st, a);
+  const int stats = std::min(kStatGrid, cdiv(a.B * a.rows * a.chunks, kWaves));
+  hipLaunchKernelGGL(sample_stats_kernel<E>, dim3(stats), dim3(kThreads), 0, st, a);
   const size_t lds = static_cast<size_t>(a.rows) * (sizeof(double) + sizeof(float));
   if (a.draft)
-    hipLaunchKernelGGL((sample_rest_kernel<E, NV>), dim3(a.B * a.chunks), dim3(kStatThreads), lds, st,
-                       a);
-  hipLaunchKernelGGL(sample_pick_kernel<E>, dim3(a.B), dim3(kPickThreads), lds, st, a,
-                     NV * kStatThreads * kVec<E>);
+    hipLaunchKernelGGL(sample_rest_kernel<E>, dim3(a.B * cdiv(a.chunks, kWaves)), dim3(kThreads), lds,
+                       st, a);
+  hipLaunchKernelGGL(sample_pick_kernel<E>, dim3(a.B), dim3(kThreads), lds, st, a);
 }
 
 }  // namespace kve
@@ -599,8 +622,8 @@ extern "C" size_t kve_sample_workspace_bytes(int num_seqs, int k, int vocab, int
   if (num_seqs <= 0 || k < 0 || k > kSampleMaxDrafts || vocab <= 0 ||
       (dtype != KVE_DTYPE_BF16 && dtype != KVE_DTYPE_F32))
     return 0;
-  return std::max(sample_cfg(num_seqs, k, vocab, dtype, true).bytes,
-                  sample_cfg(num_seqs, k, vocab, dtype, false).bytes);
+  return std::max(sample_cfg(num_seqs, k, vocab, true).bytes,
+                  sample_cfg(num_seqs, k, vocab, false).bytes);
 }
 
 extern "C" int kve_sample_verify(const void* target, int64_t target_seq_stride,
@@ -628,7 +651,7 @@ extern "C" int kve_sample_verify(const void* target, int64_t target_seq_stride,
   KVE_REQUIRE(((reinterpret_cast<uintptr_t>(target) | reinterpret_cast<uintptr_t>(draft)) &
                (esz - 1)) == 0,
               "kve_sample_verify: logits are not aligned to their type");
-  const SampleCfg c = sample_cfg(num_seqs, k, vocab, dtype, draft != nullptr && k > 0);
+  const SampleCfg c = sample_cfg(num_seqs, k, vocab, draft != nullptr && k > 0);
   KVE_REQUIRE(static_cast<long long>(num_seqs) * c.rows * c.chunks < (1ll << 31),
               "kve_sample_verify: %d x %d rows of %d too large for one launch", num_seqs, c.rows,
               vocab);
@@ -667,15 +690,7 @@ extern "C" int kve_sample_verify(const void* target, int64_t target_seq_stride,
   a.rest = reinterpret_cast<double*>(ws + c.rest);
   a.picks = reinterpret_cast<SamplePick*>(ws + c.picks);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == KVE_DTYPE_BF16) {
-    if (c.nv == 4) launch_sample<uint16_t, 4>(a, st);
-    else if (c.nv == 2) launch_sample<uint16_t, 2>(a, st);
-    else launch_sample<uint16_t, 1>(a, st);
-  } else {
-    if (c.nv == 8) launch_sample<float, 8>(a, st);
-    else if (c.nv == 4) launch_sample<float, 4>(a, st);
-    else if (c.nv == 2) launch_sample<float, 2>(a, st);
-    else launch_sample<float, 1>(a, st);
-  }
+  if (dtype == KVE_DTYPE_BF16) launch_sample<uint16_t>(a, st);
+  else launch_sample<float>(a, st);
   return check_launch("kve_sample_verify");
 }
