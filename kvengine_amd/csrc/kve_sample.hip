@@ -7,21 +7,33 @@
 // drawn from r = max(p - q, 0), else, after the last draft, from p, by inversion: the
 // lowest id whose running sum exceeds u * sum(r).
 //
-// Everything is in 64 bits. The drawn id is a place among up to 150 000 running sums,
-// and an error of e in the sums moves a draw with a probability of about 2 V e: 32-bit
+// The draw is in 64 bits. The drawn id is a place among up to 150 000 running sums, and
+// an error of e in the sums moves a draw with a probability of about 2 V e: 32-bit
 // exponentials (6e-8) would answer one or two draws in a hundred differently from the
-// definition, 64-bit ones none. A 64-bit FMA costs a wave the same four cycles here as
-// an unpacked 32-bit one, so the price is the polynomial's length.
+// definition, these (4e-14) one in 10^8. A weight costs a wave 86 cycles in 64 bits and
+// 22 in 32 bits (its logit's loads 35, at the chip's copy rate), so only the logits of
+// the position that decides are taken in 64 bits: which position that is follows from
+// 32-bit sums, whose error is known, and where a test lies within it (2 in 10^5 tests)
+// from that row's 64-bit ones.
 //
-// Launches, each a dependency of the next over the whole vocabulary:
-//  stats   every (row, chunk of 2048 logits), a chunk per wave: maximum and sum of
-//          2^((l - max) c), c = log2(e) / T, the chunk held in registers between the two
-//  rest    every (sequence, chunk), where drafts have probabilities: the rows' chunks
-//          joined, the accept tests, and the chunk's sum of r at the deciding position
-//          (one row of each side, again)
-//  pick    every sequence: the chunk that holds the drawn place, then its elements
+// Launches, each a dependency of the next over the whole vocabulary; a chunk is 2048
+// logits, one per wave:
+//  stats   every (row, chunk): maximum, and the sum of 2^((l - max) c) in 32 bits,
+//          c = log2(e) / T. Without drafts (k = 0) there is no test, and it is the
+//          64-bit sum that the draw takes.
+//  rest    every (sequence, chunk), k > 0: the rows' chunks joined, the tests, and at the
+//          deciding position the chunk's 64-bit sums
+//  pick    every sequence: the exact ratio of the two rows' sums, the chunk that holds
+//          the drawn place, then its ids
 // The stats launch reads all logits once and bounds the call; the others re-read one
-// position's rows, or one chunk.
+// position's rows, and one chunk.
+//
+// The rest without its own pass over the vocabulary. With e = 2^((target - mp) c), g the
+// draft's and L = sum(e) / sum(g), r is max(e - L g, 0) / sum(e). L is only known after
+// a pass, but to 2^-16 from the 32-bit sums (L'). So the pass sums e - L' g over the ids
+// where it is positive, and g over the same ids: the rest is the first minus (L - L')
+// times the second. An id where |e - L' g| <= 2^-16 L' g may be on either side; its chunk
+// is marked and summed again by `pick` (an id or two of 150 000, or all where p = q).
 
 #include "kve_common.h"
 
@@ -30,12 +42,19 @@
 
 namespace kve {
 
-// The deciding position of a sequence: r = 2^((l - mp) c) of the target alone (both
-// false; `skip`, a rejected draft of no distribution, left out) or max(p - q, 0).
+// The deciding position of a sequence.
 struct SamplePick {
-  double ip, iq;  // 1 / sum over the row, of the target and the draft
-  float mp, mq;   // row maxima
-  int n_acc, skip;  // skip: id left out, or -1
+  double lam;       // L' above; drafts with probabilities, not all accepted
+  float mp, mq;     // row maxima of the target and the draft
+  int n_acc, skip;  // skip: id left out (a rejected draft without a distribution), or -1
+};
+
+// What `rest` leaves of a chunk at the deciding position.
+struct RestSums {
+  double e, g;      // sums over the chunk
+  double over, gp;  // sum of e - L' g over the ids where it is positive, and of their g
+                    // (gp < 0: some id is undecided, the chunk is to be summed again);
+                    // without a draft's distribution: sum of e without `skip`, 0
 };
 
 struct SampleArgs {
@@ -47,9 +66,9 @@ struct SampleArgs {
   const int32_t *lens, *seq_rows;
   int num_rows, B, k, V, rows, chunks;  // rows per sequence: k + 1 target, then k draft
   int32_t *n_acc, *emitted, *keep;
-  double* sums;   // [B][rows][chunks]: sum of the chunk relative to its maximum
-  float* maxes;   // [B][rows][chunks]
-  double* rest;   // [B][chunks]: sum of r over the chunk
+  double* sums;    // [B][rows][chunks]: sum of the chunk relative to its maximum
+  float* maxes;    // [B][rows][chunks]
+  RestSums* rest;  // [B][chunks]
   SamplePick* picks;  // [B]
 };
 
@@ -101,6 +120,10 @@ __device__ __forceinline__ double weight_near(float l, double m, double rate) {
   const double t = fma(d, rate, kShift);
   const double p = exp2_poly(fma(d, rate, kShift - t));
   return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
+}
+
+__device__ __forceinline__ bool is_near(float l, double m, double rate) {
+  return (static_cast<double>(l) - m) * rate >= kNear;  // (false for a NaN)
 }
 
 // What weights are taken against: a maximum of -inf (no mass) counts as 0.
@@ -206,7 +229,7 @@ struct Piece {
 
 // Every wave takes chunks (sequences x rows x chunks, chunks fastest) wave, wave +
 // waves of the grid, ..., the next one loading while one is summed.
-template <typename E>
+template <typename E, bool WIDE>
 __global__ __launch_bounds__(kThreads) void sample_stats_kernel(SampleArgs a) {
   constexpr int N = Piece<E>::N, NV = Piece<E>::NV;
   const int l = threadIdx.x & 63;
@@ -232,26 +255,41 @@ __global__ __launch_bounds__(kThreads) void sample_stats_kernel(SampleArgs a) {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         m = max_nan(m, logit<E>(x.x[v], e));
-        lo = min_nan(lo, logit<E>(x.x[v], e));
+        if (WIDE) lo = min_nan(lo, logit<E>(x.x[v], e));
       }
     }
     m = wave_max(m);
-    const double c = center(m);
     double s = 0.0;
-    if (__all((static_cast<double>(lo) - c) * rate >= kNear)) {
+    if constexpr (WIDE) {
+      const double c = center(m);
+      if (__all(is_near(lo, c, rate))) {
 #pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        x.hide(v);
+        for (int v = 0; v < NV; ++v) {
+          x.hide(v);
 #pragma unroll
-        for (int e = 0; e < N; ++e) s += weight_near(logit<E>(x.x[v], e), c, rate);
+          for (int e = 0; e < N; ++e) s += weight_near(logit<E>(x.x[v], e), c, rate);
+        }
+      } else {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          x.hide(v);
+#pragma unroll
+          for (int e = 0; e < N; ++e) s += weight(logit<E>(x.x[v], e), c, rate);
+        }
       }
     } else {
+      // 32 bits: an exponent y is off by 3 roundings of it and 2^y by its instruction's, so
+      // the sum by 2^-23 (2 + 1.1 mean|y|), mean |y| being at most log2 of the vocabulary
+      // (an entropy) and a bit, and by a rounding of each of a lane's 32 additions:
+      // below 5e-6 of it (kMargin)
+      const float c = m == -INFINITY ? 0.0f : m, f = static_cast<float>(rate);
+      float p = 0.0f;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        x.hide(v);
 #pragma unroll
-        for (int e = 0; e < N; ++e) s += weight(logit<E>(x.x[v], e), c, rate);
+        for (int e = 0; e < N; ++e) p += __builtin_amdgcn_exp2f((logit<E>(x.x[v], e) - c) * f);
       }
+      s = p;
     }
     s = wave_sum64(s);
     if (l == 0) {
@@ -269,38 +307,42 @@ __device__ __forceinline__ double chunk_sum(double s, float m, double mc, double
   return m == -INFINITY ? s : s * weight(m, mc, rate);
 }
 
+// Sum of a value over the workgroup's threads, to each of them.
+__device__ __forceinline__ double block_sum(double v, double* sm, int tid) {
+  v = wave_sum64(v);
+  if ((tid & 63) == 0) sm[tid >> 6] = v;
+  __syncthreads();
+  double t = 0.0;
+#pragma unroll
+  for (int q = 0; q < kWaves; ++q) t += sm[q];
+  __syncthreads();
+  return t;
+}
+
+// How far apart u q and p (from 32-bit sums, relative to p) decide a test, and e and
+// L' g an id's sign: more than the two sums, 5e-6 each, can be off (1e-5).
+constexpr double kMargin = 1.0 / 65536;
+
 // The deciding position of sequence b, by a whole workgroup: every row's chunks joined
-// (16 lanes a row), then the drafts' tests; the lowest that fails decides. sm: rows
-// doubles, then rows floats.
+// (16 lanes a row), then the drafts' tests, a draft per thread; the lowest that fails
+// decides. sm_s: rows doubles, then rows floats.
 template <typename E>
 __device__ __forceinline__ SamplePick decide(const SampleArgs& a, int b, double rate, double* sm_s,
-                                             int* sm_acc) {
+                                             double* sm, int* sm_first) {
   float* sm_m = reinterpret_cast<float*>(sm_s + a.rows);
   const int tid = threadIdx.x, l16 = tid & 15;
-  const auto test = [&](int j, int x, float lp, float lq, float u) {
-    bool ok = false;
+  // the drafts' logits, asked for before the statistics arrive
+  int x = -1;
+  float lp = 0, lq = 0;
+  double u = 0;
+  if (tid < a.k) {
+    x = a.drafts[static_cast<size_t>(b) * a.k + tid];
+    u = a.u_accept[static_cast<size_t>(b) * a.k + tid];
     if (x >= 0 && x < a.V) {
-      const double p = weight(lp, center(sm_m[j]), rate) / sm_s[j];
-      const int r = a.k + 1 + j;
-      const double q = a.draft ? weight(lq, center(sm_m[r]), rate) / sm_s[r] : 1.0;
-      ok = static_cast<double>(u) * q < p;
+      lp = to_f32(logits_row<E>(a, b, tid)[x]);
+      if (a.draft) lq = to_f32(logits_row<E>(a, b, a.k + 1 + tid)[x]);
     }
-    if (!ok) atomicMin(sm_acc, j);
-  };
-  const auto fetch = [&](int j, int& x, float& lp, float& lq, float& u) {
-    x = a.drafts[static_cast<size_t>(b) * a.k + j];
-    u = a.u_accept[static_cast<size_t>(b) * a.k + j];
-    lp = lq = 0.0f;
-    if (x >= 0 && x < a.V) {
-      lp = to_f32(logits_row<E>(a, b, j)[x]);
-      if (a.draft) lq = to_f32(logits_row<E>(a, b, a.k + 1 + j)[x]);
-    }
-  };
-  // (asked for before the statistics arrive)
-  int x0 = -1;
-  float lp0 = 0, lq0 = 0, u0 = 0;
-  if (tid < a.k) fetch(tid, x0, lp0, lq0, u0);
-  if (tid == 0) *sm_acc = a.k;
+  }
   for (int r = tid >> 4; r < a.rows; r += kThreads / 16) {
     const size_t at = (static_cast<size_t>(b) * a.rows + r) * a.chunks;
     // the lanes' first chunks stay in registers: 80 are a vocabulary of 163840
@@ -328,85 +370,138 @@ __device__ __forceinline__ SamplePick decide(const SampleArgs& a, int b, double 
     }
   }
   __syncthreads();
-  if (tid < a.k) test(tid, x0, lp0, lq0, u0);
-  for (int j = tid + kThreads; j < a.k; j += kThreads) {
-    fetch(j, x0, lp0, lq0, u0);
-    test(j, x0, lp0, lq0, u0);
+  // 0: stands, 1: falls (a NaN too), 2: too near for 32-bit sums. Temperatures whose
+  // exponents leave 32 bits are always too near.
+  int state = 0;
+  const int rp = tid, rq = a.k + 1 + tid;
+  if (tid < a.k) {
+    state = 1;
+    if (x >= 0 && x < a.V) {
+      const double p = weight(lp, center(sm_m[rp]), rate) / sm_s[rp];
+      const double q = a.draft ? weight(lq, center(sm_m[rq]), rate) / sm_s[rq] : 1.0;
+      const bool coarse = !(rate > 1e-30 && rate < 1e30);
+      if (p > 0.0 && (coarse || fabs(u * q - p) <= kMargin * p)) state = 2;
+      else if (u * q < p) state = 0;
+      if (coarse) state = 2;
+    }
   }
-  __syncthreads();
-  const int j = rate > 0.0 ? *sm_acc : 0;
+  for (;;) {
+    if (tid == 0) *sm_first = 2 * a.k;
+    __syncthreads();
+    if (tid < a.k && state) atomicMin(sm_first, 2 * tid + (state == 2));
+    __syncthreads();
+    const int first = *sm_first;
+    __syncthreads();
+    if (!(first & 1)) break;
+    // the test in 64 bits: the two rows summed by this workgroup
+    const int j = first >> 1;
+    const auto row_sum64 = [&](int r) {
+      const E* row = logits_row<E>(a, b, r);
+      const double mc = center(sm_m[r]);
+      double s = 0.0;
+      for (int i0 = tid * kVec<E>; i0 < a.V; i0 += kThreads * kVec<E>) {
+        float y[kVec<E>];
+        load_logits<E>(row, i0, a.V, y);
+#pragma unroll
+        for (int e = 0; e < kVec<E>; ++e) s += weight(y[e], mc, rate);
+      }
+      return block_sum(s, sm, tid);
+    };
+    const double sp = row_sum64(j), sq = a.draft ? row_sum64(a.k + 1 + j) : 1.0;
+    if (tid == j) {
+      const double p = weight(lp, center(sm_m[rp]), rate) / sp;
+      const double q = a.draft ? weight(lq, center(sm_m[rq]), rate) / sq : 1.0;
+      state = u * q < p ? 0 : 1;
+    }
+  }
+  const int j = rate > 0.0 ? *sm_first >> 1 : 0;
   const bool both = a.draft && j < a.k;
   SamplePick p;
   p.n_acc = j;
   p.mp = sm_m[j];
-  p.ip = 1.0 / sm_s[j];
   p.mq = both ? sm_m[a.k + 1 + j] : 0.0f;
-  p.iq = both ? 1.0 / sm_s[a.k + 1 + j] : 0.0;
+  p.lam = both ? sm_s[j] / sm_s[a.k + 1 + j] : 0.0;
   p.skip = !a.draft && j < a.k ? a.drafts[static_cast<size_t>(b) * a.k + j] : -1;
   return p;
 }
 
-// r of the N ids from i0 on at the deciding position; ids past the vocabulary have 0.
-template <typename E>
-__device__ __forceinline__ void rest_weights(const SampleArgs& a, const SamplePick& p, bool both,
-                                             const float (&lp)[kVec<E>], const float (&lq)[kVec<E>],
-                                             int i0, double rate, double (&r)[kVec<E>]) {
-  // both products rounded, so that equal probabilities leave exactly nothing
-#pragma clang fp contract(off)
-  const double mp = center(p.mp), mq = center(p.mq);
-#pragma unroll
-  for (int e = 0; e < kVec<E>; ++e) {
-    const double w = weight(lp[e], mp, rate);
-    if (both) {
-      const double d = w * p.ip - weight(lq[e], mq, rate) * p.iq;
-      r[e] = d > 0.0 ? d : 0.0 * d;  // (a NaN stays)
-    } else {
-      r[e] = i0 + e == p.skip ? 0.0 : w;
-    }
-    // past the end both logits are -inf; 0 * (1 / sum) of a row without mass is not 0
-    if (i0 + e >= a.V) r[e] = 0.0;
-  }
-}
-
-// Grid: sequences x groups of kWaves chunks, a chunk per wave (drafts with
-// probabilities only).
+// Grid: sequences x groups of kWaves chunks, a chunk per wave.
 template <typename E>
 __global__ __launch_bounds__(kThreads) void sample_rest_kernel(SampleArgs a) {
   constexpr int N = Piece<E>::N, NV = Piece<E>::NV;
   extern __shared__ double sm_rows[];
-  __shared__ int sm_acc;
+  __shared__ double sm[kWaves];
+  __shared__ int sm_first;
   const int l = threadIdx.x & 63, groups = cdiv(a.chunks, kWaves);
   const int b = blockIdx.x / groups;
   const int ch = (blockIdx.x - b * groups) * kWaves + (threadIdx.x >> 6);
   const double rate = sample_rate(a, b);
-  const SamplePick p = decide<E>(a, b, rate, sm_rows, &sm_acc);
+  const SamplePick p = decide<E>(a, b, rate, sm_rows, sm, &sm_first);
   if (ch == 0 && l == 0) a.picks[b] = p;
   if (ch >= a.chunks) return;
-  double s = 0.0;
-  if (p.n_acc < a.k) {
-    Piece<E> x, y;
-    x.load(logits_row<E>(a, b, p.n_acc), ch, l, a.V);
-    y.load(logits_row<E>(a, b, a.k + 1 + p.n_acc), ch, l, a.V);
+  const bool both = a.draft && p.n_acc < a.k;
+  const double mp = center(p.mp), mq = center(p.mq);
+  Piece<E> x, y;
+  x.load(logits_row<E>(a, b, p.n_acc), ch, l, a.V);
+  if (both) y.load(logits_row<E>(a, b, a.k + 1 + p.n_acc), ch, l, a.V);
+  else y = x;
+  float lo_p = INFINITY, lo_q = INFINITY;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      lo_p = min_nan(lo_p, logit<E>(x.x[v], e));
+      lo_q = min_nan(lo_q, logit<E>(y.x[v], e));
+    }
+  }
+  double se = 0.0, sg = 0.0, over = 0.0, gp = 0.0;
+  bool undecided = false;
+  const double edge = kMargin * p.lam;
+  const auto sum_both = [&](auto&& w) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      float lp[N], lq[N];
-      double r[N];
+      x.hide(v);
+      y.hide(v);
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        lp[e] = logit<E>(x.x[v], e);
-        lq[e] = logit<E>(y.x[v], e);
+        const double we = w(logit<E>(x.x[v], e), mp), wg = w(logit<E>(y.x[v], e), mq);
+        const double d = we - p.lam * wg;
+        se += we;
+        sg += wg;
+        undecided |= wg > 0.0 && !(fabs(d) > edge * wg);
+        over += d > 0.0 ? d : 0.0;
+        gp += d > 0.0 ? wg : 0.0;
       }
-      rest_weights<E>(a, p, true, lp, lq, (ch * NV + v) * 64 * N + l * N, rate, r);
-#pragma unroll
-      for (int e = 0; e < N; ++e) s += r[e];
     }
-    s = wave_sum64(s);
+  };
+  const auto sum_one = [&](auto&& w) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      x.hide(v);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const double we = w(logit<E>(x.x[v], e), mp);
+        se += we;
+        over += (ch * NV + v) * 64 * N + l * N + e == p.skip ? 0.0 : we;
+      }
+    }
+  };
+  const auto near = [&](float t, double m) { return weight_near(t, m, rate); };
+  const auto any = [&](float t, double m) { return weight(t, m, rate); };
+  if (both) {
+    if (__all(is_near(lo_p, mp, rate) && is_near(lo_q, mq, rate))) sum_both(near);
+    else sum_both(any);
   } else {
-    // every draft stands: the chunk's sum is what the stats launch left
-    const size_t at = (static_cast<size_t>(b) * a.rows + a.k) * a.chunks + ch;
-    s = chunk_sum(a.sums[at], a.maxes[at], center(p.mp), rate);
+    if (__all(is_near(lo_p, mp, rate))) sum_one(near);
+    else sum_one(any);
   }
-  if (l == 0) a.rest[static_cast<size_t>(b) * a.chunks + ch] = s;
+  RestSums r{wave_sum64(se), 0.0, wave_sum64(over), 0.0};
+  if (both) {
+    r.g = wave_sum64(sg);
+    r.gp = wave_sum64(gp);
+    if (__any(undecided)) r.gp = -1.0;
+  }
+  if (l == 0) a.rest[static_cast<size_t>(b) * a.chunks + ch] = r;
 }
 
 // Exclusive prefix of a value over the workgroup's threads, and the total.
@@ -431,25 +526,59 @@ __device__ __forceinline__ double block_prefix(double v, double* sm, int tid, do
   return before + inc - v;
 }
 
-// Grid: sequences.
+// Grid: sequences. Thread t holds the sums of `per` consecutive chunks (one up to a
+// vocabulary of 524288).
 template <typename E>
 __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
   constexpr int N = kVec<E>, NV = kChunk / (kThreads * N);  // a thread's ids are consecutive
-  extern __shared__ double sm_rows[];
   __shared__ double sm[kWaves], sm_ahead;
-  __shared__ int sm_acc, sm_at, sm_last;
-  const int tid = threadIdx.x, b = blockIdx.x;
-  const double rate = sample_rate(a, b);
-  SamplePick p = a.draft ? a.picks[b] : decide<E>(a, b, rate, sm_rows, &sm_acc);
+  __shared__ float sm_max[kWaves];
+  __shared__ uint64_t sm_marked[kWaves];
+  __shared__ int sm_at, sm_last;
+  const int tid = threadIdx.x, w = tid >> 6, b = blockIdx.x;
+  const double rate = sample_rate(a, b), u = a.u_sample[b];
+  const int per = cdiv(a.chunks, kThreads), c0 = min(tid * per, a.chunks),
+            c1 = min(c0 + per, a.chunks);
+  const RestSums* rest = a.rest + static_cast<size_t>(b) * a.chunks;
+  SamplePick p{0.0, 0.0f, 0.0f, 0, -1};
+  const float* maxes = a.maxes + static_cast<size_t>(b) * a.chunks;
+  const double* sums = a.sums + static_cast<size_t>(b) * a.chunks;
+  if (a.k > 0) {
+    p = a.picks[b];
+  } else {
+    // the only row's maximum
+    float m = -INFINITY;
+    for (int c = c0; c < c1; ++c) m = max_nan(m, maxes[c]);
+    m = wave_max(m);
+    if ((tid & 63) == 0) sm_max[w] = m;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kWaves; ++q) m = max_nan(m, sm_max[q]);
+    p.mp = m;
+  }
   bool both = a.draft && p.n_acc < a.k;
-  const double u = a.u_sample[b], mc = center(p.mp);
-  const size_t prow = (static_cast<size_t>(b) * a.rows + p.n_acc) * a.chunks;
+  const double mp = center(p.mp), mq = center(p.mq);
   const E* tr = logits_row<E>(a, b, p.n_acc);
   const E* dr = both ? logits_row<E>(a, b, a.k + 1 + p.n_acc) : tr;
 
-  // r of this thread's ids of chunk c
+  // L of the two rows' 64-bit sums; no number, 0 or infinite where a row has no distribution
+  double lam = 0.0;
+  bool sound = true;
+  if (both) {
+    double se = 0.0, sg = 0.0;
+    for (int c = c0; c < c1; ++c) {
+      se += rest[c].e;
+      sg += rest[c].g;
+    }
+    se = block_sum(se, sm, tid);
+    lam = se / block_sum(sg, sm, tid);
+    sound = lam > 0.0 && lam < INFINITY;
+  }
+  // r (times sum(e)) of this thread's ids of chunk c, and their sum
   const auto ids_of = [&](int c, int v) { return c * kChunk + (tid * NV + v) * N; };
   const auto weights_of = [&](int c, double (&r)[NV][N]) {
+    // both products rounded, so that equal probabilities leave exactly nothing
+#pragma clang fp contract(off)
     float x[NV][N], y[NV][N];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -459,104 +588,108 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
     double mine = 0.0;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      rest_weights<E>(a, p, both, x[v], both ? y[v] : x[v], ids_of(c, v), rate, r[v]);
 #pragma unroll
-      for (int e = 0; e < N; ++e) mine += r[v][e];
+      for (int e = 0; e < N; ++e) {
+        const int id = ids_of(c, v) + e;
+        double t = weight(x[v][e], mp, rate);
+        if (both) {
+          t = t - lam * weight(y[v][e], mq, rate);
+          if (t < 0.0) t = 0.0;  // (a NaN stays)
+        } else if (id == p.skip) {
+          t = 0.0;
+        }
+        r[v][e] = id < a.V ? t : 0.0;
+        mine += r[v][e];
+      }
     }
     return mine;
   };
-
-  // the chunk that an id left out lies in is summed again without it (taking its weight
-  // off the sum would leave that sum's rounding error, of any size against the rest)
-  const bool skips = p.skip >= 0 && p.skip < a.V;
-  const int skip_chunk = skips ? p.skip / kChunk : -1;
-  double skip_sum = 0.0;
-  if (skips) {
-    double r[NV][N];
-    block_prefix(weights_of(skip_chunk, r), sm, tid, skip_sum);
-  }
-  // plain: p itself, where p - q or p without the draft leaves nothing
-  const auto sum_of = [&](int c, bool plain) {
-    if (c >= a.chunks) return 0.0;
-    if (both && !plain) return a.rest[static_cast<size_t>(b) * a.chunks + c];
-    if (c == skip_chunk && !plain) return skip_sum;
-    return chunk_sum(a.sums[prow + c], a.maxes[prow + c], mc, rate);
-  };
-  bool plain = false;
-  double first_sum = sum_of(tid, false), first_before, R = 0.0;  // the first kThreads chunks
-  const auto total_of = [&]() {
-    first_before = block_prefix(first_sum, sm, tid, R);
-    if (a.chunks > kThreads) {
-      double t = 0.0, more;
-      for (int c = tid + kThreads; c < a.chunks; c += kThreads) t += sum_of(c, plain);
-      block_prefix(t, sm, tid, more);
-      R += more;
+  // The sums of r over this thread's chunks; plain: of p itself, where p - q, or p without
+  // the draft, leaves nothing.
+  const auto sum_of = [&](bool plain) {
+    double t = 0.0;
+    for (int c = c0; c < c1; ++c) {
+      if (a.k == 0) t += chunk_sum(sums[c], maxes[c], mp, rate);
+      else if (plain) t += rest[c].e;
+      else if (!both) t += rest[c].over;
+      else if (rest[c].gp >= 0.0) t += fmax(rest[c].over - (lam - p.lam) * rest[c].gp, 0.0);
     }
+    return t;
   };
-  total_of();
-  if (R == 0.0 && (both || skips)) {
-    plain = true;
-    first_sum = sum_of(tid, true);
-    total_of();
+  double mine = sum_of(false);
+  if (both && sound) {
+    // marked chunks, in any order: each is one thread's to add
+    for (int g = 0; g < per; ++g) {
+      const uint64_t m = __ballot(c0 + g < c1 && !(rest[c0 + g].gp >= 0.0));
+      if ((tid & 63) == 0) sm_marked[w] = m;
+      __syncthreads();
+      for (int q = 0; q < kWaves; ++q) {
+        for (uint64_t left = sm_marked[q]; left; left &= left - 1) {
+          const int owner = q * 64 + __builtin_ctzll(left);
+          double r[NV][N];
+          const double s = block_sum(weights_of(owner * per + g, r), sm, tid);
+          if (tid == owner) mine += s;
+        }
+      }
+      __syncthreads();
+    }
+  }
+  double R, before = block_prefix(mine, sm, tid, R);
+  if (R == 0.0 && (both || p.skip >= 0)) {
+    both = false;
+    p.skip = -1;
+    mine = sum_of(true);
+    before = block_prefix(mine, sm, tid, R);
   }
   int32_t token = -1;
-  if (rate > 0.0 && R > 0.0) {
+  if (rate > 0.0 && sound && R > 0.0) {
     const double place = u * R;
-    // the first chunk whose running sum passes the place, and the sum ahead of it; the
-    // last chunk of any mass where rounding lets none pass
+    // the first thread whose running sum passes the place; the last one of any mass
+    // where rounding lets none pass
     if (tid == 0) {
-      sm_at = a.chunks;
+      sm_at = kThreads;
       sm_last = -1;
     }
     __syncthreads();
-    double carry = 0.0;
-    int c = -1;
-    for (int c0 = 0; c0 < a.chunks; c0 += kThreads) {
-      double v = first_sum, before = first_before, all = 0.0;
-      if (a.chunks > kThreads) {
-        v = sum_of(c0 + tid, plain);
-        before = carry + block_prefix(v, sm, tid, all);
-      }
-      const uint64_t some = __ballot(v > 0.0), past = __ballot(v > 0.0 && before + v > place);
+    {
+      const uint64_t some = __ballot(mine > 0.0), past = __ballot(mine > 0.0 && before + mine > place);
       if ((tid & 63) == 0) {
-        const int w0 = c0 + tid;
-        if (some) atomicMax(&sm_last, w0 + 63 - __builtin_clzll(some));
-        if (past) atomicMin(&sm_at, w0 + __builtin_ctzll(past));
+        if (some) atomicMax(&sm_last, tid + 63 - __builtin_clzll(some));
+        if (past) atomicMin(&sm_at, tid + __builtin_ctzll(past));
       }
-      __syncthreads();
-      c = sm_at < a.chunks ? sm_at : sm_last;
-      if (c == c0 + tid) sm_ahead = before;
-      carry += all;
-      if (sm_at < a.chunks) break;
     }
+    __syncthreads();
+    const int owner = sm_at < kThreads ? sm_at : sm_last;
+    if (tid == owner) sm_ahead = before;
     __syncthreads();
     if (tid == 0) {
       sm_at = a.V;
       sm_last = -1;
     }
-    if (plain) {
-      both = false;
-      p.skip = -1;
-    }
-    double r[NV][N], all;
-    double at = block_prefix(weights_of(c, r), sm, tid, all) + sm_ahead;
-    int first = a.V, last = -1;
+    double ahead = sm_ahead;
+    for (int c = owner * per; c < min((owner + 1) * per, a.chunks); ++c) {
+      double r[NV][N], all;
+      double at = ahead + block_prefix(weights_of(c, r), sm, tid, all);
+      ahead += all;
+      int first = a.V, last = -1;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
+      for (int v = 0; v < NV; ++v) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        at += r[v][e];
-        if (r[v][e] > 0.0) {
-          last = ids_of(c, v) + e;
-          if (at > place && first == a.V) first = last;
+        for (int e = 0; e < N; ++e) {
+          at += r[v][e];
+          if (r[v][e] > 0.0) {
+            last = ids_of(c, v) + e;
+            if (at > place && first == a.V) first = last;
+          }
         }
       }
+      // (ids grow with the lane)
+      const uint64_t some = __ballot(last >= 0), past = __ballot(first < a.V);
+      if (some && (tid & 63) == 63 - __builtin_clzll(some)) atomicMax(&sm_last, last);
+      if (past && (tid & 63) == __builtin_ctzll(past)) atomicMin(&sm_at, first);
+      __syncthreads();
+      if (sm_at < a.V) break;
     }
-    // (ids grow with the lane)
-    const uint64_t some = __ballot(last >= 0), past = __ballot(first < a.V);
-    if (some && (tid & 63) == 63 - __builtin_clzll(some)) atomicMax(&sm_last, last);
-    if (past && (tid & 63) == __builtin_ctzll(past)) atomicMin(&sm_at, first);
-    __syncthreads();
     token = sm_at < a.V ? sm_at : sm_last;
   }
   for (int j = tid; j <= a.k; j += kThreads) {
@@ -594,7 +727,7 @@ static SampleCfg sample_cfg(int B, int k, int V, bool draft) {
   };
   c.sums = take(parts * sizeof(double));
   c.maxes = take(parts * sizeof(float));
-  c.rest = take(static_cast<size_t>(B) * c.chunks * sizeof(double));
+  c.rest = take(k ? static_cast<size_t>(B) * c.chunks * sizeof(RestSums) : 0);
   c.picks = take(static_cast<size_t>(B) * sizeof(SamplePick));
   c.bytes = at;
   return c;
@@ -602,21 +735,23 @@ static SampleCfg sample_cfg(int B, int k, int V, bool draft) {
 
 template <typename E>
 static void launch_sample(const SampleArgs& a, hipStream_t st) {
-  const int stats = std::min(kStatGrid, cdiv(a.B * a.rows * a.chunks, kWaves));
-  hipLaunchKernelGGL(sample_stats_kernel<E>, dim3(stats), dim3(kThreads), 0, st, a);
-  const size_t lds = static_cast<size_t>(a.rows) * (sizeof(double) + sizeof(float));
-  if (a.draft)
-    hipLaunchKernelGGL(sample_rest_kernel<E>, dim3(a.B * cdiv(a.chunks, kWaves)), dim3(kThreads), lds,
-                       st, a);
-  hipLaunchKernelGGL(sample_pick_kernel<E>, dim3(a.B), dim3(kThreads), lds, st, a);
+  const dim3 stats(std::min(kStatGrid, cdiv(a.B * a.rows * a.chunks, kWaves))), wg(kThreads);
+  if (a.k > 0) {
+    hipLaunchKernelGGL((sample_stats_kernel<E, false>), stats, wg, 0, st, a);
+    hipLaunchKernelGGL(sample_rest_kernel<E>, dim3(a.B * cdiv(a.chunks, kWaves)), wg,
+                       static_cast<size_t>(a.rows) * (sizeof(double) + sizeof(float)), st, a);
+  } else {
+    hipLaunchKernelGGL((sample_stats_kernel<E, true>), stats, wg, 0, st, a);
+  }
+  hipLaunchKernelGGL(sample_pick_kernel<E>, dim3(a.B), wg, 0, st, a);
 }
 
 }  // namespace kve
 
 using namespace kve;
 
-// Drafts a sequence may have (their rows' statistics share a workgroup's LDS).
-constexpr int kSampleMaxDrafts = 1024;
+// Drafts a sequence may have: a thread each in decide().
+constexpr int kSampleMaxDrafts = kThreads;
 
 extern "C" size_t kve_sample_workspace_bytes(int num_seqs, int k, int vocab, int dtype) {
   if (num_seqs <= 0 || k < 0 || k > kSampleMaxDrafts || vocab <= 0 ||
@@ -687,7 +822,7 @@ extern "C" int kve_sample_verify(const void* target, int64_t target_seq_stride,
   a.keep = keep_lens;
   a.sums = reinterpret_cast<double*>(ws + c.sums);
   a.maxes = reinterpret_cast<float*>(ws + c.maxes);
-  a.rest = reinterpret_cast<double*>(ws + c.rest);
+  a.rest = reinterpret_cast<RestSums*>(ws + c.rest);
   a.picks = reinterpret_cast<SamplePick*>(ws + c.picks);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == KVE_DTYPE_BF16) launch_sample<uint16_t>(a, st);

@@ -885,17 +885,29 @@ TREE_MAX_NODES = 64
 
 
 def _check_on(t: torch.Tensor | None, name: str, dtype, shape: tuple, dev) -> None:
-    if t is None:
-        return
-    _need(t.dtype is dtype and tuple(t.shape) == shape and t.device == dev and t.is_contiguous(),
-          f"{name} must be contiguous {dtype} {list(shape)} on {dev}, "
-          f"got {t.dtype} {list(t.shape)} on {t.device}")
+    # (the message is only built for an error: a decode step pays for every check)
+    if t is not None and not (t.dtype is dtype and t.shape == shape and t.device == dev
+                              and t.is_contiguous()):
+        raise ValueError(f"{name} must be contiguous {dtype} {list(shape)} on {dev}, "
+                         f"got {t.dtype} {list(t.shape)} on {t.device}")
+
+
+def _call(fn, what: str, dev: torch.device, *args) -> None:
+    """fn(*args, stream) with `dev` as the current device, on its current stream."""
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream(dev))
+    if rc:
+        _lib.check(rc, what)
 
 
 def _check_tree(parents: torch.Tensor, q_lens: torch.Tensor | None) -> tuple[int, int]:
     _need(parents.dim() == 2 and parents.is_cuda, "parents must be [B, nodes] on the GPU")
     B, n = parents.shape
-    _need(1 <= n <= TREE_MAX_NODES, f"{n} nodes per tree, 1 to {TREE_MAX_NODES}")
+    if not 1 <= n <= TREE_MAX_NODES:
+        raise ValueError(f"{n} nodes per tree, 1 to {TREE_MAX_NODES}")
     _check_on(parents, "parents", torch.int32, (B, n), parents.device)
     _check_on(q_lens, "q_lens", torch.int32, (B,), parents.device)
     return B, n
@@ -910,12 +922,10 @@ def tree_masks(parents: torch.Tensor, q_lens: torch.Tensor | None = None):
     counts as none."""
     B, n = _check_tree(parents, q_lens)
     dev = parents.device
-    masks = torch.empty(B, n, dtype=torch.int64, device=dev)
-    depths = torch.empty(B, n, dtype=torch.int32, device=dev)
-    with torch.cuda.device(dev):
-        rc = _lib.lib().kve_tree_masks(parents.data_ptr(), _ptr(q_lens), B, n, masks.data_ptr(),
-                                       depths.data_ptr(), _stream(dev))
-    _lib.check(rc, "kve_tree_masks")
+    masks = torch.empty((B, n), dtype=torch.int64, device=dev)
+    depths = torch.empty((B, n), dtype=torch.int32, device=dev)
+    _call(_lib.lib().kve_tree_masks, "kve_tree_masks", dev, parents.data_ptr(), _ptr(q_lens), B, n,
+          masks.data_ptr(), depths.data_ptr())
     return masks, depths
 
 
@@ -934,52 +944,57 @@ def paged_tree_attn(q: torch.Tensor, k_layer: torch.Tensor, v_layer: torch.Tenso
     The workspace is this call's own (ws: a buffer of attn_workspace_bytes instead),
     so captured graphs share none."""
     _need(q.dim() == 4 and q.is_contiguous() and q.is_cuda, "q must be contiguous [B, T, Hq, D]")
-    dev = q.device
+    dev, dtype = q.device, q.dtype
     B, T, Hq, D = q.shape
-    _need(T <= TREE_MAX_NODES, f"{T} nodes per tree, at most {TREE_MAX_NODES}")
+    if T > TREE_MAX_NODES:
+        raise ValueError(f"{T} nodes per tree, at most {TREE_MAX_NODES}")
     _check_on(masks, "masks", torch.int64, (B, T), dev)
-    _need(k_layer.dim() == 4 and v_layer.dim() == 4, "k/v layer must be 4-d")
-    NB, Hkv, bs, Dk = k_layer.shape
-    _need(Dk == D and tuple(v_layer.shape) == (NB, Hkv, D, bs),
-          f"pool shapes k{tuple(k_layer.shape)} v{tuple(v_layer.shape)} do not match q D={D}")
-    _need(k_layer.is_contiguous() and v_layer.is_contiguous() and k_layer.device == dev
-          and v_layer.device == dev, f"k/v layer must be contiguous on {dev}")
-    _need(k_layer.dtype == q.dtype == v_layer.dtype, "q/k/v dtype mismatch")
-    _need(Hkv > 0 and Hq % Hkv == 0, f"{Hq} q heads not a multiple of {Hkv} kv heads")
-    max_blocks, num_rows = _attn_checks(block_tables, start_pos, seq_rows, q_lens, B, bs, max_ctx,
-                                        dev)
-    if plan is not None:
-        _need(plan.key == _attn_key(B, T, Hq, Hkv, D, bs, max_ctx, unit_blocks, key_waves, q.dtype)
-              and plan.buf.device == dev,
-              "attention plan was built for another shape, configuration or device")
+    _need(k_layer.dim() == 4 and block_tables.dim() == 2 and start_pos.dim() == 1,
+          "k/v layer [NB, Hkv, bs, D], block_tables [rows, max_blocks], start_pos [rows]")
+    NB, Hkv, bs, _ = k_layer.shape
+    num_rows, max_blocks = block_tables.shape
+    _check_on(k_layer, "k_layer", dtype, (NB, Hkv, bs, D), dev)
+    _check_on(v_layer, "v_layer", dtype, (NB, Hkv, D, bs), dev)
+    if Hkv < 1 or Hq % Hkv:
+        raise ValueError(f"{Hq} q heads not a multiple of {Hkv} kv heads")
+    _check_on(block_tables, "block_tables", torch.int32, (num_rows, max_blocks), dev)
+    _check_on(start_pos, "start_pos", torch.int32, start_pos.shape, dev)
+    _check_on(seq_rows, "seq_rows", torch.int32, (B,), dev)
+    _check_on(q_lens, "q_lens", torch.int32, (B,), dev)
+    if max_ctx < 1 or max_blocks * bs < max_ctx:
+        raise ValueError(f"max_ctx {max_ctx} exceeds table capacity {max_blocks * bs}")
+    _need(start_pos.numel() >= num_rows, "start_pos needs one entry per table row")
+    _need(seq_rows is not None or num_rows >= B, "too few table rows")
+    _need(plan is None or plan.key == _attn_key(B, T, Hq, Hkv, D, bs, max_ctx, unit_blocks,
+                                                key_waves, dtype) and plan.buf.device == dev,
+          "attention plan was built for another shape, configuration or device")
     if blocked:
-        _need(q.dtype == torch.bfloat16 and (Hq * D) % 32 == 0, "blocked out is bf16, Hq*D % 32")
+        _need(dtype == torch.bfloat16 and (Hq * D) % 32 == 0, "blocked out is bf16, Hq*D % 32")
         if out is None:
             out = blocked_matrix(B * T, Hq * D, dev)
-        _need(out.dtype == q.dtype and out.device == dev and out.is_contiguous()
+        _need(out.dtype == dtype and out.device == dev and out.is_contiguous()
               and out.numel() >= blocked_rows(B * T) * Hq * D, "bad blocked out")
     elif out is None:
         out = torch.empty_like(q)
     else:
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == dev
-              and out.is_contiguous(), "bad out")
+        _check_on(out, "out", dtype, (B, T, Hq, D), dev)
     scale = D ** -0.5 if scale is None else float(scale)
-    _need(scale > 0.0, f"scale {scale} must be positive")
+    if not scale > 0.0:
+        raise ValueError(f"scale {scale} must be positive")
+    code = _dtype_code(q)
     if B == 0 or T == 0:
         return out
-    nbytes = attn_workspace_bytes(B, T, Hq, Hkv, D, bs, max_ctx, unit_blocks, key_waves, q.dtype)
+    lib = _lib.lib()
+    nbytes = lib.kve_attn_workspace_bytes(B, T, Hq, Hkv, D, bs, max_ctx, unit_blocks, key_waves, code)
     if ws is None:
-        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
-    _need(ws.numel() * ws.element_size() >= nbytes and ws.device == dev,
-          "attention workspace too small")
-    with torch.cuda.device(dev):
-        rc = _lib.lib().kve_paged_tree_attn(
-            q.data_ptr(), k_layer.data_ptr(), v_layer.data_ptr(), masks.data_ptr(),
-            block_tables.data_ptr(), _ptr(seq_rows), start_pos.data_ptr(), _ptr(q_lens), B, T, Hq,
-            Hkv, D, bs, max_blocks, num_rows, NB, int(max_ctx), int(unit_blocks), int(key_waves),
-            scale, _dtype_code(q), None if plan is None else plan.buf.data_ptr(), out.data_ptr(),
-            ws.data_ptr(), ws.numel() * ws.element_size(), _layout(blocked), _stream(dev))
-    _lib.check(rc, "kve_paged_tree_attn")
+        ws = torch.empty(nbytes or 1, dtype=torch.uint8, device=dev)
+    have = ws.numel() * ws.element_size()
+    _need(have >= nbytes and ws.device == dev and ws.is_contiguous(), "attention workspace too small")
+    _call(lib.kve_paged_tree_attn, "kve_paged_tree_attn", dev, q.data_ptr(), k_layer.data_ptr(),
+          v_layer.data_ptr(), masks.data_ptr(), block_tables.data_ptr(), _ptr(seq_rows),
+          start_pos.data_ptr(), _ptr(q_lens), B, T, Hq, Hkv, D, bs, max_blocks, num_rows, NB, max_ctx,
+          unit_blocks, key_waves, scale, code, None if plan is None else plan.buf.data_ptr(),
+          out.data_ptr(), ws.data_ptr(), have, _layout(blocked))
     return out
 
 
@@ -996,33 +1011,32 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, preds: torch.Tensor
     the length to roll back to (rollback). seq_rows: table rows (default 0 .. B-1); of
     two entries with one row the first moves it."""
     B, n = _check_tree(parents, q_lens)
-    dev = parents.device
-    _check_on(tokens, "tokens", torch.int32, (B, n), dev)
-    _check_on(preds, "preds", torch.int32, (B, n), dev)
-    _check_on(seq_rows, "seq_rows", torch.int32, (B,), dev)
-    out = torch.empty(2, B, n, dtype=torch.int32, device=dev)
-    ints = torch.empty(2, B, dtype=torch.int32, device=dev)
-    emitted, path, n_acc, keep = out[0], out[1], ints[0], None
-    pools, sizes, lens, rows = (None, None, None), (0, 0, 0, 0, 0, 0, 0), None, 0
-    if kv is not None:
-        keep = ints[1]
-        L, NB, Hkv, bs, D = kv.k.shape
-        _need(tuple(kv.v.shape) == (L, NB, Hkv, D, bs) and kv.k.dtype == kv.v.dtype
-              and kv.k.is_contiguous() and kv.v.is_contiguous() and kv.k.device == dev
-              and kv.v.device == dev, "pools must be contiguous [L, NB, Hkv, bs, D] / [.., D, bs]")
-        lens, rows = kv.lens, kv.lens.numel()
-        _check_i32(lens, "lens", dev)
-        _check_i32(kv.tables, "tables", dev)
-        _need(kv.tables.dim() == 2 and kv.tables.shape[0] == rows, "one length per table row")
+    dev, i32 = parents.device, torch.int32
+    _check_on(tokens, "tokens", i32, (B, n), dev)
+    _check_on(preds, "preds", i32, (B, n), dev)
+    _check_on(seq_rows, "seq_rows", i32, (B,), dev)
+    n_acc = torch.empty(B, dtype=i32, device=dev)
+    emitted = torch.empty((B, n), dtype=i32, device=dev)
+    path = torch.empty((B, n), dtype=i32, device=dev)
+    if kv is None:
+        keep = lens = None
+        rows, pools = 0, (None, None, None, 0, 0, 0, 0, 0, 0, 0)
+    else:
+        k, v, tables, lens = kv.k, kv.v, kv.tables, kv.lens
+        _need(k.dim() == 5 and tables.dim() == 2, "pools [L, NB, Hkv, bs, D], tables [rows, blocks]")
+        L, NB, Hkv, bs, D = k.shape
+        rows, max_blocks = tables.shape
+        _check_on(k, "k pool", k.dtype, (L, NB, Hkv, bs, D), dev)
+        _check_on(v, "v pool", k.dtype, (L, NB, Hkv, D, bs), dev)
+        _check_on(tables, "tables", i32, (rows, max_blocks), dev)
+        _check_on(lens, "lens", i32, (rows,), dev)
         _need(seq_rows is not None or rows >= B, "too few table rows")
-        pools = (kv.k.data_ptr(), kv.v.data_ptr(), kv.tables.data_ptr())
-        sizes = (L, Hkv, D, bs, kv.tables.shape[1], NB, _dtype_code(kv.k))
-    with torch.cuda.device(dev):
-        rc = _lib.lib().kve_tree_accept(
-            tokens.data_ptr(), parents.data_ptr(), preds.data_ptr(), _ptr(q_lens), _ptr(lens),
-            rows, _ptr(seq_rows), B, n, n_acc.data_ptr(), emitted.data_ptr(), path.data_ptr(),
-            _ptr(keep), *pools, *sizes, _stream(dev))
-    _lib.check(rc, "kve_tree_accept")
+        keep = torch.empty(B, dtype=i32, device=dev)
+        pools = (k.data_ptr(), v.data_ptr(), tables.data_ptr(), L, Hkv, D, bs, max_blocks, NB,
+                 _dtype_code(k))
+    _call(_lib.lib().kve_tree_accept, "kve_tree_accept", dev, tokens.data_ptr(), parents.data_ptr(),
+          preds.data_ptr(), _ptr(q_lens), _ptr(lens), rows, _ptr(seq_rows), B, n, n_acc.data_ptr(),
+          emitted.data_ptr(), path.data_ptr(), _ptr(keep), *pools)
     return n_acc, emitted, path, keep
 
 
@@ -1039,47 +1053,48 @@ def sample_verify(target_logits: torch.Tensor, drafts: torch.Tensor, u_accept: t
     sequence. -> (n_acc [B], emitted [B, k+1]: accepted drafts, the sampled token, then -1,
     keep [B] = lens - k + n_acc, or None without lens). Draws are exact: 64-bit sums."""
     _need(target_logits.dim() == 3 and target_logits.is_cuda, "target_logits must be [B, k+1, V]")
-    dev = target_logits.device
+    dev, dtype, i32 = target_logits.device, target_logits.dtype, torch.int32
     B, k1, V = target_logits.shape
     k = k1 - 1
-    _need(k >= 0 and V >= 1, f"target_logits {list(target_logits.shape)}")
-    _need(target_logits.stride(2) == 1 or V == 1, "logits need a contiguous vocabulary")
-    _check_on(drafts, "drafts", torch.int32, (B, k), dev)
+    if k < 0 or V < 1:
+        raise ValueError(f"target_logits {list(target_logits.shape)}")
+    ts, tp, one = target_logits.stride()
+    _need(one == 1 or V == 1, "logits need a contiguous vocabulary")
+    _check_on(drafts, "drafts", i32, (B, k), dev)
     _check_on(u_accept, "u_accept", torch.float32, (B, k), dev)
     _check_on(u_sample, "u_sample", torch.float32, (B,), dev)
-    ds = (0, 0)
+    ds = dp = 0
     if draft_logits is not None:
-        _need(tuple(draft_logits.shape) == (B, k, V) and draft_logits.dtype == target_logits.dtype
-              and draft_logits.device == dev and (draft_logits.stride(2) == 1 or V == 1),
-              f"draft_logits must be {target_logits.dtype} {[B, k, V]} on {dev} with a contiguous "
-              f"vocabulary")
-        ds = draft_logits.stride()[:2]
+        if draft_logits.shape != (B, k, V) or draft_logits.dtype != dtype \
+                or draft_logits.device != dev or not (draft_logits.stride(2) == 1 or V == 1):
+            raise ValueError(f"draft_logits must be {dtype} {[B, k, V]} on {dev} with a contiguous "
+                             f"vocabulary, got {draft_logits.dtype} {list(draft_logits.shape)}")
+        ds, dp, _ = draft_logits.stride()
     temps = None
     if isinstance(temperature, torch.Tensor):
         temps, temperature = temperature, 1.0
         _check_on(temps, "temperature", torch.float32, (B,), dev)
-    else:
-        temperature = float(temperature)
-        _need(0.0 < temperature < float("inf"), f"temperature {temperature} must be positive")
-    _check_i32(lens, "lens", dev)
-    _check_on(seq_rows, "seq_rows", torch.int32, (B,), dev)
-    num_rows = 0 if lens is None else lens.numel()
-    _need(lens is None or seq_rows is not None or num_rows >= B, "too few length rows")
+    elif not 0.0 < temperature < float("inf"):
+        raise ValueError(f"temperature {temperature} must be positive")
+    _check_on(seq_rows, "seq_rows", i32, (B,), dev)
+    num_rows, keep = 0, None
+    if lens is not None:
+        num_rows = lens.numel()
+        _check_on(lens, "lens", i32, (num_rows,), dev)
+        _need(seq_rows is not None or num_rows >= B, "too few length rows")
+        keep = torch.empty(B, dtype=i32, device=dev)
     code = _dtype_code(target_logits)
-    n_acc = torch.empty(B, dtype=torch.int32, device=dev)
-    emitted = torch.empty(B, k1, dtype=torch.int32, device=dev)
-    keep = None if lens is None else torch.empty(B, dtype=torch.int32, device=dev)
+    n_acc = torch.empty(B, dtype=i32, device=dev)
+    emitted = torch.empty((B, k1), dtype=i32, device=dev)
     if B == 0:
         return n_acc, emitted, keep
     lib = _lib.lib()
     nbytes = lib.kve_sample_workspace_bytes(B, k, V, code)
-    _need(nbytes > 0, f"{k} drafts per sequence are too many")
+    if not nbytes:
+        raise ValueError(f"{k} drafts per sequence are too many")
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        rc = lib.kve_sample_verify(
-            target_logits.data_ptr(), *target_logits.stride()[:2], _ptr(draft_logits), *ds,
-            drafts.data_ptr(), u_accept.data_ptr(), u_sample.data_ptr(), _ptr(temps), temperature,
-            _ptr(lens), num_rows, _ptr(seq_rows), B, k, V, code, n_acc.data_ptr(),
-            emitted.data_ptr(), _ptr(keep), ws.data_ptr(), nbytes, _stream(dev))
-    _lib.check(rc, "kve_sample_verify")
+    _call(lib.kve_sample_verify, "kve_sample_verify", dev, target_logits.data_ptr(), ts, tp,
+          _ptr(draft_logits), ds, dp, drafts.data_ptr(), u_accept.data_ptr(), u_sample.data_ptr(),
+          _ptr(temps), temperature, _ptr(lens), num_rows, _ptr(seq_rows), B, k, V, code,
+          n_acc.data_ptr(), emitted.data_ptr(), _ptr(keep), ws.data_ptr(), nbytes)
     return n_acc, emitted, keep

@@ -75,7 +75,7 @@ def call_sample(**kw):
 @pytest.mark.parametrize("change,rc,text", [
     (dict(target=None), -1, "null pointer"), (dict(drafts=None), -1, "null pointer"),
     (dict(ua=None), -1, "null pointer"), (dict(us=None), -1, "null pointer"),
-    (dict(k=-1), -1, "k = -1"), (dict(k=1025), -1, "k = 1025"), (dict(V=0), -1, "vocabulary 0"),
+    (dict(k=-1), -1, "k = -1"), (dict(k=257), -1, "k = 257"), (dict(V=0), -1, "vocabulary 0"),
     (dict(dtype=7), -1, "dtype"), (dict(temp=0.0), -1, "temperature"),
     (dict(temp=float("inf")), -1, "temperature"), (dict(temp=float("nan")), -1, "temperature"),
     (dict(temp=-1.0), -1, "temperature"), (dict(keep=16), -1, "needs lens"),
