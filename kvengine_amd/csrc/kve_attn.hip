@@ -560,16 +560,16 @@ __device__ __forceinline__ uint32_t tree_bits(uint64_t vis, int k0, int start) {
 
 // Trees: a row must not take up an infinity or NaN in the V of a node that it
 // does not see, and the matrix product would make 0 * inf = NaN of it. V is
-// therefore taken without its non-finite values from the pair (32 keys) that
-// holds `start` on, and where a wave dropped any, the rows that see such a key get
-// it added here: p * inf and p * NaN of a p > 0 are the value itself. Never entered
-// while the cache is finite.
-template <int D, bool BF16>
-__device__ __forceinline__ void add_nonfinite(const AttnArgs& a, const UnitInfo& x, int lg,
+// therefore taken without the non-finite values of the tree's nodes, and where a wave
+// dropped any, the rows that see such a key of its own (key wave kw of KW, bursts of
+// NPRE tiles) get it added here: p * inf and p * NaN of a p > 0 are the value itself.
+// Never entered while the cache is finite.
+template <int D, bool BF16, int NPRE, int KW>
+__device__ __forceinline__ void add_nonfinite(const AttnArgs& a, const UnitInfo& x, int kw, int lg,
                                               f32x4 (&acc)[D / 16]) {
   using elem_t = std::conditional_t<BF16, uint16_t, float>;
   const int32_t* table = a.tables + static_cast<size_t>(x.srow) * a.max_blocks;
-  const int first = max(x.kt0 * 16, x.start - 31), end = min(x.Lk, x.kt1 * 16);
+  const int first = max(x.kt0 * 16, x.start), end = min(x.Lk, x.kt1 * 16);
 #pragma unroll
   for (int dt = 0; dt < D / 16; ++dt) {
     // (one channel group's keys at a time, so that this path takes none of the
@@ -577,7 +577,7 @@ __device__ __forceinline__ void add_nonfinite(const AttnArgs& a, const UnitInfo&
     f32x4 add = {0, 0, 0, 0};
 #pragma unroll 1
     for (int key = first; key < end; ++key) {
-      const bool sees = key < x.start || (x.vis >> (key - x.start) & 1);
+      const bool sees = x.vis >> (key - x.start) & 1 && ((key >> 4) - x.kt0) / NPRE % KW == kw;
       const int blk = safe_block(table[key / a.bs], a.num_blocks);
       const elem_t* vp = static_cast<const elem_t*>(a.v) + key % a.bs +
                          ((static_cast<size_t>(blk) * a.Hkv + x.kvh) * D + dt * 16 + 4 * lg) * a.bs;
@@ -759,7 +759,8 @@ __global__ __launch_bounds__(64 * NT * KW) void verify_attn_f32_kernel(AttnArgs 
           for (int dt = 0; dt < DT; ++dt) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const bool inf = (__float_as_uint(fr[j].v[dt][i]) & 0x7f800000u) == 0x7f800000u;
+              const bool inf = (r0 + j) * 16 + 4 * lg + i >= start &&
+                               (__float_as_uint(fr[j].v[dt][i]) & 0x7f800000u) == 0x7f800000u;
               dropped |= inf;
               fr[j].v[dt][i] = inf ? 0.0f : fr[j].v[dt][i];
             }
@@ -827,7 +828,7 @@ __global__ __launch_bounds__(64 * NT * KW) void verify_attn_f32_kernel(AttnArgs 
       }
     }
     if constexpr (TREE) {
-      if (__any(dropped)) add_nonfinite<D, false>(a, x, lg, acc);
+      if (__any(dropped)) add_nonfinite<D, false, NPRE, KW>(a, x, kw, lg, acc);
     }
     finish_unit<D, false, NT, KW, TREE>(a, x, sm_dyn, nt, kw, l, m_run, sum_across_groups(l_run), acc);
   }
@@ -1009,7 +1010,8 @@ __attribute__((amdgpu_waves_per_eu(NT >= 2 && NT * KW <= 6 ? 4 : 1))) void verif
             if ((r0 + 2 * p) * 16 + 31 >= x.start) {
 #pragma unroll
               for (int w = 0; w < 4; ++w) {
-                const bool lo = (v[w] & 0x7f80u) == 0x7f80u, hi = (v[w] & 0x7f800000u) == 0x7f800000u;
+                const bool lo = (v[w] & 0x7f80u) == 0x7f80u && k0 + 2 * w >= x.start;
+                const bool hi = (v[w] & 0x7f800000u) == 0x7f800000u && k0 + 2 * w + 1 >= x.start;
                 dropped |= lo || hi;
                 v[w] &= (lo ? 0xffff0000u : ~0u) & (hi ? 0x0000ffffu : ~0u);
               }
@@ -1235,7 +1237,7 @@ __attribute__((amdgpu_waves_per_eu(NT >= 2 && NT * KW <= 6 ? 4 : 1))) void verif
       barrier_after_vm<0>();  // the buffers are rewritten by the fold or the next unit
     }
     if constexpr (TREE) {
-      if (__any(dropped)) add_nonfinite<D, true>(a, x, lg, acc);
+      if (__any(dropped)) add_nonfinite<D, true, NPRE, KW>(a, x, kw, lg, acc);
     }
     finish_unit<D, true, NT, KW, TREE>(a, x, sm_dyn, nt, kw, l, m_run, lsum[0], acc);
   }

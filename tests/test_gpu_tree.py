@@ -263,6 +263,28 @@ def test_what_a_row_does_not_see_never_reaches_it(gpu_lib, dtype, D, order, bs):
     assert torch.equal(got[1], clean[1])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kw", [1, 2, 4])
+def test_a_seen_infinity_beside_unseen_ones_of_other_key_waves(gpu_lib, dtype, D, kw):
+    """A row that sees one infinite node takes it whole, whatever the key waves hold in
+    which the row sees no key, or only finite ones, and others are infinite."""
+    T, far = 64, (20, 28, 36, 44, 52, 60)
+    case = Case(D + kw, [96], T, 4, 2, D, dtype=dtype)
+    case.masks[0] = [1 << 3 if t >= 3 else 0 for t in range(T)]
+    for t in range(32, T, 2):
+        case.masks[0][t] |= sum(1 << n for n in far if n < t)
+    clean = case.run((10, kw))
+    for node in (3,) + far:
+        blk, off = case.slot(0, 96 + node)
+        case.pool[1, blk, off, 1, 5] = float("inf")
+    got = case.run((10, kw))
+    for t in range(3, T):
+        assert torch.equal(got[0, t, 2:, 5], torch.full((2,), float("inf"), dtype=dtype)), t
+        got[0, t, 2:, 5] = clean[0, t, 2:, 5]
+    assert torch.equal(got, clean)
+
+
 def test_rows_of_a_table_and_a_skipped_sequence(gpu_lib):
     """seq_rows in any order, one row twice, one outside the table (left as it was)."""
     case = Case(4, [20, 90, 300], 6, 4, 2, 64)
