@@ -49,23 +49,92 @@ __global__ __launch_bounds__(64) void tree_masks_kernel(const int32_t* parents,
   if (depths) depths[at] = live ? __popc(lo) + __popc(hi) - 1 : 0;
 }
 
+// n / d for 0 <= n < 2^30 without the divide's thirty instructions: with 2^(s-1) < d <=
+// 2^s, mul = ceil(2^(30+s) / d) is too large by less than one, so that n mul / 2^(30+s)
+// passes n / d by less than 2^30 / 2^(30+s) <= 1 / d, too little to reach the next whole.
+struct Divisor {
+  uint32_t mul, shift;
+  explicit Divisor(int d) {
+    uint32_t s = 0;
+    while ((1ll << s) < d) ++s;
+    shift = 30 + s;
+    mul = static_cast<uint32_t>(((1ull << shift) + d - 1) / d);
+  }
+  __device__ int operator()(int n) const {
+    return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(n)) * mul >> shift);
+  }
+};
+
 struct TreeAcceptArgs {
   const int32_t *tokens, *parents, *preds, *node_counts, *lens, *seq_rows, *tables;
   int32_t *n_acc, *emitted, *path, *keep;
   void *k, *v;
   int num_rows, nodes, L, Hkv, D, bs, max_blocks, num_blocks;
+  Divisor by_kwidth, by_dim, by_kv;  // K's pieces a row, head_dim, the kv heads
 };
 
 // Grid (sequences, parts): every wave walks the sequence's tree (a few shuffles and
 // ballots on values that one load each brought in), the first workgroup of a
-// sequence writes the results, and all of them share the moves, a thread owning one
-// 16-byte piece of a K row or one channel of V in one (layer, kv head) and taking
-// the path's nodes in order. A node moves to a slot at or below its own and every
-// later node lies above that slot, so a thread that reads kMoves nodes and then
-// writes them never overwrites a node still to be read. K rows are contiguous; V is
-// channel-major, so a moved token is one element of a 32-byte run per channel.
+// sequence writes the results, and all of them share the moves. What bounds it is the
+// way to the data: the launch and the tree's loads 4 us, then K/V that nothing has
+// touched since the forward, pages apart from layer to layer: 32 trees of 16 nodes in 36
+// layers of 2 heads of 128 move 3.1 MB in 14.6 us (21.0 with a lane taking all of its
+// column's moves, whose loads under branches waited for each other).
 constexpr int kAcceptThreads = 256;
-constexpr int kMoves = 8;
+constexpr int kMoves = 8;  // loads in flight of a lane
+
+// Where a lane's move takes from and puts to: element offsets in a layer's first head.
+struct Move {
+  size_t from, to;
+  bool live;
+};
+
+// The moves of 64 columns of one pool, `columns` in all and `width` a kv head: K's
+// pieces of 16 bytes or V's channels, T one of either, column c of a slot at c * cstep.
+// 2^lg lanes share a column, a move each, so that all of a column's loads are one
+// instruction and come before its stores, whichever slots they overlap; the 2^lg turns
+// that the wave takes for its 64 columns are loaded Q at a time. Every lane loads (one
+// with nothing to move loads its column's slot 0 of block 0): a load under a branch is
+// waited for before the next.
+template <int Q, typename T>
+__device__ __forceinline__ void move_columns(T* pool, size_t layer_stride, size_t head_stride,
+                                             int first, int columns, int width, Divisor by_width,
+                                             int Hkv, Divisor by_kv, int cstep, Move mv, int lg) {
+  const int l = threadIdx.x & 63;
+  for (int turn = 0; turn < 1 << lg; turn += Q) {
+    T *dst[Q], x[Q];
+    bool ok[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int column = first + (turn + q) * (64 >> lg) + (l >> lg);
+      ok[q] = mv.live && column < columns;
+      const int at = min(column, columns - 1), lh = by_width(at), layer = by_kv(lh);
+      T* base = pool + layer * layer_stride + (lh - layer * Hkv) * head_stride +
+                (at - lh * width) * cstep;
+      x[q] = base[mv.from];
+      dst[q] = base + mv.to;
+    }
+#pragma unroll
+    for (int q = 0; q < Q; ++q) asm volatile("" ::"v"(x[q]));  // (or it loads under `ok`)
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+      if (ok[q]) *dst[q] = x[q];
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void move_columns(T* pool, size_t layer_stride, size_t head_stride,
+                                             int first, int columns, int width, Divisor by_width,
+                                             int Hkv, Divisor by_kv, int cstep, Move mv, int lg) {
+  const auto go = [&](auto q) {
+    move_columns<decltype(q)::value>(pool, layer_stride, head_stride, first, columns, width,
+                                     by_width, Hkv, by_kv, cstep, mv, lg);
+  };
+  if (lg >= 3) go(std::integral_constant<int, kMoves>{});
+  else if (lg == 2) go(std::integral_constant<int, 4>{});
+  else if (lg == 1) go(std::integral_constant<int, 2>{});
+  else go(std::integral_constant<int, 1>{});
+}
 
 template <typename E>
 __global__ __launch_bounds__(kAcceptThreads) void tree_accept_kernel(TreeAcceptArgs a) {
@@ -74,10 +143,26 @@ __global__ __launch_bounds__(kAcceptThreads) void tree_accept_kernel(TreeAcceptA
   const int row = a.seq_rows ? a.seq_rows[i] : i;
   const bool has_row = a.lens && row >= 0 && row < a.num_rows;
   const int start = has_row ? a.lens[row] - max(n, 0) : 0;
+  // all loads before the walk: one wait instead of one after the other
   const size_t at = static_cast<size_t>(i) * a.nodes + l;
+  int parent = -1, token = 0, pred = 0;
+  if (l < a.nodes) {
+    parent = a.parents[at];
+    token = a.tokens[at];
+    pred = a.preds[at];
+  }
+  // lane t: slot start + t, as its block (-1: none) and its offset in it
+  const bool moving = a.k && has_row && start >= 0;
+  int blk = -1, off = 0;
+  if (moving) {
+    const uint32_t slot = static_cast<uint32_t>(start) + l, entry = slot / a.bs;
+    off = slot - entry * a.bs;
+    if (entry < static_cast<uint32_t>(a.max_blocks))
+      blk = a.tables[static_cast<size_t>(row) * a.max_blocks + entry];
+    if (blk >= a.num_blocks) blk = -1;
+  }
   const bool in = l < n;
-  const int parent = tree_parent(a.parents + static_cast<size_t>(i) * a.nodes, l, n);
-  const int token = in ? a.tokens[at] : 0, pred = in ? a.preds[at] : 0;
+  if (!in || parent >= l) parent = -1;
 
   uint64_t taken = n > 0 ? 1 : 0;
   int cur = 0;
@@ -112,7 +197,7 @@ __global__ __launch_bounds__(kAcceptThreads) void tree_accept_kernel(TreeAcceptA
     }
   }
 
-  if (!a.k || !has_row || start < 0) return;
+  if (!moving) return;
   // nodes below the first gap in the path are where they belong
   if ((taken & (taken + 1)) == 0) return;
   const int j0 = __builtin_ctzll(~taken);
@@ -122,53 +207,34 @@ __global__ __launch_bounds__(kAcceptThreads) void tree_accept_kernel(TreeAcceptA
     for (int e = l; e < i; e += 64) again |= a.seq_rows[e] == row;
     if (__any(again)) return;
   }
-  constexpr int VEC = 16 / sizeof(E);
-  const int kpieces = a.D / VEC, per_head = kpieces + a.D;
-  const int items = a.L * a.Hkv * per_head;
-  const int32_t* table = a.tables + static_cast<size_t>(row) * a.max_blocks;
-  const int cap = a.max_blocks * a.bs;
-  for (int it = blockIdx.y * kAcceptThreads + threadIdx.x; it < items;
-       it += gridDim.y * kAcceptThreads) {
-    const int lh = it / per_head, c = it - lh * per_head;
-    const int layer = lh / a.Hkv, h = lh - layer * a.Hkv;
-    // element of (block, offset): a K piece c < kpieces, or V channel c - kpieces
-    const size_t head0 = (static_cast<size_t>(layer) * a.num_blocks * a.Hkv + h) * a.bs * a.D;
-    const size_t blk_step = static_cast<size_t>(a.Hkv) * a.bs * a.D;
-    const bool is_k = c < kpieces;
-    const int off_step = is_k ? a.D : 1;
-    const size_t first = head0 + (is_k ? c * VEC : static_cast<size_t>(c - kpieces) * a.bs);
-    uint64_t left = taken >> j0 << j0;
-    int j = j0;
-    while (left) {
-      E* dst[kMoves];
-      u32x4 kx[kMoves];
-      E vx[kMoves];
-      int m = 0;
-#pragma unroll
-      for (int q = 0; q < kMoves; ++q) {
-        dst[q] = nullptr;
-        if (!left) continue;
-        const int node = __builtin_ctzll(left);
-        left &= left - 1;
-        const int sp = start + node, dp = start + j + m;
-        ++m;
-        if (sp >= cap) continue;
-        const int sb = table[sp / a.bs], db = table[dp / a.bs];
-        if (sb < 0 || sb >= a.num_blocks || db < 0 || db >= a.num_blocks) continue;
-        const size_t so = first + sb * blk_step + static_cast<size_t>(sp % a.bs) * off_step;
-        const size_t dof = first + db * blk_step + static_cast<size_t>(dp % a.bs) * off_step;
-        dst[q] = static_cast<E*>(is_k ? a.k : a.v) + dof;
-        if (is_k) kx[q] = *reinterpret_cast<const u32x4*>(static_cast<const E*>(a.k) + so);
-        else vx[q] = static_cast<const E*>(a.v)[so];
-      }
-      j += m;
-#pragma unroll
-      for (int q = 0; q < kMoves; ++q) {
-        if (!dst[q]) continue;
-        if (is_k) *reinterpret_cast<u32x4*>(dst[q]) = kx[q];
-        else *dst[q] = vx[q];
-      }
-    }
+  // P lanes to a column, P the power of two that holds the moves; lane l takes move
+  // l mod P: the node that becomes the path's entry j0 + l mod P
+  const int moves = steps - j0, lg = moves > 1 ? 32 - __builtin_clz(moves - 1) : 0;
+  const int move = l & ((1 << lg) - 1), to = min(j0 + move, 63);
+  // (lanes off the path write to the last entry, which then is not the path's)
+  const int entry_of = taken >> l & 1 ? __popcll(taken & ((1ull << l) - 1)) : 63;
+  const int from = __shfl(__builtin_amdgcn_ds_permute(4 * entry_of, l), to) & 63;
+  const int sb = __shfl(blk, from), so = __shfl(off, from);
+  const int db = __shfl(blk, to), dof = __shfl(off, to);
+  const bool live = move < moves && sb >= 0 && db >= 0;
+  const auto mv = [&](size_t head, int step) {
+    return live ? Move{sb * (a.Hkv * head) + so * step, db * (a.Hkv * head) + dof * step, true}
+                : Move{0, 0, false};
+  };
+
+  const int kw = a.D / static_cast<int>(16 / sizeof(E)), heads = a.L * a.Hkv;
+  const int kchunks = cdiv(heads * kw, 64), chunks = kchunks + cdiv(heads * a.D, 64);
+  const size_t khead = static_cast<size_t>(a.bs) * kw, vhead = static_cast<size_t>(a.bs) * a.D;
+  const Move mk = mv(khead, kw), mvv = mv(vhead, 1);
+  // a wave's 64 columns lie together: it meets one head's pages or two's
+  for (int c = blockIdx.y * (kAcceptThreads / 64) + (threadIdx.x >> 6); c < chunks;
+       c += gridDim.y * (kAcceptThreads / 64)) {
+    if (c < kchunks)
+      move_columns(static_cast<u32x4*>(a.k), a.num_blocks * (a.Hkv * khead), khead, c * 64,
+                   heads * kw, kw, a.by_kwidth, a.Hkv, a.by_kv, 1, mk, lg);
+    else
+      move_columns(static_cast<E*>(a.v), a.num_blocks * (a.Hkv * vhead), vhead,
+                   (c - kchunks) * 64, heads * a.D, a.D, a.by_dim, a.Hkv, a.by_kv, a.bs, mvv, lg);
   }
 }
 
@@ -206,7 +272,7 @@ extern "C" int kve_tree_accept(const int32_t* tokens, const int32_t* parents, co
   KVE_REQUIRE(!(k_pool || keep_lens) || (lens && num_rows > 0),
               "kve_tree_accept: the pools and keep_lens need lens");
   KVE_REQUIRE(!k_pool == !v_pool, "kve_tree_accept: k_pool and v_pool go together");
-  int parts = 1;
+  int parts = 1, kwidth = 1;
   if (k_pool) {
     KVE_REQUIRE(block_tables && num_layers > 0 && num_kv_heads > 0 && block_size > 0 &&
                     max_blocks > 0 && num_blocks > 0,
@@ -217,17 +283,20 @@ extern "C" int kve_tree_accept(const int32_t* tokens, const int32_t* parents, co
     KVE_REQUIRE(head_dim > 0 && head_dim % vec == 0, "kve_tree_accept: head_dim %d", head_dim);
     KVE_REQUIRE(((reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) & 15) == 0,
                 "kve_tree_accept: k_pool and v_pool must be 16-byte aligned");
+    kwidth = head_dim / vec;
     const long long items =
-        static_cast<long long>(num_layers) * num_kv_heads * (head_dim / vec + head_dim);
+        static_cast<long long>(num_layers) * num_kv_heads * (kwidth + head_dim);
     KVE_REQUIRE(items < (1ll << 30) && static_cast<long long>(max_blocks) * block_size < (1ll << 30),
                 "kve_tree_accept: %d layers x %d heads, %d blocks a row: too large", num_layers,
                 num_kv_heads, max_blocks);
-    parts = static_cast<int>((items + kAcceptThreads - 1) / kAcceptThreads);
+    parts = static_cast<int>(items / kAcceptThreads + 1);
     if (parts > 1024) parts = 1024;
   }
   const TreeAcceptArgs a{tokens, parents, preds, node_counts, lens, seq_rows, block_tables,
                          n_acc, emitted, path, keep_lens, k_pool, v_pool, num_rows, nodes,
-                         num_layers, num_kv_heads, head_dim, block_size, max_blocks, num_blocks};
+                         num_layers, num_kv_heads, head_dim, block_size, max_blocks, num_blocks,
+                         Divisor(kwidth), Divisor(k_pool ? head_dim : 1),
+                         Divisor(k_pool ? num_kv_heads : 1)};
   const dim3 grid(num_seqs, parts);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (k_pool && dtype == KVE_DTYPE_F32)

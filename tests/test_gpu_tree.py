@@ -462,6 +462,57 @@ def test_accept_moves_the_path(gpu_lib, dtype, bs, D, n):
         assert keep[b] == (lens[row] - counts[b] + 1 + int(n_acc[b]) if row < 5 else 0)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bs", [16, 5])
+def test_accept_moves_any_number_of_nodes(gpu_lib, dtype, bs):
+    """1 to 62 moves: node 1 hangs off the path 0, 2, 3, .., so that all behind it move by
+    one slot, into slots that other moves read."""
+    n, counts = 64, list(range(1, 63))
+    B, D, g = len(counts), 72, torch.Generator().manual_seed(bs)
+    trees = [[-1, 0, 0] + list(range(2, n - 1))] * B
+    tokens = [[0, 1] + [5] * (n - 2)] * B
+    preds = [[5 if t < m + 1 else 7 for t in range(n)] for m in counts]
+    starts = [3 + 2 * b for b in range(B)]
+    width = -(-(starts[-1] + n) // bs)
+    ids = torch.randperm(B * width, generator=g).view(B, width)
+    k = torch.randn(2, B * width, 3, bs, D, generator=g).to(dtype)
+    v = torch.randn(2, B * width, 3, D, bs, generator=g).to(dtype)
+    want_k, want_v = k.clone(), v.clone()
+    for b, m in enumerate(counts):
+        for j in range(1, m + 1):
+            (sb, so), (db, do) = ((int(ids[b, x // bs]), x % bs)
+                                  for x in (starts[b] + j + 1, starts[b] + j))
+            want_k[:, db, :, do] = k[:, sb, :, so]
+            want_v[:, db, :, :, do] = v[:, sb, :, :, so]
+    kv = DeviceKV(k.to(DEV), v.to(DEV), ids.to(torch.int32).to(DEV), i32([s + n for s in starts]), bs)
+    n_acc, _, _, keep = kernels.tree_accept(i32(tokens), i32(trees), i32(preds), kv=kv)
+    assert n_acc.tolist() == counts
+    assert keep.tolist() == [s + 1 + m for s, m in zip(starts, counts)]
+    assert torch.equal(kv.k.cpu(), want_k) and torch.equal(kv.v.cpu(), want_v)
+
+
+def test_accept_over_many_heads(gpu_lib):
+    """More columns than one turn of the launch's workgroups takes: 2048 heads."""
+    L, Hkv, D, bs, n, start = 64, 32, 128, 16, 12, 13
+    g = torch.Generator(device=DEV).manual_seed(1)
+    k = torch.randn(L, 3, Hkv, bs, D, generator=g, device=DEV, dtype=torch.bfloat16)
+    v = torch.randn(L, 3, Hkv, D, bs, generator=g, device=DEV, dtype=torch.bfloat16)
+    want_k, want_v = k.clone(), v.clone()
+    path, table = [0, 3, 4, 8, 11], [2, 0]
+    parents = [-1, 0, 0, 0, 3, 0, 1, 2, 4, 7, 9, 8]
+    for j, c in enumerate(path):
+        (sb, so), (db, do) = ((table[x // bs], x % bs) for x in (start + c, start + j))
+        want_k[:, db, :, do] = k[:, sb, :, so]
+        want_v[:, db, :, :, do] = v[:, sb, :, :, so]
+    kv = DeviceKV(k, v, i32([table]), i32([start + n]), bs)
+    tokens = i32([list(range(n))])
+    preds = i32([[3, 0, 0, 4, 8, 0, 0, 0, 11, 0, 0, 2]])
+    n_acc, emitted, got, _ = kernels.tree_accept(tokens, i32([parents]), preds, kv=kv)
+    assert n_acc.tolist() == [4] and got[0, :5].tolist() == path
+    assert emitted[0, :5].tolist() == [3, 4, 8, 11, 2]
+    assert torch.equal(k, want_k) and torch.equal(v, want_v)
+
+
 def test_accept_with_bad_blocks_and_lengths_moves_nothing_outside(gpu_lib):
     """Unallocated or out-of-range table entries and lengths are never followed."""
     n = 16
