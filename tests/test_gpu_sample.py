@@ -342,3 +342,68 @@ def test_emitted_tokens_follow_the_target(gpu_lib):
                                     draft_logits=None if d is None else d.to(DEV).expand(N, 1, V))
         f = torch.bincount(got[1][:, 0].cpu().long(), minlength=V).double() / N
         assert ((f - p).abs() <= 5 * (p * (1 - p) / N).sqrt()).all(), (f, p)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("with_draft", [True, False])
+def test_uniform_numbers_beside_a_test_s_edge(gpu_lib, dtype, with_draft):
+    """u the fp32 numbers around p(x) / q(x): 32-bit sums do not decide these tests, and
+    several of a sequence follow each other. An fp32 number lies some 1e-8 from the edge."""
+    B, k, V = 24, 5, 4099
+    target, drafts, ua, us, draft = draw_inputs(77, B, k, V, dtype, near=0.5)
+    p = torch.softmax(target[:, :k].double(), -1).gather(2, drafts.long()[..., None])[..., 0]
+    q = torch.softmax(draft.double(), -1).gather(2, drafts.long()[..., None])[..., 0]
+    edge = (p / q if with_draft else p).float()
+    for b in range(B):
+        for j in range(k):
+            if edge[b, j] >= 1 or (b + j) % 5 == 4:
+                continue
+            u = edge[b, j]
+            for _ in range((b + 3 * j) % 4):
+                u = torch.nextafter(u, torch.tensor(0.0 if (b + j) % 2 else 2.0))
+            ua[b, j] = u
+    n_acc, _ = check((target, drafts, ua, us, draft if with_draft else None))
+    assert len(set(n_acc.tolist())) > 2
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_probabilities_that_differ_by_less_than_the_sums(gpu_lib, dtype):
+    """Every id's p - q is a few millionths of p, all of one sign but the draft's."""
+    B, V = 6, 30011
+    g = torch.Generator().manual_seed(5)
+    target = (0.25 * torch.randn(B, 2, V, generator=g)).to(dtype)
+    draft = target[:, :1].clone()
+    x = torch.randint(0, V, (B,), generator=g, dtype=torch.int32)
+    for b in range(B):
+        draft[b, 0, x[b]] += 0.125
+    us = torch.rand(B, generator=g)
+    n_acc, emitted = check((target, x[:, None], torch.full((B, 1), 1 - 2.0 ** -24), us, draft))
+    assert n_acc.tolist() == [0] * B
+    n_acc, emitted = check((target, x[:, None], torch.full((B, 1), 0.5), us, draft))
+    assert n_acc.tolist() == [1] * B
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_more_chunks_than_threads(gpu_lib, dtype):
+    args = draw_inputs(6, 3, 1, 700001, dtype)
+    check(args)
+    target, drafts, _, us, draft = args
+    draft = target[:, :1].clone()
+    drafts = torch.tensor([[3], [400000], [700000]], dtype=torch.int32)
+    for b in range(3):
+        draft[b, 0, drafts[b, 0]] += 4.0
+    check((target, drafts, torch.full((3, 1), 0.99), us, draft))
+    check((target[:, :1], torch.zeros(3, 0, dtype=torch.int32), torch.zeros(3, 0), us))
+
+
+@pytest.mark.parametrize("with_draft", [True, False])
+def test_as_many_drafts_as_a_call_takes(gpu_lib, with_draft):
+    """256 drafts of a sequence, the sequences differing in the one that falls."""
+    B, k, V = 5, 256, 61
+    target, drafts, ua, us, draft = draw_inputs(8, B, k, V, torch.float32, near=0.05)
+    ua = ua * 1e-6
+    for b, j in enumerate((0, 1, 63, 255)):
+        ua[b, j], target[b, j, drafts[b, j]] = 0.9, -30.0
+    n_acc, _ = check((target, drafts, ua, us, draft if with_draft else None))
+    if with_draft:  # (without one a draft of p(x) < u <= 1e-6 falls too)
+        assert n_acc.tolist() == [0, 1, 63, 255, 256]
