@@ -1243,6 +1243,272 @@ __attribute__((amdgpu_waves_per_eu(NT >= 2 && NT * KW <= 6 ? 4 : 1))) void verif
   }
 }
 
+// Trees with several row tiles (bf16, 16-token blocks): verify_attn_bf16_kernel's rows,
+// units, bursts, key waves and order of every sum, and so its bits, as a kernel of its own.
+// A chunk wholly in the history, nearly all of them, runs through straight code; the masks
+// and what the tree's V needs are in a loop of their own, where V is mended in LDS before
+// any wave reads it. What bounds it is LDS: a wave reads 16 KB of fragments for 26 MFMAs of
+// 16 cycles, and LDS gives a CU 64 bytes a cycle, 2048 cycles of reads for the 832 of
+// MFMAs and some 600 of exponentials of 8 waves (two a SIMD). So workgroups of 8 waves
+// hold 128 registers and 64 KB, and two of them share a CU: the reads of one run beside
+// the products of the other. One layer, 16 sequences x 64 nodes, 8000 tokens (3B, units
+// of 512 keys, merge included): 238 us with the masks in one loop and one workgroup a CU,
+// 184 with two, 160 so. Two row tiles per wave, half the reads and half the waves: 154
+// there, but 314 for 283 with units of 256 keys in two key waves, and 33.3 for 32.0 at 32
+// sequences x 16 nodes.
+template <int D, int NT, int KW>
+struct TreeTiles {
+  static constexpr int NW = NT * KW;                // waves
+  static constexpr int CT = KW * burst_tiles<D, true>();  // tiles per chunk
+  static constexpr int kChunk = CT * kDmaTileBytes<D>();
+  // Two workgroups share a CU at 128 registers and 64 KB each, where the key waves' fold
+  // and masks leave a wave with that: 32 sequences x 8 nodes (3B, four row tiles in two key
+  // waves) 19.9 us with one and no spills, 23.3 with two.
+  static constexpr bool kPair = NW <= 8 && (KW == 1 || NW <= 6);
+  static constexpr int kEu = kPair ? 4 : NW <= 8 ? 2 : 3;
+  static constexpr int fit = (kPair ? 64 : 128) * 1024 / kChunk;
+  static constexpr int NBUF = fit < 2 ? 2 : fit > 8 ? 8 : fit;
+  // LDS: the chunk buffers, or the key waves' states (finish_unit), then a flag. (In a
+  // variable of its own it would move the buffers off their alignment: 505 us for 160.)
+  static constexpr int kFold = NT * (KW - 1) * (32 * 4 + (D / 16) * 1024);
+  static constexpr int kFlag = NBUF * kChunk > kFold ? NBUF * kChunk : kFold;
+  static constexpr int kLds = kFlag + 16;
+};
+
+template <int D, int NT, int KW>
+__global__ __launch_bounds__(64 * NT * KW)
+__attribute__((amdgpu_waves_per_eu((TreeTiles<D, NT, KW>::kEu)))) void tree_attn_bf16_kernel(AttnArgs a) {
+  using C = TreeTiles<D, NT, KW>;
+  constexpr int NPRE = burst_tiles<D, true>(), NP = NPRE / 2, DT = D / 16, DQ = D / 4, KS = D / 32;
+  constexpr int KI = D / 32, TI = 2 * KI, TB = kDmaTileBytes<D>();
+  constexpr int NW = C::NW, CT = C::CT, NBUF = C::NBUF;
+  constexpr int CPIECES = CT * TI, LPW = (CPIECES + NW - 1) / NW;
+  static_assert((NBUF - 2) * LPW <= 63, "vmcnt range");
+  extern __shared__ int sm_dyn[];
+
+  const int tid = threadIdx.x;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int nt = wid / KW, kw = wid - nt * KW;
+  const int32_t* recs = a.plan + kPlanHead;
+  const uint16_t* qb = static_cast<const uint16_t*>(a.q);
+  const char* kg = static_cast<const char*>(a.k);
+  const char* vg = static_cast<const char*>(a.v);
+  const float c = a.scale_log2;
+  const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // bf16 1.0 x 8
+  char* kvl = reinterpret_cast<char*>(sm_dyn);
+  int& sm_found = sm_dyn[C::kFlag / 4];  // a chunk's V held a non-finite value of the tree's
+
+  int nunits = a.plan[0];
+  int rec = recs[static_cast<size_t>(blockIdx.x / a.Hkv) * kRecInts + (tid & 63)];
+  nunits = __builtin_amdgcn_readfirstlane(min(nunits, a.max_units)) * a.Hkv;
+  for (int u = blockIdx.x; u < nunits; u += gridDim.x) {
+    // (hidden, or what follows from the lane stays in registers from unit to unit)
+    int l = tid & 63;
+    asm volatile("" : "+v"(l));
+    const int lr = l & 15, lg = l >> 4;
+    const int tv = rec;  // block ids: lane kRecHead + j holds tile kt0 + j
+    const UnitInfo x = unit_info<NT, true>(a, tv, u, nt, lr);
+    const int next = min(u + static_cast<int>(gridDim.x), nunits - 1);
+    rec = recs[static_cast<size_t>(next / a.Hkv) * kRecInts + l];
+    const int kt0 = x.kt0, kt1 = x.kt1, start = x.start;
+    const int vlim = min(x.Lk, kt1 * 16);
+    const int nch = cdiv(kt1 - kt0, CT);
+    // chunks wholly in the history: no mask, V as it is
+    const int nfull = max(0, min(start, vlim) / 16 - kt0) / CT;
+    const auto buffer = [&](int ch) { return kvl + (ch % NBUF) * C::kChunk; };
+    const auto issue_chunk = [&](int ch) {
+      char* buf = buffer(ch);
+#pragma unroll
+      for (int i = 0; i < LPW; ++i) {
+        const int g = min(wid + i * NW, CPIECES - 1);
+        const int t = g / TI, part = g - t * TI;
+        const int lane = min(kRecHead + ch * CT + t, 63);
+        const int blk = safe_block(__builtin_amdgcn_readlane(tv, lane), a.num_blocks);
+        const size_t tb = (static_cast<size_t>(blk) * a.Hkv + x.kvh) * 16 * D;
+        const char* src;
+        if (part < KI) {
+          const int j = part * 64 + l, row = j / (D / 8), pc = j - row * (D / 8);
+          src = kg + (tb + static_cast<size_t>(row) * D) * 2 + ((pc ^ ksw<D>(row, t)) << 4);
+        } else {
+          const int j = (part - KI) * 64 + l, chn = j >> 1;
+          src = vg + (tb + static_cast<size_t>(chn) * 16) * 2 + (((j & 1) ^ vsw(chn)) << 4);
+        }
+        __builtin_amdgcn_global_load_lds(
+            (__attribute__((address_space(1))) void*)(src),
+            (__attribute__((address_space(3))) void*)(buf + t * TB + part * 1024), 16, 0, 0);
+      }
+    };
+    if (tid == 0) sm_found = 0;  // (the last unit's waves have met since they read it)
+#pragma unroll
+    for (int ch = 0; ch < NBUF - 1; ++ch)
+      if (ch < nch) issue_chunk(ch);
+
+    u32x4 qf[KS];
+    {
+      const bool ok = x.r < x.R;
+      const int t = ok ? div_g(x.r, a) : 0;
+      const int h = x.kvh * a.G + (ok ? x.r - t * a.G : 0);
+      const uint16_t* qp = qb + ((static_cast<size_t>(x.b) * a.Tq + t) * a.Hq + h) * D + lg * DQ;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        qf[ks] = reinterpret_cast<const u32x4*>(qp)[ks];
+        if (!ok) qf[ks] = u32x4{0, 0, 0, 0};
+        // q's wait here, once: at its first use in the loops it would be every chunk's
+        // wait for all loads under way
+        asm volatile("" : "+v"(qf[ks]));
+      }
+    }
+    float m_run = kNegBig;
+    f32x4 acc[DT], lsum = {0, 0, 0, 0};
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0, 0, 0, 0};
+
+    // This wave's burst of chunk ch: scores, the online-softmax step and P V, each as in
+    // verify_attn_bf16_kernel. Fragments are read together and ahead of their products.
+    const auto burst = [&](int ch, int lane, auto masked) {
+      const int r = lane & 15, g = lane >> 4;
+      const char* tb0 = buffer(ch) + kw * NPRE * TB;
+      u32x4 k[NP][2][KS], v[NP][DT];
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const char* tk = tb0 + (2 * p + (r >> 3)) * TB;  // the tile of this lane's K row
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = pair_key_of_row(r, h) & 15;
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            const int cch = g * (DQ / 8) + ks;
+            k[p][h][ks] = *reinterpret_cast<const u32x4*>(
+                tk + row * 2 * D + ((cch ^ ksw<D>(row, r >> 3)) << 4));
+          }
+        }
+      }
+      f32x4 sc[NP][2];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            sc[p][h] = mfma16x16x32_bf16(k[p][h][ks], qf[ks], ks ? sc[p][h] : f32x4{0, 0, 0, 0});
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const char* tvv = tb0 + (2 * p + (g >> 1)) * TB + 32 * D;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const int chn = dt * 16 + r;
+          v[p][dt] = *reinterpret_cast<const u32x4*>(tvv + chn * 32 + (((g & 1) ^ vsw(chn)) << 4));
+        }
+      }
+      if constexpr (decltype(masked)::value) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          const int k0 = (kt0 + ch * CT + kw * NPRE + 2 * p) * 16 + 8 * g;
+          const uint32_t bits = k0 < kt1 * 16 ? tree_bits(x.vis, k0, start) : 0u;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (!(bits >> (4 * h + i) & 1)) sc[p][h][i] = -INFINITY;
+          }
+        }
+      }
+      float smax = -INFINITY;
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          smax = fmaxf(fmaxf(smax, sc[p][h][0]), sc[p][h][1]);
+          smax = fmaxf(fmaxf(smax, sc[p][h][2]), sc[p][h][3]);
+        }
+      }
+      const float m_new = fmaxf(m_run, max_across_groups(smax) * c);
+      const bool grow = m_new > m_run + 8.0f;  // (the first burst's from kNegBig: 0 scaled by 0)
+      if (__any(grow)) {
+        const float m_use = grow ? m_new : m_run;
+        const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+        m_run = m_use;
+        lsum *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
+      }
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        f32x4 e[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) e[h][i] = __builtin_amdgcn_exp2f(fmaf(sc[p][h][i], c, -m_run));
+        }
+        u32x4 ph, pl;  // P = hi + lo
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float pa = e[q >> 1][2 * (q & 1)], pb = e[q >> 1][2 * (q & 1) + 1];
+          const uint32_t ua = __float_as_uint(pa), ub = __float_as_uint(pb);
+          ph[q] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+          pl[q] = pack_bf16x2(pa - __uint_as_float(ua & 0xffff0000u),
+                              pb - __uint_as_float(ub & 0xffff0000u));
+        }
+        // (hi of every accumulator, then lo: each one's own order, no product waiting for
+        // the one before)
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+            acc[dt] = mfma16x16x32_bf16(v[p][dt], part ? pl : ph, acc[dt]);
+          lsum = mfma16x16x32_bf16(ones, part ? pl : ph, lsum);
+        }
+      }
+    };
+    // Chunk ch has landed, and every wave is done with chunk ch - 1, whose buffer takes
+    // the next one.
+    const auto advance = [&](int ch) {
+      barrier_after_chunks<LPW, NBUF - 2>(min(NBUF - 2, nch - 1 - ch));
+      if (ch + NBUF - 1 < nch) issue_chunk(ch + NBUF - 1);
+    };
+    for (int ch = 0; ch < nfull; ++ch) {
+      advance(ch);
+      if (x.active) burst(ch, l, std::false_type{});
+    }
+    bool dropped = false;
+    for (int ch = nfull; ch < nch; ++ch) {
+      advance(ch);
+      const int ck0 = (kt0 + ch * CT) * 16;
+      // V of a chunk that reaches the tree or the unit's end: keys from vlim on (stale
+      // slots, tiles past the unit) become zero, and so do non-finite values of the
+      // tree's nodes (add_nonfinite).
+      for (int i = tid; i < CT * 2 * D; i += 64 * NW) {
+        const int t = i / (2 * D), piece = i - t * (2 * D), chn = piece >> 1;
+        const int k0 = ck0 + t * 16 + (((piece & 1) ^ vsw(chn)) << 3);
+        if (k0 + 7 < min(start, vlim)) continue;
+        u32x4* at = reinterpret_cast<u32x4*>(buffer(ch) + t * TB + 32 * D + piece * 16);
+        u32x4 v = *at;
+        bool found = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t m = e & 1 ? 0xffff0000u : 0x0000ffffu, inf = 0x7f807f80u & m;
+          const bool drop = k0 + e >= start && (v[e >> 1] & inf) == inf && k0 + e < vlim;
+          found |= drop;
+          if (drop || k0 + e >= vlim) v[e >> 1] &= ~m;
+        }
+        *at = v;
+        if (found) sm_found = 1;
+      }
+      barrier_after_vm<63>();  // (no wait for the loads under way)
+      dropped |= sm_found != 0;
+      if (!x.active || kt0 + ch * CT + kw * NPRE >= kt1) continue;
+      int lane = l;
+      asm volatile("" : "+v"(lane));  // (its addresses are not worth the other loop's registers)
+      burst(ch, lane, std::true_type{});
+    }
+    barrier_after_vm<0>();  // the buffers are rewritten by the fold or the next unit
+    if (dropped) add_nonfinite<D, true, NPRE, KW>(a, x, kw, lg, acc);
+    finish_unit<D, true, NT, KW, true>(a, x, sm_dyn, nt, kw, l, m_run, lsum[0], acc);
+  }
+}
+
 // Merge the units of one split item (and kv head): the units' states folded
 // in unit order with fold_state -- as the waves of a unit are -- then
 // normalised. Grid (split-item bound, Hkv * D/16 parts); thread (row, 4 channels).
@@ -1508,22 +1774,26 @@ static int merge_batch(long long workgroups, int max_item_units) {
 
 template <int D, bool BF16, int NT, int KW, bool TREE>
 static int launch_attn_t(const AttnArgs& a, const AttnCfg& p, hipStream_t st, bool bs16) {
-  auto go = [&](auto kernel) {
-    const int rc = grant_lds(kernel, p.lds, "kve_paged_verify_attn");
+  auto go = [&](auto kernel, int threads, size_t lds) {
+    const int rc = grant_lds(kernel, lds, "kve_paged_verify_attn");
     if (rc) return rc;
-    const int nwg = resident_workgroups(kernel, 64 * NT * KW, p.lds);
+    const int nwg = resident_workgroups(kernel, threads, lds);
     const long long max_units = static_cast<long long>(p.max_units) * a.Hkv;
     const int grid = static_cast<int>(std::max(1LL, std::min<long long>(nwg, max_units)));
-    hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * NT * KW), p.lds, st, a);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), lds, st, a);
     return KVE_OK;
   };
   int rc;
-  if constexpr (BF16)
-    rc = bs16 ? go(verify_attn_bf16_kernel<D, NT, true, KW, TREE>)
-              : go(verify_attn_bf16_kernel<D, NT, false, KW, TREE>);
+  constexpr int threads = 64 * NT * KW;
+  if constexpr (BF16 && TREE && NT >= 2) {
+    rc = bs16 ? go(tree_attn_bf16_kernel<D, NT, KW>, threads, TreeTiles<D, NT, KW>::kLds)
+              : go(verify_attn_bf16_kernel<D, NT, false, KW, TREE>, threads, p.lds);
+  } else if constexpr (BF16)
+    rc = bs16 ? go(verify_attn_bf16_kernel<D, NT, true, KW, TREE>, threads, p.lds)
+              : go(verify_attn_bf16_kernel<D, NT, false, KW, TREE>, threads, p.lds);
   else
-    rc = bs16 ? go(verify_attn_f32_kernel<D, NT, true, KW, TREE>)
-              : go(verify_attn_f32_kernel<D, NT, false, KW, TREE>);
+    rc = bs16 ? go(verify_attn_f32_kernel<D, NT, true, KW, TREE>, threads, p.lds)
+              : go(verify_attn_f32_kernel<D, NT, false, KW, TREE>, threads, p.lds);
   if (rc) return rc;
   // histories longer than one unit: merge their units' states (only launched
   // when max_ctx allows more than one unit per history)
