@@ -1353,10 +1353,11 @@ __attribute__((amdgpu_waves_per_eu((TreeTiles<D, NT, KW>::kEu)))) void tree_attn
       for (int ks = 0; ks < KS; ++ks) {
         qf[ks] = reinterpret_cast<const u32x4*>(qp)[ks];
         if (!ok) qf[ks] = u32x4{0, 0, 0, 0};
-        // q's wait here, once: at its first use in the loops it would be every chunk's
-        // wait for all loads under way
-        asm volatile("" : "+v"(qf[ks]));
       }
+      // q's wait here, once: at its first use in the loops it would be every chunk's wait
+      // for all loads under way
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
     }
     float m_run = kNegBig;
     f32x4 acc[DT], lsum = {0, 0, 0, 0};
