@@ -787,7 +787,7 @@ extern "C" int kve_sample_verify(const void* target, int64_t target_seq_stride,
                (esz - 1)) == 0,
               "kve_sample_verify: logits are not aligned to their type");
   const SampleCfg c = sample_cfg(num_seqs, k, vocab, draft != nullptr && k > 0);
-  KVE_REQUIRE(static_cast<long long>(num_seqs) * c.rows * c.chunks < (1ll << 31),
+  KVE_REQUIRE(static_cast<long long>(num_seqs) * c.rows * c.chunks < (1ll << 30),
               "kve_sample_verify: %d x %d rows of %d too large for one launch", num_seqs, c.rows,
               vocab);
   KVE_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,

@@ -82,6 +82,7 @@ def call_sample(**kw):
     (dict(target=17), -1, "aligned"), (dict(draft=18, dtype=0), -1, "aligned"),
     (dict(ws=None), -1, "workspace"), (dict(ws=8), -1, "16-byte"), (dict(wsb=8), -2, "workspace"),
     (dict(B=1 << 24, k=128, V=1 << 20), -1, "too large"),
+    (dict(B=1 << 20, k=0, V=2048 * 1024), -1, "too large"),
 ])
 def test_sample_verify_refuses(change, rc, text):
     got, msg = call_sample(**change)
