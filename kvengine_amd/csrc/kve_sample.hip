@@ -32,8 +32,12 @@
 // draft's and L = sum(e) / sum(g), r is max(e - L g, 0) / sum(e). L is only known after
 // a pass, but to 2^-16 from the 32-bit sums (L'). So the pass sums e - L' g over the ids
 // where it is positive, and g over the same ids: the rest is the first minus (L - L')
-// times the second. An id where |e - L' g| <= 2^-16 L' g may be on either side; its chunk
-// is marked and summed again by `pick` (an id or two of 150 000, or all where p = q).
+// times the second. An id where |e - L' g| <= 2^-16 L' g may be on either side. Those are
+// summed apart, with the least and the largest e / g among them: L above all of them
+// leaves them out, below all of them takes them in, and only a chunk with L between them
+// is summed again by `pick`. In bf16 logits t - d takes few values, so that where L is
+// near one's e / g nearly every chunk has ids there, all of one e / g: re-summing those 75
+// chunks took one call in three of 32 sequences 145 us for 44.
 
 #include "kve_common.h"
 
@@ -52,9 +56,16 @@ struct SamplePick {
 // What `rest` leaves of a chunk at the deciding position.
 struct RestSums {
   double e, g;      // sums over the chunk
-  double over, gp;  // sum of e - L' g over the ids where it is positive, and of their g
-                    // (gp < 0: some id is undecided, the chunk is to be summed again);
+  double over, gp;  // sum of e - L' g over the ids where it is positive, and of their g;
                     // without a draft's distribution: sum of e without `skip`, 0
+  double eu, gu;    // sums of e and g over the undecided ids
+  double lo, hi;    // the least and the largest e / g of those (none: inf, -inf; nothing
+                    // known: -inf, inf)
+  // for L the undecided ids are all out, all in, or the chunk is to be summed again
+  // (also where L is as near to them as 64-bit weights are apart)
+  __device__ __forceinline__ bool out(double lam) const { return lam >= hi; }
+  __device__ __forceinline__ bool in(double lam) const { return lam < lo * (1.0 - 0x1p-40); }
+  __device__ __forceinline__ bool marked(double lam) const { return !out(lam) && !in(lam); }
 };
 
 struct SampleArgs {
@@ -454,7 +465,7 @@ __global__ __launch_bounds__(kThreads) void sample_rest_kernel(SampleArgs a) {
       lo_q = min_nan(lo_q, logit<E>(y.x[v], e));
     }
   }
-  double se = 0.0, sg = 0.0, over = 0.0, gp = 0.0;
+  RestSums r{0.0, 0.0, 0.0, 0.0, 0.0, 0.0, INFINITY, -INFINITY};
   bool undecided = false;
   const double edge = kMargin * p.lam;
   const auto sum_both = [&](auto&& w) {
@@ -466,12 +477,45 @@ __global__ __launch_bounds__(kThreads) void sample_rest_kernel(SampleArgs a) {
       for (int e = 0; e < N; ++e) {
         const double we = w(logit<E>(x.x[v], e), mp), wg = w(logit<E>(y.x[v], e), mq);
         const double d = we - p.lam * wg;
-        se += we;
-        sg += wg;
+        r.e += we;
+        r.g += wg;
         undecided |= wg > 0.0 && !(fabs(d) > edge * wg);
-        over += d > 0.0 ? d : 0.0;
-        gp += d > 0.0 ? wg : 0.0;
+        r.over += d > 0.0 ? d : 0.0;
+        r.gp += d > 0.0 ? wg : 0.0;
       }
+    }
+  };
+  // The chunk once more, from memory and in a rolled loop (from the registers its weights
+  // took 256 of them, and every chunk's pass 25 us for 17).
+  const auto sum_apart = [&]() {
+    const E *tr = logits_row<E>(a, b, p.n_acc), *dr = logits_row<E>(a, b, a.k + 1 + p.n_acc);
+    r.over = r.gp = 0.0;
+#pragma unroll 1
+    for (int v = 0; v < NV; ++v) {
+      const int i0 = (ch * NV + v) * 64 * N + l * N;
+      const u32x4 xv = load_raw<E>(tr, i0, a.V), yv = load_raw<E>(dr, i0, a.V);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const double we = weight(logit<E>(xv, e), mp, rate), wg = weight(logit<E>(yv, e), mq, rate);
+        const double d = we - p.lam * wg;
+        if (wg > 0.0 && !(fabs(d) > edge * wg)) {
+          const double ratio = we / wg;
+          r.eu += we;
+          r.gu += wg;
+          r.lo = fmin(r.lo, ratio);
+          r.hi = fmax(r.hi, ratio);
+        } else if (d > 0.0) {
+          r.over += d;
+          r.gp += wg;
+        }
+      }
+    }
+    r.eu = wave_sum64(r.eu);
+    r.gu = wave_sum64(r.gu);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      r.lo = fmin(r.lo, __shfl_xor(r.lo, o));
+      r.hi = fmax(r.hi, __shfl_xor(r.hi, o));
     }
   };
   const auto sum_one = [&](auto&& w) {
@@ -481,8 +525,8 @@ __global__ __launch_bounds__(kThreads) void sample_rest_kernel(SampleArgs a) {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         const double we = w(logit<E>(x.x[v], e), mp);
-        se += we;
-        over += (ch * NV + v) * 64 * N + l * N + e == p.skip ? 0.0 : we;
+        r.e += we;
+        r.over += (ch * NV + v) * 64 * N + l * N + e == p.skip ? 0.0 : we;
       }
     }
   };
@@ -491,16 +535,20 @@ __global__ __launch_bounds__(kThreads) void sample_rest_kernel(SampleArgs a) {
   if (both) {
     if (__all(is_near(lo_p, mp, rate) && is_near(lo_q, mq, rate))) sum_both(near);
     else sum_both(any);
+    if (!(p.lam > 0.0 && p.lam < INFINITY)) {  // no number to test against
+      r.lo = -INFINITY;
+      r.hi = INFINITY;
+    } else if (__any(undecided)) {
+      sum_apart();
+    }
+    r.g = wave_sum64(r.g);
+    r.gp = wave_sum64(r.gp);
   } else {
     if (__all(is_near(lo_p, mp, rate))) sum_one(near);
     else sum_one(any);
   }
-  RestSums r{wave_sum64(se), 0.0, wave_sum64(over), 0.0};
-  if (both) {
-    r.g = wave_sum64(sg);
-    r.gp = wave_sum64(gp);
-    if (__any(undecided)) r.gp = -1.0;
-  }
+  r.e = wave_sum64(r.e);
+  r.over = wave_sum64(r.over);
   if (l == 0) a.rest[static_cast<size_t>(b) * a.chunks + ch] = r;
 }
 
@@ -612,7 +660,9 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
       if (a.k == 0) t += chunk_sum(sums[c], maxes[c], mp, rate);
       else if (plain) t += rest[c].e;
       else if (!both) t += rest[c].over;
-      else if (rest[c].gp >= 0.0) t += fmax(rest[c].over - (lam - p.lam) * rest[c].gp, 0.0);
+      else if (!rest[c].marked(lam))
+        t += fmax(rest[c].over - (lam - p.lam) * rest[c].gp, 0.0) +
+             (rest[c].in(lam) ? rest[c].eu - lam * rest[c].gu : 0.0);
     }
     return t;
   };
@@ -620,7 +670,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
   if (both && sound) {
     // marked chunks, in any order: each is one thread's to add
     for (int g = 0; g < per; ++g) {
-      const uint64_t m = __ballot(c0 + g < c1 && !(rest[c0 + g].gp >= 0.0));
+      const uint64_t m = __ballot(c0 + g < c1 && rest[c0 + g].marked(lam));
       if ((tid & 63) == 0) sm_marked[w] = m;
       __syncthreads();
       for (int q = 0; q < kWaves; ++q) {

@@ -383,6 +383,35 @@ def test_probabilities_that_differ_by_less_than_the_sums(gpu_lib, dtype):
     assert n_acc.tolist() == [1] * B
 
 
+def test_probabilities_that_differ_by_as_little_both_ways(gpu_lib):
+    """Every id's p / q lies within some millionths of the ratio that decides its side."""
+    B, V = 4, 5003
+    g = torch.Generator().manual_seed(9)
+    target = 0.25 * torch.randn(B, 2, V, generator=g)
+    draft = target[:, :1] + 2e-6 * torch.randn(B, 1, V, generator=g)
+    x = torch.randint(0, V, (B,), generator=g, dtype=torch.int32)
+    for b in range(B):
+        draft[b, 0, x[b]] += 0.125
+    n_acc, _ = check((target, x[:, None], torch.full((B, 1), 0.99), torch.rand(B, generator=g), draft))
+    assert n_acc.tolist() == [0] * B
+
+
+@pytest.mark.parametrize("V", [2048, 30011])
+def test_bf16_logits_with_few_differences(gpu_lib, V):
+    """Target and draft differ by one of two values, so that nearly all ids have one of two
+    p / q, and the deciding ratio may be either of them to any accuracy."""
+    B = 8
+    g = torch.Generator().manual_seed(V)
+    target = torch.randint(-40, 40, (B, 2, V), generator=g).to(torch.bfloat16) / 16
+    step = torch.zeros(B, 1, V)
+    for b in range(B):
+        step[b, 0, torch.randperm(V, generator=g)[:[0, 1, 2, 40, V // 2, V - 2, V - 1, V][b]]] = 0.25
+    draft = (target[:, :1].float() + step).to(torch.bfloat16)
+    x = torch.stack([(draft[b, 0].float() - target[b, 0].float()).argmax() for b in range(B)])
+    u = torch.full((B, 1), 1 - 2.0 ** -24)
+    check((target, x[:, None].to(torch.int32), u, torch.rand(B, generator=g), draft))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_more_chunks_than_threads(gpu_lib, dtype):
     args = draw_inputs(6, 3, 1, 700001, dtype)
