@@ -519,6 +519,15 @@ struct UnitInfo {
   uint64_t vis;  // trees: bit j set where the row sees the key at start + j
 };
 
+// Trees: the nodes that the lane's row sees. Bits above the query's own node are no
+// ancestors: the plan's tile count (keys up to the group's last query) then holds for
+// every tree.
+__device__ __forceinline__ uint64_t tree_row(const AttnArgs& a, const UnitInfo& x) {
+  if (x.r >= x.R) return 0;
+  const int t = x.qlim - x.start;
+  return a.masks[static_cast<size_t>(x.b) * a.Tq + t] & (~0ull >> (63 - t));
+}
+
 template <int NT, bool TREE>
 __device__ __forceinline__ UnitInfo unit_info(const AttnArgs& a, int rec, int u, int nt, int lr) {
   UnitInfo x;
@@ -538,15 +547,7 @@ __device__ __forceinline__ UnitInfo unit_info(const AttnArgs& a, int rec, int u,
   const int row_end = min(x.R, row0 + 16 * NT);
   x.Lk = x.start + div_g(row_end - 1, a) + 1;  // keys visible to the row group
   x.qlim = x.r < x.R ? x.start + div_g(x.r, a) : -1;
-  x.vis = 0;
-  if constexpr (TREE) {
-    // bits above the query's own node are no ancestors: the plan's tile count
-    // (keys up to the group's last query) then holds for every tree
-    if (x.r < x.R) {
-      const int t = x.qlim - x.start;
-      x.vis = a.masks[static_cast<size_t>(x.b) * a.Tq + t] & (~0ull >> (63 - t));
-    }
-  }
+  x.vis = TREE ? tree_row(a, x) : 0;
   return x;
 }
 
@@ -1307,7 +1308,7 @@ __attribute__((amdgpu_waves_per_eu((TreeTiles<D, NT, KW>::kEu)))) void tree_attn
     asm volatile("" : "+v"(l));
     const int lr = l & 15, lg = l >> 4;
     const int tv = rec;  // block ids: lane kRecHead + j holds tile kt0 + j
-    const UnitInfo x = unit_info<NT, true>(a, tv, u, nt, lr);
+    UnitInfo x = unit_info<NT, false>(a, tv, u, nt, lr);  // (its mask only for the tree's chunks)
     const int next = min(u + static_cast<int>(gridDim.x), nunits - 1);
     rec = recs[static_cast<size_t>(next / a.Hkv) * kRecInts + l];
     const int kt0 = x.kt0, kt1 = x.kt1, start = x.start;
@@ -1474,6 +1475,7 @@ __attribute__((amdgpu_waves_per_eu((TreeTiles<D, NT, KW>::kEu)))) void tree_attn
       if (x.active) burst(ch, l, std::false_type{});
     }
     bool dropped = false;
+    if (nfull < nch) x.vis = tree_row(a, x);
     for (int ch = nfull; ch < nch; ++ch) {
       advance(ch);
       const int ck0 = (kt0 + ch * CT) * 16;
