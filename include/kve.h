@@ -226,8 +226,9 @@ int kve_tree_accept(const int32_t* tokens, const int32_t* parents, const int32_t
  *      sequence and position (any alignment of the type)
  * drafts [num_seqs, k], k <= 256 (an id outside [0, V) is rejected), u_accept [num_seqs, k] float,
  *      u_sample [num_seqs] float; k = 0 samples one token per sequence
- * temperatures [num_seqs] float, or NULL: `temperature` for all; where T is not
- *      positive and finite, n_acc is 0 and emitted -1
+ * temperatures [num_seqs] float, or NULL: `temperature` for all, taken in 64 bits like the
+ *      sums (in the range of positive floats); where a sequence's T is not positive and
+ *      finite, its n_acc is 0 and emitted -1
  * n_acc [num_seqs]; emitted [num_seqs, k + 1]: accepted drafts, the sampled token, then
  *      -1. A position whose logits have no distribution (NaN, +inf, all -inf) rejects its
  *      draft and emits -1.
@@ -240,7 +241,7 @@ size_t kve_sample_workspace_bytes(int num_seqs, int k, int vocab, int dtype);
 int kve_sample_verify(const void* target, int64_t target_seq_stride, int64_t target_pos_stride,
                       const void* draft, int64_t draft_seq_stride, int64_t draft_pos_stride,
                       const int32_t* drafts, const float* u_accept, const float* u_sample,
-                      const float* temperatures, float temperature, const int32_t* lens,
+                      const float* temperatures, double temperature, const int32_t* lens,
                       int num_rows, const int32_t* seq_rows, int num_seqs, int k, int vocab,
                       int dtype, int32_t* n_acc, int32_t* emitted, int32_t* keep_lens,
                       void* workspace, size_t workspace_bytes, void* stream);

@@ -65,6 +65,7 @@ P = ctypes.c_void_p
 I = ctypes.c_int
 I64 = ctypes.c_int64
 F = ctypes.c_float
+F64 = ctypes.c_double
 SZ = ctypes.c_size_t
 
 _SIGS = {
@@ -110,8 +111,8 @@ _SIGS = {
                                 P, P, SZ, I, P]),
     "kve_tree_accept": (I, [P, P, P, P, P, I, P, I, I, P, P, P, P, P, P, P, I, I, I, I, I, I, I, P]),
     "kve_sample_workspace_bytes": (SZ, [I, I, I, I]),
-    "kve_sample_verify": (I, [P, I64, I64, P, I64, I64, P, P, P, P, F, P, I, P, I, I, I, I, P, P, P,
-                              P, SZ, P]),
+    "kve_sample_verify": (I, [P, I64, I64, P, I64, I64, P, P, P, P, F64, P, I, P, I, I, I, I, P, P,
+                              P, P, SZ, P]),
 }
 
 

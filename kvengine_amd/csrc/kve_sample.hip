@@ -73,7 +73,7 @@ struct SampleArgs {
   int64_t ts, tp, ds, dp;  // element strides per sequence and position
   const int32_t* drafts;
   const float *u_accept, *u_sample, *temps;
-  float temp;
+  double temp;
   const int32_t *lens, *seq_rows;
   int num_rows, B, k, V, rows, chunks;  // rows per sequence: k + 1 target, then k draft
   int32_t *n_acc, *emitted, *keep;
@@ -87,10 +87,12 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kChunk = 2048;  // logits: 32 per lane of a wave, 8 per thread of a workgroup
 
-// log2(e) / T, or 0 where T is not positive and finite (the sequence has no answer)
+// log2(e) / T, or 0 where T is not positive and finite (the sequence has no answer). T in 32
+// bits would move every weight by up to 3e-8 (l - max) / T of it: 2 to 3 draws in 10^4 of
+// 151936 ids at T = 0.7 and 0.8, which are no 32-bit numbers.
 __device__ __forceinline__ double sample_rate(const SampleArgs& a, int b) {
-  const float t = a.temps ? a.temps[b] : a.temp;
-  return t > 0.0f && t < INFINITY ? 1.4426950408889634074 / static_cast<double>(t) : 0.0;
+  const double t = a.temps ? a.temps[b] : a.temp;
+  return t > 0.0 && t < INFINITY ? 1.4426950408889634074 / t : 0.0;
 }
 
 // 2^y = 2^n 2^f with n = round(y), f = y - n: 1 + f q(f), q the polynomial of degree 8
@@ -816,7 +818,7 @@ extern "C" int kve_sample_verify(const void* target, int64_t target_seq_stride,
                                  int64_t draft_seq_stride, int64_t draft_pos_stride,
                                  const int32_t* drafts, const float* u_accept,
                                  const float* u_sample, const float* temperatures,
-                                 float temperature, const int32_t* lens, int num_rows,
+                                 double temperature, const int32_t* lens, int num_rows,
                                  const int32_t* seq_rows, int num_seqs, int k, int vocab,
                                  int dtype, int32_t* n_acc, int32_t* emitted, int32_t* keep_lens,
                                  void* workspace, size_t workspace_bytes, void* stream) {
@@ -829,8 +831,9 @@ extern "C" int kve_sample_verify(const void* target, int64_t target_seq_stride,
               kSampleMaxDrafts, vocab);
   KVE_REQUIRE(dtype == KVE_DTYPE_BF16 || dtype == KVE_DTYPE_F32, "kve_sample_verify: dtype %d",
               dtype);
-  KVE_REQUIRE(temperatures || (temperature > 0.0f && temperature < INFINITY),
-              "kve_sample_verify: temperature %g", static_cast<double>(temperature));
+  // (the range of positive 32-bit numbers, over which no exponent leaves 64 bits)
+  KVE_REQUIRE(temperatures || (temperature > 0x1p-150 && temperature < 0x1.ffffffp127),
+              "kve_sample_verify: temperature %g", temperature);
   KVE_REQUIRE(!keep_lens || (lens && num_rows > 0), "kve_sample_verify: keep_lens needs lens");
   const size_t esz = dtype == KVE_DTYPE_BF16 ? 2 : 4;
   KVE_REQUIRE(((reinterpret_cast<uintptr_t>(target) | reinterpret_cast<uintptr_t>(draft)) &

@@ -1049,9 +1049,10 @@ def sample_verify(target_logits: torch.Tensor, drafts: torch.Tensor, u_accept: t
     (bf16 or float32; vocabulary contiguous, the other strides free), drafts [B, k] int32
     sampled from the draft's softmax at the same temperature; None: drafts that were not
     sampled (a greedy draft, a tree's node). u_accept [B, k], u_sample [B] float32 uniform
-    in [0, 1). temperature: a positive number, or [B] float32. k = 0 samples one token per
-    sequence. -> (n_acc [B], emitted [B, k+1]: accepted drafts, the sampled token, then -1,
-    keep [B] = lens - k + n_acc, or None without lens). Draws are exact: 64-bit sums."""
+    in [0, 1). temperature: a positive number, taken in 64 bits, or [B] float32. k = 0 samples
+    one token per sequence. -> (n_acc [B], emitted [B, k+1]: accepted drafts, the sampled
+    token, then -1, keep [B] = lens - k + n_acc, or None without lens). Draws are those of
+    64-bit sums."""
     _need(target_logits.dim() == 3 and target_logits.is_cuda, "target_logits must be [B, k+1, V]")
     dev, dtype, i32 = target_logits.device, target_logits.dtype, torch.int32
     B, k1, V = target_logits.shape

@@ -436,3 +436,25 @@ def test_as_many_drafts_as_a_call_takes(gpu_lib, with_draft):
     n_acc, _ = check((target, drafts, ua, us, draft if with_draft else None))
     if with_draft:  # (without one a draft of p(x) < u <= 1e-6 falls too)
         assert n_acc.tolist() == [0, 1, 63, 255, 256]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,top", [(0.8, 48.0), (0.7, 42.0), (0.3, 18.0), (1.3, 78.0)])
+@pytest.mark.parametrize("V", [2, 5000])
+def test_the_temperature_is_taken_in_64_bits(gpu_lib, dtype, T, top, V):
+    """Id 0 has p = 1 / (1 + e^(top / T)), and rounding T to 32 bits moves it by up to 60 x
+    3e-8 of it: u half way between the two values lies 2e-7 of it or more from either, ten
+    times the spacing of fp32 numbers and far past the sums' errors (1e-13)."""
+    logits = torch.full((1, 1, V), -INF, dtype=dtype)
+    logits[..., 0], logits[..., V - 1] = 0.0, top
+    p = [1.0 / (1.0 + torch.tensor(top / t, dtype=torch.float64).exp().item())
+         for t in (T, torch.tensor(T, dtype=torch.float32).item())]
+    u = torch.tensor([(p[0] + p[1]) / 2])
+    assert min(abs(float(u) / x - 1) for x in p) > 1e-7
+    none = torch.zeros(1, 0)
+    check((logits, none.int(), none, u), T)
+    two, first = logits.expand(1, 2, V).clone(), torch.zeros(1, 1, dtype=torch.int32)
+    check((two, first, u[None], torch.tensor([0.5]), None), T)
+    even = torch.full((1, 1, V), -INF, dtype=dtype)
+    even[..., 0] = even[..., V - 1] = 1.0
+    check((two, first, 2 * u[None], torch.tensor([0.5]), even), T)

@@ -116,3 +116,11 @@ def test_forward_hidden_checks_the_trees_shape():
     tree = torch.zeros(2, 5, dtype=torch.int64), torch.zeros(2, 5, dtype=torch.int32)
     with pytest.raises(ValueError, match="tree masks"):
         forward_hidden(None, ids, None, None, 16, fused=False, tree=tree)
+
+
+@pytest.mark.parametrize("T", [1e-46, 3.5e38, 1e300, 5e-324, -0.8])
+def test_sample_verify_refuses_temperatures_past_the_floats(T):
+    """(nothing is launched for them: the workspace is refused next)"""
+    rc, msg = call_sample(temp=T, wsb=8)
+    assert rc == -1 and "temperature" in msg
+    assert call_sample(temp=1e-45, wsb=8)[0] == call_sample(temp=3.4e38, wsb=8)[0] == -2
