@@ -427,7 +427,7 @@ __device__ __forceinline__ SamplePick decide(const SampleArgs& a, int b, double 
       state = u * q < p ? 0 : 1;
     }
   }
-  const int j = rate > 0.0 ? *sm_first >> 1 : 0;
+  const int j = *sm_first >> 1;
   const bool both = a.draft && j < a.k;
   SamplePick p;
   p.n_acc = j;
@@ -449,6 +449,7 @@ __global__ __launch_bounds__(kThreads) void sample_rest_kernel(SampleArgs a) {
   const int b = blockIdx.x / groups;
   const int ch = (blockIdx.x - b * groups) * kWaves + (threadIdx.x >> 6);
   const double rate = sample_rate(a, b);
+  if (!(rate > 0.0)) return;  // no answer: sample_pick_kernel says so without any sums
   const SamplePick p = decide<E>(a, b, rate, sm_rows, sm, &sm_first);
   if (ch == 0 && l == 0) a.picks[b] = p;
   if (ch >= a.chunks) return;
@@ -587,6 +588,23 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
   __shared__ int sm_at, sm_last;
   const int tid = threadIdx.x, w = tid >> 6, b = blockIdx.x;
   const double rate = sample_rate(a, b), u = a.u_sample[b];
+  const auto answer = [&](int n_acc, int32_t token) {
+    for (int j = tid; j <= a.k; j += kThreads) {
+      const int32_t d = j < a.k ? a.drafts[static_cast<size_t>(b) * a.k + j] : -1;
+      a.emitted[static_cast<size_t>(b) * (a.k + 1) + j] = j < n_acc ? d : j == n_acc ? token : -1;
+    }
+    if (tid == 0) {
+      a.n_acc[b] = n_acc;
+      if (a.keep) {
+        const int row = a.seq_rows ? a.seq_rows[b] : b;
+        a.keep[b] = row >= 0 && row < a.num_rows ? a.lens[row] - a.k + n_acc : 0;
+      }
+    }
+  };
+  if (!(rate > 0.0)) {  // a temperature without an answer (the whole workgroup's)
+    answer(0, -1);
+    return;
+  }
   const int per = cdiv(a.chunks, kThreads), c0 = min(tid * per, a.chunks),
             c1 = min(c0 + per, a.chunks);
   const RestSums* rest = a.rest + static_cast<size_t>(b) * a.chunks;
@@ -694,7 +712,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
     before = block_prefix(mine, sm, tid, R);
   }
   int32_t token = -1;
-  if (rate > 0.0 && sound && R > 0.0) {
+  if (sound && R > 0.0) {
     const double place = u * R;
     // the first thread whose running sum passes the place; the last one of any mass
     // where rounding lets none pass
@@ -744,18 +762,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
     }
     token = sm_at < a.V ? sm_at : sm_last;
   }
-  for (int j = tid; j <= a.k; j += kThreads) {
-    const int32_t d = j < a.k ? a.drafts[static_cast<size_t>(b) * a.k + j] : -1;
-    a.emitted[static_cast<size_t>(b) * (a.k + 1) + j] =
-        j < p.n_acc ? d : j == p.n_acc ? token : -1;
-  }
-  if (tid == 0) {
-    a.n_acc[b] = p.n_acc;
-    if (a.keep) {
-      const int row = a.seq_rows ? a.seq_rows[b] : b;
-      a.keep[b] = row >= 0 && row < a.num_rows ? a.lens[row] - a.k + p.n_acc : 0;
-    }
-  }
+  answer(p.n_acc, token);
 }
 
 // Workgroups of the stats launch that the chip holds at once (8 per compute unit).

@@ -458,3 +458,39 @@ def test_the_temperature_is_taken_in_64_bits(gpu_lib, dtype, T, top, V):
     even = torch.full((1, 1, V), -INF, dtype=dtype)
     even[..., 0] = even[..., V - 1] = 1.0
     check((two, first, 2 * u[None], torch.tensor([0.5]), even), T)
+
+
+def test_a_bad_temperature_costs_the_others_nothing(gpu_lib):
+    """Sequences without an answer (a greedy request's T = 0 among sampled ones) are not
+    tested in 64 bits draft by draft: the call is no slower for them (a third's slack), with
+    whole logits and with a filtered vocabulary."""
+    B, k, V = 6, 12, 151936
+    args = [t.to(DEV) for t in draw_inputs(12, B, k, V, torch.bfloat16)]
+    good = torch.ones(B, device=DEV)
+    bad = torch.tensor([1.0, 0.0, -1.0, INF, 0.0, 1.0], device=DEV)
+
+    def call(temps):
+        return kernels.sample_verify(*args[:4], draft_logits=args[4], temperature=temps)
+
+    def cost(temps):
+        times = []
+        for _ in range(7):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(10):
+                call(temps)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+    for filtered in (False, True):
+        if filtered:
+            for x in (args[0], args[4]):
+                x[:, :, 7::3] = -INF
+        want, got = call(good), call(bad)
+        for b in range(B):
+            if 0.0 < float(bad[b]) < INF:
+                assert got[0][b] == want[0][b] and torch.equal(got[1][b], want[1][b])
+            else:
+                assert got[0][b] == 0 and (got[1][b] == -1).all()
+        assert cost(bad) < 1.34 * cost(good)
