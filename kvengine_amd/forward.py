@@ -219,9 +219,11 @@ def forward_hidden(model, input_ids: torch.Tensor, kv: DeviceKV, rows: torch.Ten
     tree: the T tokens of a sequence are the nodes of a tree of drafts, (masks,
     depths) of kernels.tree_masks: node t's K/V lands at slot kv.lens + t, its
     rotary position is kv.lens + depth, and it attends to the history and the
-    nodes above it. The passes that issue their layers by one host call
-    (kernels.small_pass, kernels.f32_pass) take chains only: trees run the
-    split-K layer, or the library GEMMs where that does not fit. After the commit
+    nodes above it. In bf16 a pass over trees runs the layer that a chain's pass
+    of as many rows runs, so that a chain-shaped tree (one node: a decode step) has
+    the chain's bits for one attn_order, and invariant_gemm_rows holds for both.
+    The fp32 pass of one host call (kernels.f32_pass) takes chains only: trees run
+    the library GEMMs there, whose sums have another order. After the commit
     kernels.tree_accept picks the path and makes its K/V consecutive.
     """
     if tree is not None:
@@ -239,11 +241,12 @@ def forward_hidden(model, input_ids: torch.Tensor, kv: DeviceKV, rows: torch.Ten
         return _forward_splitk(model, input_ids, kv, rows, max_ctx, q_lens, attn_order, wide=True,
                                blocked_out=blocked_out, tree=tree)
     if fused:
-        if _small_fusable(model, n) and (tree is None or _splitk_ok(model, n)):
-            if tree is not None or _small_path(model, n) == "splitk":
+        if _small_fusable(model, n):
+            if _small_path(model, n) != "splitk":
+                return _forward_small(model, input_ids, kv, rows, max_ctx, q_lens, attn_order, tree)
+            if tree is None or _splitk_ok(model, n):
                 return _forward_splitk(model, input_ids, kv, rows, max_ctx, q_lens, attn_order,
                                        blocked_out=blocked_out, tree=tree)
-            return _forward_small(model, input_ids, kv, rows, max_ctx, q_lens, attn_order)
         if _wide_ok(model, n) and (n <= SPLITK_MAX_ROWS or _plain_tokens(model, input_ids)):
             return _forward_splitk(model, input_ids, kv, rows, max_ctx, q_lens, attn_order, wide=True,
                                    blocked_out=blocked_out, tree=tree)
@@ -309,12 +312,12 @@ def _splitk_ok(model, rows: int) -> bool:
 def invariant_gemm_rows(model, rows: int, wide: bool = False) -> tuple[bool, int | None]:
     """(ok, gemm_rows): with ok, forward_hidden(..., gemm_rows=gemm_rows) gives
     each sequence the same bits in every pass of at most `rows` rows, whatever
-    else shares the pass. gemm_rows is None when the decode layer takes every
-    such pass (<= 64 rows), else `rows` (the wide split-K layer). wide: take
-    the wide layer whatever the row count (its arithmetic is also what
-    forward_packed_wide gives a prefill, so a model whose every pass is wide
-    gets the same bits for a token from a prefill, a recompute or a verify
-    pass)."""
+    else shares the pass, as a chain or as a chain-shaped tree. gemm_rows is None
+    when the decode layer takes every such pass (<= 64 rows), else `rows` (the
+    wide split-K layer). wide: take the wide layer whatever the row count (its
+    arithmetic is also what forward_packed_wide gives a prefill, so a model whose
+    every pass is wide gets the same bits for a token from a prefill, a recompute
+    or a verify pass)."""
     if not _fusable(model):
         return False, None
     if wide:
@@ -541,13 +544,17 @@ def forward_packed_wide(model, ids: torch.Tensor, dst: torch.Tensor, B: int, T: 
     return xn
 
 
-def _prologue(model, input_ids, kv: DeviceKV, rows, max_ctx):
+def _prologue(model, input_ids, kv: DeviceKV, rows, max_ctx, tree=None):
     """Embedding rows and RoPE cos/sin of a pass's tokens in one launch (the
     same values as embed_tokens and rotary_emb's table lookup)."""
     inner = model.model
     emb = inner.embed_tokens.weight
     cos_t, sin_t = inner.rotary_emb.table(emb, max_ctx)
-    return kernels.pass_prologue(input_ids, emb, kv.lens, rows, cos_t, sin_t)
+    residual, cos, sin = kernels.pass_prologue(input_ids, emb, kv.lens, rows, cos_t, sin_t)
+    if tree is not None:  # the launch's angles are a chain's
+        at = _positions(kv, rows, input_ids.shape[1], tree)
+        cos, sin = (t.contiguous() for t in inner.rotary_emb(residual, at, max_ctx))
+    return residual, cos, sin
 
 
 def _plain_tokens(model, input_ids) -> bool:
@@ -559,18 +566,29 @@ def _plain_tokens(model, input_ids) -> bool:
             and emb.weight.is_contiguous() and emb.weight.data_ptr() % 16 == 0)
 
 
-def _forward_small(model, input_ids, kv: DeviceKV, rows, max_ctx, q_lens, attn_order):
+def _forward_small(model, input_ids, kv: DeviceKV, rows, max_ctx, q_lens, attn_order, tree=None):
     """Five launches per layer: fused QKV (RMSNorm, bias, RoPE, KV write),
     attention (+ its split merge), o_proj + residual, fused gate/up (RMSNorm,
-    SiLU*up), down_proj + residual, all issued by one host call. The residual
-    stream is updated in place."""
+    SiLU*up), down_proj + residual, all issued by one host call (trees: one by
+    one, that call's attention being a chain's). The residual stream is updated
+    in place."""
     inner = model.model
     B, T = input_ids.shape
     blk = _has_blocked(model)  # weights only: the kernels' other operands stay row-major
-    residual, cos, sin = _prologue(model, input_ids, kv, rows, max_ctx)
+    residual, cos, sin = _prologue(model, input_ids, kv, rows, max_ctx, tree)
     Hq = _q_heads(model, kv)
-    layer_attn = LayerAttention(kv, rows, B, T, Hq, max_ctx, q_lens, kv.k.dtype, attn_order)
+    layer_attn = LayerAttention(kv, rows, B, T, Hq, max_ctx, q_lens, kv.k.dtype, attn_order, tree)
     layers, consts = _pass_layers(model, blk)
+    if tree is not None:
+        for (li, norm, qkv, bias, o, post, gate_up, down), (eps, post_eps, scale) in zip(layers, consts):
+            q = kernels.fused_qkv(residual, norm, eps, qkv, bias, cos, sin, kv.k[li], kv.v[li],
+                                  kv.tables, kv.lens, Hq, seq_rows=rows, q_lens=q_lens,
+                                  blocked_w=blk)
+            out = layer_attn(q, li, scale)
+            kernels.linear_residual(out.view(B * T, -1), o, residual, blocked_w=blk)
+            act = kernels.fused_gate_up(residual, post, post_eps, gate_up, blocked_w=blk)
+            kernels.linear_residual(act, down, residual, blocked_w=blk)
+        return kernels.rmsnorm(residual, inner.norm.weight, inner.norm.variance_epsilon)
     return kernels.small_pass(layers, consts, residual, cos, sin, kv, rows, q_lens, Hq,
                               layer_attn.plan, max_ctx, attn_order, inner.norm.weight,
                               inner.norm.variance_epsilon, blk)
@@ -678,10 +696,7 @@ def _forward_splitk(model, input_ids, kv: DeviceKV, rows, max_ctx, q_lens, attn_
     n = B * T
     blk = _has_blocked(model)
     fused_o = not wide and SPLITK_FUSED_O and n <= SPLITK_FUSED_O_ROWS
-    residual, cos, sin = _prologue(model, input_ids, kv, rows, max_ctx)
-    if tree is not None:  # the prologue's angles are a chain's
-        cos, sin = inner.rotary_emb(residual, _positions(kv, rows, T, tree), max_ctx)
-        cos, sin = cos.contiguous(), sin.contiguous()
+    residual, cos, sin = _prologue(model, input_ids, kv, rows, max_ctx, tree)
     slots = kernels.kv_slots(kv.tables, kv.lens, B, T, kv.block_size, kv.k.shape[1], seq_rows=rows,
                              q_lens=q_lens)
     first = layers[0].input_layernorm

@@ -11,6 +11,8 @@ and the output is rounded by half a bf16 step (2^-8 of it). Each relative error 
 moves an output by at most that times max|v|.
 """
 
+import dataclasses
+import functools
 import random
 
 import pytest
@@ -681,3 +683,45 @@ def test_sampled_tree_decoding_gives_the_sampled_tokens(gpu_lib):
         accepted += int(n_acc[0])
     assert got[:len(prompt) + budget] == text[:len(prompt) + budget]
     assert accepted > 3
+
+
+@functools.lru_cache(maxsize=1)
+def twelve_layers():
+    from kvengine_amd.arch import QWEN25_0_5B
+    from kvengine_amd.model import build_model
+
+    arch = dataclasses.replace(QWEN25_0_5B, name="twelve layers", num_layers=12, vocab=1000)
+    return build_model(arch, seed=3, dtype=torch.bfloat16, device=DEV)
+
+
+@pytest.mark.parametrize("B,T", [(1, 1), (1, 2), (2, 2), (1, 4), (1, 5), (3, 6), (2, 16), (5, 13)])
+@pytest.mark.parametrize("name", ["tiny-gqa7-d64", "tiny-gqa8-d128", None])
+def test_a_chain_shaped_trees_pass_has_the_chains_bits(gpu_lib, name, B, T):
+    """bf16: hidden states and the whole pool, at every layer the row count selects and at the
+    wide layer that invariant_gemm_rows picks. (None: twelve layers of the 0.5B model's widths.
+    Sums in another order change one bf16 value in some 2^14, a few of a pass of four rows.)"""
+    from kvengine_amd.forward import forward_hidden, forward_with_own_cache, invariant_gemm_rows
+    from kvengine_amd.paged import PagedKVCache
+
+    model = tiny_model(name, torch.bfloat16) if name else twelve_layers()
+    ok, rows = invariant_gemm_rows(model, 160)
+    assert ok
+    chain = kernels.tree_masks(i32([[t - 1 for t in range(T)]] * B))
+    for seed in range(3):
+        r = random.Random(seed)
+        prompts = [[r.randrange(900) for _ in range(m)] for m in (3, 20, 45, 31, 16)[:B]]
+        ids = torch.tensor([[r.randrange(900) for _ in range(T)] for _ in prompts], device=DEV)
+        for kw in ({}, {"gemm_rows": rows}):
+            out = []
+            for tree in (None, chain):
+                pool = PagedKVCache.for_model(model, num_blocks=60, max_seqs=8)
+                seqs = [pool.new_sequence(i) for i in range(B)]
+                for s, p in zip(seqs, prompts):
+                    forward_with_own_cache(model, torch.tensor([p], device=DEV), s)
+                    s.reserve(T)
+                kv = pool.device_kv()
+                hid = forward_hidden(model, ids, kv, i32([s.row for s in seqs]), 45 + T,
+                                     attn_order=(8, 2), tree=tree, **kw)
+                out.append((hid, kv.k.clone(), kv.v.clone()))
+            for a, b in zip(*out):
+                assert torch.equal(a, b), (seed, kw)
