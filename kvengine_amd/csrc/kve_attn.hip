@@ -1776,9 +1776,10 @@ static int merge_batch(long long workgroups, int max_item_units) {
 }
 
 template <int D, bool BF16, int NT, int KW, bool TREE>
-static int launch_attn_t(const AttnArgs& a, const AttnCfg& p, hipStream_t st, bool bs16) {
+static int launch_attn_t(const char* name, const AttnArgs& a, const AttnCfg& p, hipStream_t st,
+                         bool bs16) {
   auto go = [&](auto kernel, int threads, size_t lds) {
-    const int rc = grant_lds(kernel, lds, "kve_paged_verify_attn");
+    const int rc = grant_lds(kernel, lds, name);
     if (rc) return rc;
     const int nwg = resident_workgroups(kernel, threads, lds);
     const long long max_units = static_cast<long long>(p.max_units) * a.Hkv;
@@ -1814,10 +1815,11 @@ static int launch_attn_t(const AttnArgs& a, const AttnCfg& p, hipStream_t st, bo
 // Instantiated (row tiles, key waves): (1, 1), (1, 2), (1, 4), (1, 8), (2-4, 1),
 // (2-4, 2), (2-3, 4), (6, 1), (6, 2), (8, 1).
 template <int D, bool BF16, bool TREE>
-static int launch_attn_nt(const AttnArgs& a, const AttnCfg& p, hipStream_t st, bool bs16) {
+static int launch_attn_nt(const char* name, const AttnArgs& a, const AttnCfg& p, hipStream_t st,
+                          bool bs16) {
   const int NT = p.NT, KW = p.KW;
 #define KVE_ATTN_CASE(nt, kw) \
-  if (NT == nt && KW == kw) return launch_attn_t<D, BF16, nt, kw, TREE>(a, p, st, bs16);
+  if (NT == nt && KW == kw) return launch_attn_t<D, BF16, nt, kw, TREE>(name, a, p, st, bs16);
   KVE_ATTN_CASE(1, 8)
   KVE_ATTN_CASE(1, 4)
   KVE_ATTN_CASE(1, 2)
@@ -1834,7 +1836,7 @@ static int launch_attn_nt(const AttnArgs& a, const AttnCfg& p, hipStream_t st, b
   KVE_ATTN_CASE(6, 2)
   KVE_ATTN_CASE(8, 1)
 #undef KVE_ATTN_CASE
-  set_error("kve_paged_verify_attn: no kernel for %d row tiles x %d key waves", NT, KW);
+  set_error("%s: no kernel for %d row tiles x %d key waves", name, NT, KW);
   return KVE_EUNSUPPORTED;
 }
 
@@ -2009,8 +2011,8 @@ static int paged_attn(const char* name, const uint64_t* masks, const void* q, co
   const bool bs16 = block_size == 16;
   const auto launch = [&](auto bf16, auto tree) {
     constexpr bool BF16 = decltype(bf16)::value, TREE = decltype(tree)::value;
-    return head_dim == 64 ? launch_attn_nt<64, BF16, TREE>(a, p, st, bs16)
-                          : launch_attn_nt<128, BF16, TREE>(a, p, st, bs16);
+    return head_dim == 64 ? launch_attn_nt<64, BF16, TREE>(name, a, p, st, bs16)
+                          : launch_attn_nt<128, BF16, TREE>(name, a, p, st, bs16);
   };
   const std::true_type yes{};
   const std::false_type no{};

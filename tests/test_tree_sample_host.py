@@ -1,6 +1,10 @@
 """Refusals of the tree and sampled verification entry points, and forward_hidden's tree
 argument checks: nothing is launched, so none of it needs a GPU."""
 
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -124,3 +128,22 @@ def test_sample_verify_refuses_temperatures_past_the_floats(T):
     rc, msg = call_sample(temp=T, wsb=8)
     assert rc == -1 and "temperature" in msg
     assert call_sample(temp=1e-45, wsb=8)[0] == call_sample(temp=3.4e38, wsb=8)[0] == -2
+
+
+def test_an_lds_refusal_names_the_trees_call():
+    """Without a device (hidden from the child, so that nothing can be launched) the first
+    thing an order of several row tiles asks for is refused."""
+    code = """if True:
+        from kvengine_amd import _lib
+        args = dict(q=16, k=16, v=16, masks=16, tables=16, rows=None, start=16, q_lens=None, B=2,
+                    T=16, Hq=16, Hkv=2, D=128, bs=16, max_blocks=16, num_rows=2, num_blocks=32,
+                    max_ctx=128, unit=8, kw=2, scale=0.125, dtype=1, plan=16, out=16, ws=256,
+                    wsb=1 << 30, layout=0)
+        rc = _lib.lib().kve_paged_tree_attn(*args.values(), None)
+        print(rc, _lib.lib().kve_last_error().decode())
+    """
+    env = dict(os.environ, HIP_VISIBLE_DEVICES="-1", ROCR_VISIBLE_DEVICES="-1")
+    out = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True,
+                         cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert out.returncode == 0, out.stderr
+    assert "LDS refused" in out.stdout and "kve_paged_tree_attn" in out.stdout, out.stdout
