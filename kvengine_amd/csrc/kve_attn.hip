@@ -1262,10 +1262,17 @@ struct TreeTiles {
   static constexpr int NW = NT * KW;                // waves
   static constexpr int CT = KW * burst_tiles<D, true>();  // tiles per chunk
   static constexpr int kChunk = CT * kDmaTileBytes<D>();
-  // Two workgroups share a CU at 128 registers and 64 KB each, where the key waves' fold
-  // and masks leave a wave with that: 32 sequences x 8 nodes (3B, four row tiles in two key
-  // waves) 19.9 us with one and no spills, 23.3 with two.
-  static constexpr bool kPair = NW <= 8 && (KW == 1 || NW <= 6);
+  // Two workgroups share a CU at 128 registers and 64 KB each: always with one key wave
+  // (at D = 128 4 to 16 registers spill), with two at D = 64 up to three row tiles (17 and 3
+  // spill). At D = 128 two key waves of two and three row tiles spill 47 and 34 that way,
+  // and one workgroup (151 and 147 registers) is the faster one. One layer, merge included,
+  // us with one workgroup / two:
+  //   3B, 4 nodes: 8 x 3000 tokens 14.8 / 17.4, 32 x 4000 31.9 / 35.5, 16 x 8000 33.8 / 39.9;
+  //   6 nodes: 15.8 / 18.5, 35.2 / 36.1, 37.4 / 40.5; 8 nodes (four row tiles) 32 short
+  //   histories 19.9 / 23.3
+  //   0.5B, 4 nodes: 8 x 3000 13.6 / 14.0, 32 x 4000 24.1 / 23.0, 16 x 8000 26.2 / 25.5;
+  //   6 nodes: 14.4 / 14.6, 26.1 / 22.7, 28.1 / 24.1
+  static constexpr bool kPair = NW <= 8 && (KW == 1 || (D == 64 && NW <= 6));
   static constexpr int kEu = kPair ? 4 : NW <= 8 ? 2 : 3;
   static constexpr int fit = (kPair ? 64 : 128) * 1024 / kChunk;
   static constexpr int NBUF = fit < 2 ? 2 : fit > 8 ? 8 : fit;
