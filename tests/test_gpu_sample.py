@@ -494,3 +494,16 @@ def test_a_bad_temperature_costs_the_others_nothing(gpu_lib):
             else:
                 assert got[0][b] == 0 and (got[1][b] == -1).all()
         assert cost(bad) < 1.34 * cost(good)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_greedy_drafts_of_a_whole_vocabulary(gpu_lib, dtype):
+    """Drafts without a distribution (the greedy draft's) at the models' vocabulary: sequences
+    whose drafts are the target's likeliest tokens, accepted to different lengths."""
+    B, k, V, T = 6, 4, 151936, 0.7
+    target, _, ua, us, _ = draw_inputs(15, B, k, V, dtype)
+    drafts = target[:, :k].argmax(-1).to(torch.int32)
+    for b in range(B):
+        target[b, torch.arange(min(b, k)), drafts[b, :min(b, k)].long()] += 20.0
+    n_acc, _ = check((target, drafts, ua, us, None), T)
+    assert n_acc.tolist() == sorted(n_acc.tolist()) and n_acc[0] < k and n_acc[-1] == k

@@ -725,3 +725,147 @@ def test_a_chain_shaped_trees_pass_has_the_chains_bits(gpu_lib, name, B, T):
                 out.append((hid, kv.k.clone(), kv.v.clone()))
             for a, b in zip(*out):
                 assert torch.equal(a, b), (seed, kw)
+
+
+@pytest.mark.parametrize("name,dtype,kw", [
+    ("tiny-gqa7-d64", torch.bfloat16, {}), ("tiny-gqa8-d128", torch.bfloat16, {"gemm_rows": 160}),
+    ("tiny-gqa7-d64", torch.float32, {}), ("tiny-gqa8-d128", torch.float32, {"fused": False})])
+@pytest.mark.parametrize("B,n", [(1, 3), (3, 11)])
+def test_a_captured_step_of_tree_decoding(gpu_lib, name, dtype, kw, B, n):
+    """Masks, pass, commit, picks, accept with compaction and rollback in one graph: replays
+    with other tokens and trees, eager steps and a second graph in between, leave what the
+    eager step leaves."""
+    from kvengine_amd.capture import no_gc
+    from kvengine_amd.forward import forward_hidden, forward_with_own_cache
+    from kvengine_amd.model import lm_head_weight
+    from kvengine_amd.paged import PagedKVCache
+
+    model = tiny_model(name, dtype)
+    r = random.Random(n)
+    pool = PagedKVCache.for_model(model, num_blocks=60, max_seqs=8)
+    seqs = [pool.new_sequence(i) for i in range(B)]
+    for s, m in zip(seqs, (5, 30, 47)):
+        forward_with_own_cache(model, torch.tensor([[r.randrange(900) for _ in range(m)]], device=DEV), s)
+        s.reserve(n)
+    kv, rows = pool.device_kv(), i32([s.row for s in seqs])
+    weight = lm_head_weight(model)
+    ids, parents = torch.zeros(B, n, dtype=torch.int32, device=DEV), i32([[-1] * n] * B)
+
+    def step():
+        hid = forward_hidden(model, ids.long(), kv, rows, 60, tree=kernels.tree_masks(parents), **kw)
+        kernels.commit(kv.lens, B, n, seq_rows=rows)
+        preds = kernels.lmhead_argmax(hid.reshape(B * n, -1), weight).view(B, n)
+        got = kernels.tree_accept(ids, parents, preds, kv=kv, seq_rows=rows)
+        kernels.rollback(kv.tables, kv.lens, got[3], pool.block_size, seq_rows=rows)
+        return (hid, preds) + got
+
+    start = [t.clone() for t in (kv.k, kv.v, kv.tables, kv.lens)]
+
+    def inputs(seed):
+        r = random.Random(seed)
+        trees = [random_tree(n, r) for _ in range(B)]
+        parents.copy_(i32(trees))
+        ids.copy_(i32([[r.randrange(900) for _ in range(n)] for _ in range(B)]))
+        back()
+        # the picks of a few nodes put into their children, so that paths are accepted
+        for _ in range(3):
+            preds = step()[1].tolist()
+            back()
+            ids.copy_(i32([[t if not j or r.random() < 0.3 else preds[b][trees[b][j]]
+                            for j, t in enumerate(row)] for b, row in enumerate(ids.tolist())]))
+
+    def back():
+        for t, was in zip((kv.k, kv.v, kv.tables, kv.lens), start):
+            t.copy_(was)
+
+    def state(got):
+        return [t.clone() for t in got] + [t.clone() for t in (kv.k, kv.v, kv.tables, kv.lens)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        inputs(1)
+        step()
+        back()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with no_gc(), torch.cuda.graph(g, stream=side):
+            out = step()
+        graphs.append((g, out))
+    moved = 0
+    for i in range(4):
+        inputs(i)
+        want = state(step())
+        moved += int(want[2].sum())
+        for g, out in graphs:
+            back()
+            g.replay()
+            for a, b in zip(state(out), want):
+                assert torch.equal(a, b), i
+    assert moved > 0
+
+
+@pytest.mark.parametrize("dtype,D,T,order", [
+    (torch.bfloat16, 64, 8, (0, 0)), (torch.bfloat16, 128, 16, (0, 0)),
+    (torch.bfloat16, 128, 13, (8, 2)), (torch.bfloat16, 128, 64, (16, 2)),
+    (torch.float32, 64, 11, (0, 0)), (torch.float32, 128, 40, (4, 2))])
+def test_the_same_call_gives_the_same_bits(gpu_lib, dtype, D, T, order):
+    case = Case(T, [603, 0, 1500, 77], T, 14 if D == 64 else 16, 2, D, dtype=dtype)
+    want = case.run(order)
+    case.check(want)
+    for _ in range(3):
+        assert torch.equal(case.run(order), want)
+
+
+@pytest.mark.parametrize("T,order", [(16, (2, 2)), (64, (2, 2)), (64, (4, 1))])
+def test_offsets_past_32_bits_with_several_row_tiles(gpu_lib, T, order):
+    """Blocks at the end of a pool of more than 2^32 elements for the kernel of several row
+    tiles, with an infinity in a node, which it reads from the pool a second time."""
+    Hq, Hkv, D, start = 16, 2, 128, 75
+    case = Case(12, [start], T, Hq, Hkv, D)
+    blk, off = case.slot(0, start + 2)
+    case.pool[1, blk, off, 1, 7] = float("inf")
+    want = case.run(order)
+    assert want.isinf().any() and not want.isnan().any()
+    NB = (1 << 32) // (Hkv * 16 * D) + 40
+    k = torch.empty(NB, Hkv, 16, D, dtype=torch.bfloat16, device=DEV)
+    v = torch.empty(NB, Hkv, D, 16, dtype=torch.bfloat16, device=DEV)
+    kk, vv = to_kernel_layout(case.pool[0], case.pool[1])
+    far = [NB - 1 - 3 * i for i in range(len(case.tables[0]))]
+    for b, f in zip(case.tables[0], far):
+        k[f], v[f] = kk[b].to(DEV), vv[b].to(DEV)
+    got = kernels.paged_tree_attn(case.q.to(DEV), k, v, i32([far]), i32([start]), start + T,
+                                  mask_tensor(case.masks), unit_blocks=order[0], key_waves=order[1])
+    assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("layers", [1, 3])
+def test_accept_moves_past_32_bits(gpu_lib, layers):
+    """Blocks at the end of a pool of more than 2^32 elements, in one layer and over three."""
+    Hkv, D, bs, n, start = 2, 128, 16, 40, 9
+    NB = (1 << 32) // (layers * Hkv * bs * D) + 60
+    k = torch.empty(layers, NB, Hkv, bs, D, dtype=torch.bfloat16, device=DEV)
+    v = torch.empty(layers, NB, Hkv, D, bs, dtype=torch.bfloat16, device=DEV)
+    table = [NB - 1, NB - 30, 2, NB - 2]
+    g = torch.Generator(device=DEV).manual_seed(layers)
+    for b in table:
+        k[:, b] = torch.randn(layers, Hkv, bs, D, generator=g, device=DEV).bfloat16()
+        v[:, b] = torch.randn(layers, Hkv, D, bs, generator=g, device=DEV).bfloat16()
+    near_k, near_v = k[:, table].cpu(), v[:, table].cpu()
+    path = [0, 5, 11, 12, 30, 39]
+    parents = [-1] + [0] * (n - 1)
+    for a, b in zip(path, path[1:]):
+        parents[b] = a
+    preds = [99] * n
+    for a, b in zip(path, path[1:]):
+        preds[a] = b
+    want_k, want_v = near_k.clone(), near_v.clone()
+    for j, c in enumerate(path):
+        (sb, so), (db, do) = (divmod(start + x, bs) for x in (c, j))
+        want_k[:, db, :, do] = near_k[:, sb, :, so]
+        want_v[:, db, :, :, do] = near_v[:, sb, :, :, so]
+    kv = DeviceKV(k, v, i32([table]), i32([start + n]), bs)
+    n_acc, _, _, keep = kernels.tree_accept(i32([list(range(n))]), i32([parents]), i32([preds]), kv=kv)
+    assert n_acc.tolist() == [5] and keep.tolist() == [start + 6]
+    assert torch.equal(k[:, table].cpu(), want_k) and torch.equal(v[:, table].cpu(), want_v)

@@ -147,3 +147,15 @@ def test_an_lds_refusal_names_the_trees_call():
                          cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     assert out.returncode == 0, out.stderr
     assert "LDS refused" in out.stdout and "kve_paged_tree_attn" in out.stdout, out.stdout
+
+
+def test_sample_workspace_holds_every_chunk():
+    """A sum (8 bytes) and a maximum (4) per row and chunk of 2048 logits, and 64 bytes of the
+    deciding position's sums per sequence and chunk, for 2k + 1 rows with a draft's logits."""
+    ws = _lib.lib().kve_sample_workspace_bytes
+    for B, k, V in ((32, 4, 151936), (1, 1, 2049), (3, 0, 50257), (2, 256, 4096)):
+        chunks = -(-V // 2048)
+        need = B * (2 * k + 1) * chunks * 12 + (B * chunks * 64 if k else 0)
+        assert ws(B, k, V, 1) >= need and ws(B, k, V, 0) >= need
+        rc, msg = call_sample(B=B, k=k, V=V, ts=(k + 1) * V, tp=V, ds=k * V, dp=V, wsb=need - 1)
+        assert rc == -2 and "workspace" in msg
