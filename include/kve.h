@@ -169,8 +169,8 @@ int kve_tree_masks(const int32_t* parents, const int32_t* node_counts, int num_s
  * [num_seqs, q_len] (kve_tree_masks), q_len <= KVE_TREE_MAX_NODES. A row that sees
  * no key at all is zeros. What a node that a row does not see holds, infinities and
  * NaN too, never reaches that row; a seen node's infinity or NaN does (the history,
- * which every row sees, is read as kve_paged_verify_attn reads it). scale > 0. The masks of a chain (bits 0..t) give
- * kve_paged_verify_attn's bits.
+ * which every row sees, is read as kve_paged_verify_attn reads it). scale > 0. The masks
+ * of a chain (bits 0..t) give kve_paged_verify_attn's bits.
  */
 int kve_paged_tree_attn(const void* q, const void* k_pool, const void* v_pool,
                         const int64_t* masks, const int32_t* block_tables,
@@ -219,8 +219,8 @@ int kve_tree_accept(const int32_t* tokens, const int32_t* parents, const int32_t
  * r = max(p_j - q_j, 0) at the first rejected j (p_j itself where that has no mass) and
  * r = p_k where every draft was accepted. So emitted tokens are distributed as the
  * target's own samples, for uniform numbers in [0, 1). The results are those of 64-bit
- * sums: a token is a place among V running sums, and 32-bit ones would move one draw in a
- * hundred. Tests of drafts use 32-bit sums where their error cannot decide one.
+ * sums: a token is a place among V running sums, and 32-bit ones would move a few draws in
+ * a thousand. Tests of drafts use 32-bit sums where their error cannot decide one.
  * target: [num_seqs, k + 1, V] logits, draft: [num_seqs, k, V] or NULL (drafts that were
  *      not sampled: q_j is one at x_j), both `dtype`, with element strides per
  *      sequence and position (any alignment of the type)

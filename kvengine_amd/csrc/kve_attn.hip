@@ -55,7 +55,6 @@
 // microbench against 1.2e-3 with the split), and the row sums l are the
 // product of a row of ones with the same hi and lo P^T on the matrix cores
 // instead of VALU adds.
-
 //
 // Trees (TREE, kve_paged_tree_attn): the new tokens are the nodes of a tree of
 // drafts, node t at cache slot start + t, and query t sees the history and those
@@ -1248,11 +1247,14 @@ __attribute__((amdgpu_waves_per_eu(NT >= 2 && NT * KW <= 6 ? 4 : 1))) void verif
 // units, bursts, key waves and order of every sum, and so its bits, as a kernel of its own.
 // A chunk wholly in the history, nearly all of them, runs through straight code; the masks
 // and what the tree's V needs are in a loop of their own, where V is mended in LDS before
-// any wave reads it. What bounds it is LDS: a wave reads 16 KB of fragments for 26 MFMAs of
-// 16 cycles, and LDS gives a CU 64 bytes a cycle, 2048 cycles of reads for the 832 of
-// MFMAs and some 600 of exponentials of 8 waves (two a SIMD). So workgroups of 8 waves
-// hold 128 registers and 64 KB, and two of them share a CU: the reads of one run beside
-// the products of the other. One layer, 16 sequences x 64 nodes, 8000 tokens (3B, units
+// any wave reads it. What bounds it is no pipe alone: a wave reads 16 KB of fragments (8
+// cycles a KB, as a benchmark of these addresses and the kernel's counters both have it)
+// for 26 MFMAs of 16 cycles, 1024 cycles of reads for the 832 of MFMAs and some 600 of
+// exponentials of 8 waves (two a SIMD). They come one after another in a wave, and the
+// kernel takes about their sum: at 16 sequences x 64 nodes over 8000 tokens, 309000 cycles
+// (140 us), LDS is busy for 39 % of them, the matrix pipes for 31 %, the vector ALU for
+// about as many. So workgroups of 8 waves hold 128 registers and 64 KB, and two of them
+// share a CU: some reads of one run beside products of the other. One layer, 16 sequences x 64 nodes, 8000 tokens (3B, units
 // of 512 keys, merge included): 238 us with the masks in one loop and one workgroup a CU,
 // 184 with two, 160 so. Two row tiles per wave, half the reads and half the waves: 154
 // there, but 314 for 283 with units of 256 keys in two key waves, and 33.3 for 32.0 at 32

@@ -7,14 +7,16 @@
 // drawn from r = max(p - q, 0), else, after the last draft, from p, by inversion: the
 // lowest id whose running sum exceeds u * sum(r).
 //
-// The draw is in 64 bits. The drawn id is a place among up to 150 000 running sums, and
-// an error of e in the sums moves a draw with a probability of about 2 V e: 32-bit
-// exponentials (6e-8) would answer one or two draws in a hundred differently from the
-// definition, these (4e-14) one in 10^8. A weight costs a wave 86 cycles in 64 bits and
-// 22 in 32 bits (its logit's loads 35, at the chip's copy rate), so only the logits of
-// the position that decides are taken in 64 bits: which position that is follows from
-// 32-bit sums, whose error is known, and where a test lies within it (2 in 10^5 tests)
-// from that row's 64-bit ones.
+// The draw is in 64 bits. The drawn id is a place among up to 150 000 running sums, and an
+// error in a sum moves the draws whose place falls between its two values. 400000 draws of
+// 151936 ids of spread 3 (T = 0.7, 0.8, 1; on the CPU) differ from the definition's in 8 to
+// 32 of a hundred with 32-bit sums one after another, in 1 to 3 of a thousand with 32-bit
+// sums by chunks of 2048, and still in 0.5 to 4 of 10^4 with 64-bit sums of 32-bit weights.
+// Weights within e of theirs move at most about 2 V e: these (4e-14) one draw in 10^8. A
+// weight costs a wave 86 cycles in 64 bits and 22 in 32 bits (its logit's loads 35, at the
+// chip's copy rate), so only the logits of the position that decides are taken in 64 bits:
+// which position that is follows from 32-bit sums, whose error is known, and where a test
+// lies within it (2 in 10^5 tests) from that row's 64-bit ones.
 //
 // Launches, each a dependency of the next over the whole vocabulary; a chunk is 2048
 // logits, one per wave:
@@ -765,7 +767,8 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
   answer(p.n_acc, token);
 }
 
-// Workgroups of the stats launch that the chip holds at once (8 per compute unit).
+// Workgroups of the stats launch: 8 per compute unit, what the chip holds at once in bf16
+// (58 and 63 registers). In fp32 (84 and 90) it holds 5, and the others follow.
 constexpr int kStatGrid = 2048;
 
 struct SampleCfg {
