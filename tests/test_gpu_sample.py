@@ -462,8 +462,8 @@ def test_the_temperature_is_taken_in_64_bits(gpu_lib, dtype, T, top, V):
 
 def test_a_bad_temperature_costs_the_others_nothing(gpu_lib):
     """Sequences without an answer (a greedy request's T = 0 among sampled ones) are not
-    tested in 64 bits draft by draft: the call is no slower for them (a third's slack), with
-    whole logits and with a filtered vocabulary."""
+    tested in 64 bits draft by draft: the call is not slower for them (it was, 38 times; twice
+    is the slack of short timings), with whole logits and with a filtered vocabulary."""
     B, k, V = 6, 12, 151936
     args = [t.to(DEV) for t in draw_inputs(12, B, k, V, torch.bfloat16)]
     good = torch.ones(B, device=DEV)
@@ -473,16 +473,13 @@ def test_a_bad_temperature_costs_the_others_nothing(gpu_lib):
         return kernels.sample_verify(*args[:4], draft_logits=args[4], temperature=temps)
 
     def cost(temps):
-        times = []
-        for _ in range(7):
-            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
-            a.record()
-            for _ in range(10):
-                call(temps)
-            b.record()
-            b.synchronize()
-            times.append(a.elapsed_time(b))
-        return min(times)
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        for _ in range(10):
+            call(temps)
+        b.record()
+        b.synchronize()
+        return a.elapsed_time(b)
     for filtered in (False, True):
         if filtered:
             for x in (args[0], args[4]):
@@ -493,7 +490,8 @@ def test_a_bad_temperature_costs_the_others_nothing(gpu_lib):
                 assert got[0][b] == want[0][b] and torch.equal(got[1][b], want[1][b])
             else:
                 assert got[0][b] == 0 and (got[1][b] == -1).all()
-        assert cost(bad) < 1.34 * cost(good)
+        times = [(cost(good), cost(bad)) for _ in range(12)]
+        assert min(t[1] for t in times) < 2 * min(t[0] for t in times)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
