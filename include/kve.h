@@ -42,6 +42,8 @@ extern "C" {
 
 #define KVE_DTYPE_F32 0
 #define KVE_DTYPE_BF16 1
+#define KVE_DTYPE_I8 2   /* codes of an 8-bit pool (kve_kv_write_q8) */
+#define KVE_DTYPE_E4M3 3 /* the same, 4 significant bits and an exponent, at most 448 */
 
 /*
  * Matrix layouts of the projections' operands (the `layout` argument).
@@ -245,6 +247,77 @@ int kve_sample_verify(const void* target, int64_t target_seq_stride, int64_t tar
                       int num_rows, const int32_t* seq_rows, int num_seqs, int k, int vocab,
                       int dtype, int32_t* n_acc, int32_t* emitted, int32_t* keep_lens,
                       void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The 8-bit cache: pools of one byte per value in the layout above, and for K and for V
+ * one float scale per block and kv head, [num_blocks, num_kv_heads]. A value is its code
+ * times its block's scale. pool_dtype KVE_DTYPE_I8: codes -127 .. 127, scale = largest
+ * value / 127; KVE_DTYPE_E4M3: scale = the least power of two that brings the largest value
+ * to 448 or below. Scales are at least 2^-100 (0 where the block is all zeros).
+ *
+ * kve_kv_write_q8: kve_kv_write into such a pool (kvengine/paged.py:197-205, 288-311).
+ * A block that the pass writes from its first row on takes the scale of its new rows; a
+ * block that holds rows already keeps its scale, or takes a larger one where a new row
+ * needs it, and then the held rows' codes are rounded to it. Codes are the exact
+ * quotients to the nearest, ties to even (E4M3: exact while every scale is a power of two).
+ * NaN becomes 0; an infinity becomes the largest code and does not count for the scale.
+ * Rows behind the pass's last keep their codes. A sequence's row may stand once in a
+ * launch, and no two sequences of it may share a block that they write.
+ * k_new, v_new, src_token_stride, dtype: as for kve_kv_write; block_size % 16 == 0,
+ * head_dim % 8 == 0 and <= 1024; rows and pools 16-byte aligned.
+ */
+int kve_kv_write_q8(const void* k_new, const void* v_new, int64_t src_token_stride, void* k_pool,
+                    void* v_pool, float* k_scale, float* v_scale, const int32_t* block_tables,
+                    const int32_t* seq_rows, const int32_t* start_pos, const int32_t* q_lens,
+                    int num_seqs, int q_len, int num_kv_heads, int head_dim, int block_size,
+                    int max_blocks, int num_rows, int num_blocks, int dtype, int pool_dtype,
+                    void* stream);
+
+/*
+ * kve_paged_window_attn: kve_paged_verify_attn where the query at position p sees the
+ * keys j <= p with j > p - window or j < sinks (window 0: every key up to p), over a pool of
+ * the queries' type or, with scales, an 8-bit one. The reference refuses models with a
+ * window (forward.py:186-188) and has no such cache.
+ * A key that a row does not see contributes nothing to it, whatever its K, V or scale
+ * holds, and blocks that no query of the pass sees are not read (their table entries may
+ * name anything). out: the shape and dtype of q; rows past q_lens and sequences that are
+ * skipped keep what is there.
+ * pool_dtype: dtype, KVE_DTYPE_I8 or KVE_DTYPE_E4M3 (k_scale, v_scale as above; else NULL)
+ * block_size % 16 == 0, head_dim 64 or 128, num_q_heads / num_kv_heads * q_len < 65536,
+ * scale > 0; q, pools, out and workspace 16-byte aligned
+ * workspace: kve_window_workspace_bytes(...) bytes (0: none needed), no initialisation
+ */
+size_t kve_window_workspace_bytes(int num_seqs, int q_len, int num_q_heads, int num_kv_heads,
+                                  int head_dim, int max_ctx, int window, int sinks,
+                                  int pool_dtype);
+
+int kve_paged_window_attn(const void* q, const void* k_layer, const void* v_layer,
+                          const float* k_scale, const float* v_scale, const int32_t* block_tables,
+                          const int32_t* seq_rows, const int32_t* start_pos, const int32_t* q_lens,
+                          int num_seqs, int q_len, int num_q_heads, int num_kv_heads, int head_dim,
+                          int block_size, int max_blocks, int num_rows, int num_blocks, int max_ctx,
+                          int window, int sinks, float scale, int dtype, int pool_dtype, void* out,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * kve_token_logprobs: for rows of logits [rows, vocab] (dtype, element stride row_stride,
+ * any alignment of the type) the log probability of a given token, the entropy of the
+ * softmax, and the `top` likeliest ids with their log probabilities (equal logits: lowest
+ * id first; a NaN ranks above every number). No counterpart in the reference, which decodes
+ * greedily and scores nothing.
+ * tokens [rows]: an id outside [0, vocab) gets NaN
+ * logprobs, entropy [rows] float; top_ids [rows, top], top_logprobs [rows, top] (NULL where
+ *      top = 0); top <= 32 and <= vocab
+ * A row without a distribution (a NaN, +inf, all -inf) has NaN log probabilities and entropy.
+ * workspace: kve_logprobs_workspace_bytes(...) bytes, 16-byte aligned; no
+ *      initialisation needed
+ */
+size_t kve_logprobs_workspace_bytes(int rows, int vocab, int top, int dtype);
+
+int kve_token_logprobs(const void* logits, int64_t row_stride, const int32_t* tokens, int rows,
+                       int vocab, int top, int dtype, float* logprobs, float* entropy,
+                       int32_t* top_ids, float* top_logprobs, void* workspace,
+                       size_t workspace_bytes, void* stream);
 
 /*
  * Scatter the new K/V rows of one layer into their paged slots.

@@ -53,10 +53,17 @@ EXPORTS = (
     "kve_tree_accept",
     "kve_sample_workspace_bytes",
     "kve_sample_verify",
+    "kve_kv_write_q8",
+    "kve_window_workspace_bytes",
+    "kve_paged_window_attn",
+    "kve_logprobs_workspace_bytes",
+    "kve_token_logprobs",
 )
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+DTYPE_I8 = 2
+DTYPE_E4M3 = 3
 
 _lock = threading.Lock()
 _lib = None
@@ -113,6 +120,12 @@ _SIGS = {
     "kve_sample_workspace_bytes": (SZ, [I, I, I, I]),
     "kve_sample_verify": (I, [P, I64, I64, P, I64, I64, P, P, P, P, F64, P, I, P, I, I, I, I, P, P,
                               P, P, SZ, P]),
+    "kve_kv_write_q8": (I, [P, P, I64, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, P]),
+    "kve_window_workspace_bytes": (SZ, [I, I, I, I, I, I, I, I, I]),
+    "kve_paged_window_attn": (I, [P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, I, F, I,
+                                  I, P, P, SZ, P]),
+    "kve_logprobs_workspace_bytes": (SZ, [I, I, I, I]),
+    "kve_token_logprobs": (I, [P, I64, P, I, I, I, I, P, P, P, P, P, SZ, P]),
 }
 
 

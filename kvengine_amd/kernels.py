@@ -1099,3 +1099,175 @@ def sample_verify(target_logits: torch.Tensor, drafts: torch.Tensor, u_accept: t
           _ptr(temps), temperature, _ptr(lens), num_rows, _ptr(seq_rows), B, k, V, code,
           n_acc.data_ptr(), emitted.data_ptr(), _ptr(keep), ws.data_ptr(), nbytes)
     return n_acc, emitted, keep
+
+
+# ---- 8-bit cache, windowed attention, log probabilities --------------------------
+
+# the types of an 8-bit pool's codes
+Q8_DTYPES = {torch.int8: _lib.DTYPE_I8, torch.float8_e4m3fn: _lib.DTYPE_E4M3}
+LOGPROBS_MAX_TOP = 32
+
+
+def _q8_code(t: torch.Tensor) -> int:
+    code = Q8_DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"unsupported pool dtype {t.dtype} (int8 or float8_e4m3fn)")
+    return code
+
+
+def _check_paged(block_tables, start_pos, seq_rows, q_lens, B: int, dev) -> tuple[int, int]:
+    """-> (rows, blocks per row) of the tables."""
+    _need(block_tables.dim() == 2 and start_pos.dim() == 1,
+          "block_tables [rows, max_blocks], start_pos [rows]")
+    num_rows, max_blocks = block_tables.shape
+    _check_on(block_tables, "block_tables", torch.int32, (num_rows, max_blocks), dev)
+    _check_on(start_pos, "start_pos", torch.int32, start_pos.shape, dev)
+    _check_on(seq_rows, "seq_rows", torch.int32, (B,), dev)
+    _check_on(q_lens, "q_lens", torch.int32, (B,), dev)
+    _need(start_pos.numel() >= num_rows, "start_pos needs one entry per table row")
+    _need(seq_rows is not None or num_rows >= B, "too few table rows")
+    return num_rows, max_blocks
+
+
+def kv_write_q8(k_new: torch.Tensor, v_new: torch.Tensor, k_layer: torch.Tensor,
+                v_layer: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                block_tables: torch.Tensor, start_pos: torch.Tensor,
+                seq_rows: torch.Tensor | None = None, q_lens: torch.Tensor | None = None) -> None:
+    """kv_write into an 8-bit pool: k_layer [NB, Hkv, bs, D], v_layer [NB, Hkv, D, bs] of
+    int8 or float8_e4m3fn codes, k_scale, v_scale [NB, Hkv] float32; a value is its code
+    times its block's scale. A block written from its first row on takes the scale of its
+    new rows (int8: largest / 127, e4m3: the least power of two that brings it to 448); one
+    that holds rows keeps its scale or takes a larger one, and its rows follow. Codes are
+    to the nearest, ties to even; NaN becomes 0, an infinity the largest code. bs a
+    multiple of 16. No two sequences of a call may write one block."""
+    _need(k_new.dim() == 4 and k_new.shape == v_new.shape and k_new.is_cuda,
+          "k_new/v_new must be [B, T, Hkv, D] on the GPU")
+    dev = k_new.device
+    B, T, Hkv, D = k_new.shape
+    _need(v_new.dtype == k_new.dtype and v_new.device == dev, "k_new/v_new differ")
+    _need(k_layer.dim() == 4, "k layer must be [NB, Hkv, bs, D]")
+    NB, _, bs, _ = k_layer.shape
+    pool = _q8_code(k_layer)
+    _check_on(k_layer, "k_layer", k_layer.dtype, (NB, Hkv, bs, D), dev)
+    _check_on(v_layer, "v_layer", k_layer.dtype, (NB, Hkv, D, bs), dev)
+    _check_on(k_scale, "k_scale", torch.float32, (NB, Hkv), dev)
+    _check_on(v_scale, "v_scale", torch.float32, (NB, Hkv), dev)
+    num_rows, max_blocks = _check_paged(block_tables, start_pos, seq_rows, q_lens, B, dev)
+    code = _dtype_code(k_new)
+    if B == 0 or T == 0:
+        return
+    st = k_new.stride()
+    if st != v_new.stride() or st[3] != 1 or st[2] != D or (B > 1 and st[0] != T * st[1]):
+        raise ValueError(f"k_new/v_new layouts {st}, {v_new.stride()} not [B, T, Hkv, D] with "
+                         "contiguous heads")
+    _call(_lib.lib().kve_kv_write_q8, "kve_kv_write_q8", dev, k_new.data_ptr(), v_new.data_ptr(),
+          st[1], k_layer.data_ptr(), v_layer.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+          block_tables.data_ptr(), _ptr(seq_rows), start_pos.data_ptr(), _ptr(q_lens), B, T, Hkv, D,
+          bs, max_blocks, num_rows, NB, code, pool)
+
+
+def _window_attn(q, k_layer, v_layer, k_scale, v_scale, block_tables, start_pos, max_ctx, window,
+                 sinks, seq_rows, q_lens, scale, out, code: int, pool: int):
+    dev, dtype = q.device, q.dtype
+    B, T, Hq, D = q.shape
+    NB, Hkv, bs, _ = k_layer.shape
+    _check_on(k_layer, "k_layer", k_layer.dtype, (NB, Hkv, bs, D), dev)
+    _check_on(v_layer, "v_layer", k_layer.dtype, (NB, Hkv, D, bs), dev)
+    if Hkv < 1 or Hq % Hkv:
+        raise ValueError(f"{Hq} q heads not a multiple of {Hkv} kv heads")
+    num_rows, max_blocks = _check_paged(block_tables, start_pos, seq_rows, q_lens, B, dev)
+    if max_ctx < 1 or max_blocks * bs < max_ctx:
+        raise ValueError(f"max_ctx {max_ctx} exceeds table capacity {max_blocks * bs}")
+    if sinks < 0:
+        raise ValueError(f"{sinks} sinks")
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _check_on(out, "out", dtype, (B, T, Hq, D), dev)
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not scale > 0.0:
+        raise ValueError(f"scale {scale} must be positive")
+    if B == 0 or T == 0:
+        return out
+    lib = _lib.lib()
+    # (a window of 2^30 tokens sees what none does)
+    window, sinks = min(window, 1 << 30), min(sinks, 1 << 30)
+    nbytes = lib.kve_window_workspace_bytes(B, T, Hq, Hkv, D, max_ctx, window, sinks, pool)
+    # the call's own, so that captured graphs share none
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _call(lib.kve_paged_window_attn, "kve_paged_window_attn", dev, q.data_ptr(), k_layer.data_ptr(),
+          v_layer.data_ptr(), _ptr(k_scale), _ptr(v_scale), block_tables.data_ptr(), _ptr(seq_rows),
+          start_pos.data_ptr(), _ptr(q_lens), B, T, Hq, Hkv, D, bs, max_blocks, num_rows, NB, max_ctx,
+          window, sinks, scale, code, pool, out.data_ptr(), _ptr(ws), nbytes)
+    return out
+
+
+def paged_window_attn(q: torch.Tensor, k_layer: torch.Tensor, v_layer: torch.Tensor,
+                      block_tables: torch.Tensor, start_pos: torch.Tensor, max_ctx: int, window: int,
+                      sinks: int = 0, seq_rows: torch.Tensor | None = None,
+                      q_lens: torch.Tensor | None = None, scale: float | None = None,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+    """paged_verify_attn under a sliding window: the query at position p sees the keys
+    j <= p with j > p - window (itself and the window - 1 before it) or j < sinks. q
+    [B, T, Hq, D], pools and tables as there; blocks of a multiple of 16 tokens. Blocks
+    that no query of the pass sees are not read, so they may have been given away. Rows
+    past q_lens, and sequences that max_ctx does not cover, keep what out holds. The
+    workspace is the call's own, so captured graphs share none."""
+    _need(q.dim() == 4 and q.is_contiguous() and q.is_cuda, "q must be contiguous [B, T, Hq, D]")
+    _need(k_layer.dim() == 4 and k_layer.dtype == q.dtype, "k layer must be [NB, Hkv, bs, D] of q's dtype")
+    if window < 1:
+        raise ValueError(f"window {window}, at least 1")
+    code = _dtype_code(q)
+    return _window_attn(q, k_layer, v_layer, None, None, block_tables, start_pos, max_ctx, window,
+                        sinks, seq_rows, q_lens, scale, out, code, code)
+
+
+def paged_q8_attn(q: torch.Tensor, k_layer: torch.Tensor, v_layer: torch.Tensor,
+                  k_scale: torch.Tensor, v_scale: torch.Tensor, block_tables: torch.Tensor,
+                  start_pos: torch.Tensor, max_ctx: int, window: int | None = None, sinks: int = 0,
+                  seq_rows: torch.Tensor | None = None, q_lens: torch.Tensor | None = None,
+                  scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """paged_verify_attn over an 8-bit pool (kv_write_q8: codes [NB, Hkv, bs, D] and
+    [NB, Hkv, D, bs] of int8 or float8_e4m3fn, scales [NB, Hkv] float32), q bf16 or float32.
+    window: None (every key up to the query's own) or paged_window_attn's, with its sinks;
+    the other arguments, what is not read and the result as there."""
+    _need(q.dim() == 4 and q.is_contiguous() and q.is_cuda, "q must be contiguous [B, T, Hq, D]")
+    _need(k_layer.dim() == 4, "k layer must be [NB, Hkv, bs, D]")
+    if window is not None and window < 1:
+        raise ValueError(f"window {window}, at least 1 (None: no window)")
+    NB, Hkv = k_layer.shape[:2]
+    pool = _q8_code(k_layer)
+    _check_on(k_scale, "k_scale", torch.float32, (NB, Hkv), q.device)
+    _check_on(v_scale, "v_scale", torch.float32, (NB, Hkv), q.device)
+    return _window_attn(q, k_layer, v_layer, k_scale, v_scale, block_tables, start_pos, max_ctx,
+                        window or 0, sinks, seq_rows, q_lens, scale, out, _dtype_code(q), pool)
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
+    """logits [R, V] (bf16 or float32, vocabulary contiguous, any row stride), tokens [R]
+    int32 -> (logprobs [R]: log softmax at the given tokens, entropy [R] of the softmax,
+    top_ids [R, top] int32: the likeliest ids, equal logits lowest id first, top_logprobs
+    [R, top]), float32. top <= LOGPROBS_MAX_TOP. An id outside the vocabulary gets NaN, as
+    does a row without a distribution."""
+    _need(logits.dim() == 2 and logits.is_cuda, "logits must be [R, V] on the GPU")
+    dev = logits.device
+    R, V = logits.shape
+    stride, one = logits.stride()
+    _need(one == 1 or V == 1, "logits need a contiguous vocabulary")
+    _check_on(tokens, "tokens", torch.int32, (R,), dev)
+    if not 0 <= top <= min(LOGPROBS_MAX_TOP, V):
+        raise ValueError(f"{top} alternatives of {V} ids, at most {LOGPROBS_MAX_TOP}")
+    code = _dtype_code(logits)
+    logprobs = torch.empty(R, dtype=torch.float32, device=dev)
+    entropy = torch.empty(R, dtype=torch.float32, device=dev)
+    ids = torch.empty((R, top), dtype=torch.int32, device=dev)
+    tops = torch.empty((R, top), dtype=torch.float32, device=dev)
+    if R == 0:
+        return logprobs, entropy, ids, tops
+    lib = _lib.lib()
+    nbytes = lib.kve_logprobs_workspace_bytes(R, V, top, code)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _call(lib.kve_token_logprobs, "kve_token_logprobs", dev, logits.data_ptr(), stride,
+          tokens.data_ptr(), R, V, top, code, logprobs.data_ptr(), entropy.data_ptr(),
+          ids.data_ptr() if top else None, tops.data_ptr() if top else None, ws.data_ptr(), nbytes)
+    return logprobs, entropy, ids, tops
