@@ -288,7 +288,7 @@ int kve_kv_write_q8(const void* k_new, const void* v_new, int64_t src_token_stri
  * workspace: kve_window_workspace_bytes(...) bytes (0: none needed), no initialisation
  */
 size_t kve_window_workspace_bytes(int num_seqs, int q_len, int num_q_heads, int num_kv_heads,
-                                  int head_dim, int max_ctx, int window, int sinks,
+                                  int head_dim, int max_ctx, int window, int sinks, int dtype,
                                   int pool_dtype);
 
 int kve_paged_window_attn(const void* q, const void* k_layer, const void* v_layer,

@@ -121,7 +121,7 @@ _SIGS = {
     "kve_sample_verify": (I, [P, I64, I64, P, I64, I64, P, P, P, P, F64, P, I, P, I, I, I, I, P, P,
                               P, P, SZ, P]),
     "kve_kv_write_q8": (I, [P, P, I64, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, P]),
-    "kve_window_workspace_bytes": (SZ, [I, I, I, I, I, I, I, I, I]),
+    "kve_window_workspace_bytes": (SZ, [I, I, I, I, I, I, I, I, I, I]),
     "kve_paged_window_attn": (I, [P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, I, I, F, I,
                                   I, P, P, SZ, P]),
     "kve_logprobs_workspace_bytes": (SZ, [I, I, I, I]),

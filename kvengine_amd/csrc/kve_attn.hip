@@ -348,21 +348,6 @@ __device__ __forceinline__ void wave_wait_vm() {
   __asm__ volatile("" ::: "memory");
 }
 
-// Workgroup barrier once this wave has at most `ahead` chunks of LPW direct
-// loads outstanding (0 <= ahead <= K; the count must be an immediate).
-template <int LPW, int K>
-__device__ __forceinline__ void barrier_after_chunks(int ahead) {
-  if constexpr (K > 0) {
-    if (ahead >= K) {
-      barrier_after_vm<K * LPW>();
-      return;
-    }
-    barrier_after_chunks<LPW, K - 1>(ahead);
-  } else {
-    barrier_after_vm<0>();
-  }
-}
-
 // Per-sequence state of a launch.
 struct SeqInfo {
   int row, start, T;  // T = 0: sequence skipped (bad row or length)

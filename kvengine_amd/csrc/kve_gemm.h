@@ -47,6 +47,21 @@ __device__ __forceinline__ void barrier_after_vm() {
   __asm__ volatile("" ::: "memory");
 }
 
+// Workgroup barrier once this wave has at most `ahead` chunks of LPW direct
+// loads outstanding (0 <= ahead <= K; the count must be an immediate).
+template <int LPW, int K>
+__device__ __forceinline__ void barrier_after_chunks(int ahead) {
+  if constexpr (K > 0) {
+    if (ahead >= K) {
+      barrier_after_vm<K * LPW>();
+      return;
+    }
+    barrier_after_chunks<LPW, K - 1>(ahead);
+  } else {
+    barrier_after_vm<0>();
+  }
+}
+
 // Workgroup of NW waves in NR row groups of NC = NW / NR: wave w (column
 // wc = w % NC, row group wr = w / NC) owns WN 16-row weight tiles and MTW =
 // MT / NR activation row tiles: BN = 16 WN NC weight rows (tile row r of

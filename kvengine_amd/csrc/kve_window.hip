@@ -10,21 +10,25 @@
 // with the codes.
 //
 // Work. Rows: the G = Hq / Hkv query heads of a kv head times the new tokens (row r =
-// t G + head). A wave holds MT tiles of 16 rows and walks the keys they see in steps of
-// SK = 16 NT keys (NT = 4 / bytes of an element: 16 fp32, 32 bf16, 64 8-bit): first the steps
-// that hold sinks, then those of the window; what lies between is not read. A workgroup is
-// four waves, RW row waves times KW = 4 / RW key waves that take steps in turn and are folded
-// through LDS; a long walk is cut into chunks of steps, a workgroup each, that a second launch
-// joins in chunk order.
+// t G + head). Rows walk the keys they see in steps of 64 (32 in fp32 at head_dim 128): first
+// the steps that hold sinks, then those of the window; what lies between is not read. A workgroup is four waves, in one of two forms:
+//  * up to 16 rows (decoding): one tile of 16 rows, the waves take the walk's steps in turn,
+//    each K/V byte goes into the registers of the one wave that multiplies it, and the four
+//    states are folded through LDS;
+//  * more rows (drafts, prompts): every wave has MT tiles of its own and all walk together;
+//    a step's K/V comes into LDS once, by direct loads into a ring of 64 KB (two workgroups
+//    a CU), RING - 1 steps ahead, and one barrier a step hands it over.
+// A long walk is cut into chunks of steps, a workgroup each, that a second launch joins in
+// chunk order.
 //
-// A step. Every lane loads 16 bytes at a time straight into registers: of K, lane (lr, lg)
-// of score product t reads key 4 NT (lr / 4) + 4 t + lr % 4 of the step, of V channel
-// 16 dt + lr, keys 4 NT lg ... Scores are S^T = K Q^T (16x16 matrix products, rows of K on
-// the M side): lane (lr, lg) then holds the scores of row lr and keys 4 NT lg + 4 t + i,
-// which are the keys of its V bytes, so P^T goes back as an operand of O^T = V^T P^T without
-// leaving the lane. K and V are read by the one wave that needs them (other row waves' reads
-// hit the caches), so nothing is staged and no barrier stands in the walk: while one step's
-// probabilities are taken the next one's K is on its way, and its V during the scores.
+// A step. The unit of reading is a fragment: 16 bytes a lane, as the lane needs them for a
+// matrix product. A step has parts of 16 NS keys, NS = 4 / bytes of an element (one part in
+// 8 bits, two in bf16). Of K, lane (lr, lg) of a part's score product t reads key 4 NS (lr / 4) +
+// 4 t + lr % 4, of V channel 16 dt + lr, keys 4 NS lg ... Scores are S^T = K Q^T
+// (16x16 matrix products, rows of K on the M side): lane (lr, lg) then holds the scores of
+// row lr and keys 4 NS lg + 4 t + i, which are the keys of its V bytes, so P^T goes back
+// as an operand of O^T = V^T P^T without leaving the lane. A direct load writes its 64 lanes'
+// 16 bytes one after another, so a fragment is read back from LDS without bank conflicts.
 //
 // Numbers. bf16: products in bf16, P as the sum of two bf16 (16 bits of it). fp32: fp32
 // products. 8 bits: codes are exact in fp16, so the products are fp16's: q is scaled to the
@@ -37,6 +41,7 @@
 // row sees in part are taken without the non-finite values, which are then added to the rows
 // that do see them (add_nonfinite). Other steps are seen whole by every row.
 
+#include "kve_gemm.h"
 #include "kve_q8.h"
 
 #include <algorithm>
@@ -60,9 +65,9 @@ struct WindowArgs {
   float* part_ml;  // [B][Hkv][splits][rows][2]
   int B, Tq, Hq, Hkv, G, bs, tpb, max_blocks, num_rows, num_blocks, max_ctx;
   int window, sinks;
-  int rw, row_groups, chunk, splits;  // chunk: steps of a workgroup
+  int row_groups, chunk, splits;  // chunk: steps of a workgroup
   float scale_log2;
-  uint32_t g_magic, tpb_magic;
+  uint32_t g_magic;
 };
 
 constexpr int kWinThreads = 256;
@@ -106,14 +111,20 @@ __device__ __forceinline__ Walk walk_of(const WindowArgs& a, const WinSeq& s, in
   return w;
 }
 
+// Keys of a step: 64, or what 32 KB of K and V hold (half the ring).
+__host__ __device__ constexpr int step_keys(int elem_bytes, int D) {
+  return elem_bytes * D == 512 ? 32 : 64;
+}
+
 // ---- element types ----------------------------------------------------------------
 
-template <Pool P>
+template <Pool P, int D>
 struct PoolOf {
   static constexpr int ES = P == Pool::kF32 ? 4 : P == Pool::kBf16 ? 2 : 1;
-  static constexpr int NT = 4 / ES;    // 16-key tiles of a step
-  static constexpr int SK = 16 * NT;
   static constexpr bool Q8B = ES == 1;
+  static constexpr int NS = 4 / ES;                  // 16-key tiles of a part of a step
+  static constexpr int U = step_keys(ES, D) / (16 * NS);  // parts
+  static constexpr int NT = NS * U, SK = 16 * NT;    // tiles and keys of a step
 };
 
 // 4 codes -> 4 fp16, exact: int8 + 128 set into the low bits of 1024 + x, less 1152.
@@ -203,19 +214,32 @@ __device__ __forceinline__ float nonfinite_of(const uint8_t* p) {
 }
 
 // ---- the walk ---------------------------------------------------------------------
-// PARTS: 16-bit parts that P is taken as (and, over 8-bit pools, q): 8-bit pools 1 for bf16
-// queries and 2 for fp32 ones, bf16 2; fp32 takes P whole (1).
-template <Pool P, int PARTS, int D, int MT>
-__global__ __launch_bounds__(kWinThreads, 2) void window_attn_kernel(WindowArgs a) {
-  using X = PoolOf<P>;
-  constexpr int ES = X::ES, NT = X::NT, SK = X::SK;
+
+constexpr int kRingBytes = 64 * 1024;
+
+// How far a row's maximum may lag behind its scores (in powers of 2) before its state is
+// rescaled: P stays below 2^8 in fp32 and bf16, below 2^15 in fp16.
+template <bool F16>
+constexpr float kLag = F16 ? 1.0f : 8.0f;
+
+// QP: fp16 parts that q is taken as over 8-bit pools (1: bf16 queries, 2: fp32; else 1).
+// PP: 16-bit parts of P (fp32 pools: 1, whole).
+template <Pool P, int QP, int PP, int D, int MT, bool SHARED>
+__global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void window_attn_kernel(WindowArgs a) {
+  using X = PoolOf<P, D>;
+  constexpr int ES = X::ES, NS = X::NS, U = X::U, NT = X::NT, SK = X::SK, SP = 16 * NS;
   constexpr bool Q8B = X::Q8B, F32 = P == Pool::kF32;
-  constexpr bool QBF = P == Pool::kBf16 || (Q8B && PARTS == 1);  // q and out in bf16
-  constexpr int QP = Q8B ? PARTS : 1;
-  constexpr int NJ = D * ES / 64;  // 16-byte pieces of a K row per lane
+  constexpr bool QBF = P == Pool::kBf16 || (Q8B && QP == 1);  // q and out in bf16
+  constexpr int KW = SHARED ? 1 : 4;
+  constexpr int ROWS = 16 * MT * (4 / KW);
+  constexpr int NJ = D * ES / 64;  // fragments of a K row
   constexpr int DT = D / 16;
-  constexpr int NF = F32 ? D / 16 : D / 32;  // q fragments of 16 bytes
-  constexpr int BATCH = 64 / NT;             // steps whose block ids a wave holds
+  constexpr int NF = F32 ? D / 16 : D / 32;  // fragments of q
+  constexpr int FRAGS = U * 2 * DT;          // of a step: each part's K (NS NJ = DT), then its V
+  constexpr int LPW = FRAGS / 4;             // a wave's loads of a shared step
+  static_assert(NS * NJ == DT, "as many fragments of K as of V");
+  constexpr int RING = kRingBytes / (FRAGS * 1024);
+  constexpr int BATCH = 64 / NT;  // steps whose block ids a wave holds
   extern __shared__ float sm[];
 
   const int tid = threadIdx.x, l = tid & 63, lr = l & 15, lg = l >> 4;
@@ -226,20 +250,195 @@ __global__ __launch_bounds__(kWinThreads, 2) void window_attn_kernel(WindowArgs 
   const int c = u % a.splits;
   u /= a.splits;
   const int kvh = u % a.Hkv, b = u / a.Hkv;
-  const int KW = 4 / a.rw, rwi = wid / KW, kw = wid - rwi * KW;
   const WinSeq s = win_seq(a, b);
-  const int R = a.G * s.T, rows = 16 * MT * a.rw;
-  if (rg * rows >= R) return;
-  const int row0 = rg * rows + rwi * 16 * MT, row1 = min(R, row0 + 16 * MT);
+  const int R = a.G * s.T, g0 = rg * ROWS;
+  if (g0 >= R) return;
+  const Walk w = walk_of<SK>(a, s, g0, min(R, g0 + ROWS));
+  const int chunks = cdiv(w.total, a.chunk);
+  if (c >= chunks) return;
+  // the wave's rows, and its steps at, at + KW, ... (n of them)
+  const int row0 = SHARED ? g0 + wid * 16 * MT : g0, row1 = min(R, row0 + 16 * MT);
+  const int kw = SHARED ? 0 : wid, at = c * a.chunk + kw;
+  const int n = cdiv(max(min(w.total, (c + 1) * a.chunk) - at, 0), KW);
   const bool active = row0 < R;
-  const Walk w = walk_of<SK>(a, s, active ? row0 : 0, active ? row1 : 1);
-  const int chunks = active ? cdiv(w.total, a.chunk) : 0;
-  // (row waves of one workgroup may end at different chunks; they meet at the fold only)
-  const int end = c < chunks ? min(w.total, (c + 1) * a.chunk) : 0;
+  const int p0 = active ? s.start + div_magic(row0, a.G, a.g_magic) : w.p0;
+  const int p1 = active ? s.start + div_magic(row1 - 1, a.G, a.g_magic) : w.p1;
+
+  // q as it lies in memory: the lane's channels of row lr of each tile, in the order of its
+  // K fragments. Asked for first, for behind the first K and V it would wait for all of them.
+  constexpr int QV = Q8B && !QBF ? 2 : 1;  // vectors of a fragment of 8 channels
+  u32x4 qf[MT][QP][NF], qraw[MT][Q8B ? NF * QV : 1];
+  int qpos[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int r = min(row0 + mt * 16 + lr, R - 1);
+    const int t = div_magic(r, a.G, a.g_magic), h = kvh * a.G + r - t * a.G;
+    qpos[mt] = s.start + t;
+    const size_t qat = ((static_cast<size_t>(b) * a.Tq + t) * a.Hq + h) * D;
+    if constexpr (!Q8B) {
+      const uint8_t* qp = static_cast<const uint8_t*>(a.q) + qat * ES + lg * 16;
+#pragma unroll
+      for (int j = 0; j < NF; ++j) qf[mt][0][j] = *reinterpret_cast<const u32x4*>(qp + j * 64);
+    } else {
+      // channels 64 j + 16 lg + 8 f .. of fragment 2 j + f
+      const uint8_t* qp = static_cast<const uint8_t*>(a.q) + (qat + lg * 16) * (2 * QV);
+#pragma unroll
+      for (int x = 0; x < NF * QV; ++x)
+        qraw[mt][x] = *reinterpret_cast<const u32x4*>(
+            qp + ((x / QV >> 1) * 64 + (x / QV & 1) * 8) * (2 * QV) + x % QV * 16);
+    }
+  }
+
+  // the first steps' block ids
+  const int32_t* table = a.tables + static_cast<size_t>(s.row) * a.max_blocks;
+  const int last_tile = w.p1 >> 4;
+  const auto tile_of = [&](int i) {  // lane: tile l % NT of step i + l / NT (past the last: it again)
+    const int st = w.step(at + min(i + l / NT, n - 1) * KW);
+    return min(st * NT + l % NT, last_tile);
+  };
+  const auto read_table = [&](int i) {  // (within the table: start + T <= max_ctx <= its blocks)
+    const int tile = tile_of(i);
+    return table[a.tpb == 1 ? tile : tile / a.tpb];
+  };
+  // Where the tile is, in units of 16 bytes from the start of the K and the V pool (the host
+  // holds pools below 2^36 bytes), and its (block, head).
+  struct Place {
+    uint32_t k, v;
+    int bh;
+  };
+  const auto place = [&](int blk, int i) {
+    const int part = a.tpb == 1 ? 0 : tile_of(i) % a.tpb;
+    Place x;
+    x.bh = (static_cast<unsigned>(blk) < static_cast<unsigned>(a.num_blocks) ? blk : 0) * a.Hkv + kvh;
+    const uint32_t first = static_cast<uint32_t>(x.bh) * static_cast<uint32_t>(a.bs * D * ES / 16);
+    x.k = first + part * (D * ES);
+    x.v = first + part * ES;
+    return x;
+  };
+  Place ids{}, ids1{};  // of the batch, of the next one
+  int raw1 = 0;         // the next batch's table entries
+  float ksl = 0, vsl = 0, ks1 = 0, vs1 = 0;  // the lane's tile's scales, the next batch's
+  if (n > 0) {
+    ids = place(read_table(0), 0);
+    if (n > BATCH) raw1 = read_table(BATCH);
+  }
+
+  // fragments: where the lane reads within a tile
+  const int kk = 4 * NS * (lr >> 2) + (lr & 3), vk = 4 * NS * lg;
+  const size_t vrow = static_cast<size_t>(a.bs) * ES;
+  const uint8_t* klane = a.k + (kk & 15) * D * ES + lg * 16;
+  const uint8_t* vlane = a.v + lr * vrow + (vk & 15) * ES;
+  // the lane's K or V address of part p of step i; `now`: the step whose batch `ids` is
+  const auto k_at = [&](int i, int p, int now) {
+    const int id = __shfl(static_cast<int>(i / BATCH == now / BATCH ? ids.k : ids1.k),
+                          i % BATCH * NT + p * NS + (kk >> 4));
+    return klane + static_cast<uint64_t>(static_cast<uint32_t>(id)) * 16;
+  };
+  const auto v_at = [&](int i, int p, int now) {
+    const int id = __shfl(static_cast<int>(i / BATCH == now / BATCH ? ids.v : ids1.v),
+                          i % BATCH * NT + p * NS + (vk >> 4));
+    return vlane + static_cast<uint64_t>(static_cast<uint32_t>(id)) * 16;
+  };
+
+  u32x4 kf[U][SHARED ? 1 : DT], vf[U][SHARED ? 1 : DT];
+  uint8_t* ring = reinterpret_cast<uint8_t*>(sm);
+  const auto load_k = [&](int i, int now) {
+#pragma unroll
+    for (int p = 0; p < U; ++p) {
+      const uint8_t* at = k_at(i, p, now);
+#pragma unroll
+      for (int f = 0; f < DT; ++f)
+        kf[p][f] = *reinterpret_cast<const u32x4*>(at + f / NJ * (4 * D * ES) + f % NJ * 64);
+    }
+  };
+  const auto load_v = [&](int i, int now) {
+#pragma unroll
+    for (int p = 0; p < U; ++p) {
+      const uint8_t* at = v_at(i, p, now);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        vf[p][dt] = *reinterpret_cast<const u32x4*>(at + dt * 16 * vrow);
+    }
+  };
+  // Waves 0 and 1 load a shared step's K fragments, 2 and 3 its V's: what they read is
+  // settled here, for the loop.
+  const bool is_k = wid < 2;
+  const int f0 = (wid & 1) * (DT / 2);
+  const uint8_t* mine = is_k ? klane : vlane;
+  const int my_tile = is_k ? kk >> 4 : vk >> 4;
+  uint32_t skip[DT / 2];  // from the lane's address to each fragment
+#pragma unroll
+  for (int x = 0; x < DT / 2; ++x)
+    skip[x] = is_k ? (f0 + x) / NJ * (4 * D * ES) + (f0 + x) % NJ * 64
+                   : static_cast<uint32_t>((f0 + x) * 16 * vrow);
+  const auto stage = [&](int i, int now) {
+    const bool here = i / BATCH == now / BATCH;
+    const int id = static_cast<int>(is_k ? (here ? ids.k : ids1.k) : (here ? ids.v : ids1.v));
+    uint8_t* to = ring + (i % RING) * (FRAGS * 1024) + ((is_k ? 0 : DT) + f0) * 1024;
+#pragma unroll
+    for (int p = 0; p < U; ++p) {
+      const uint32_t off = __shfl(id, i % BATCH * NT + p * NS + my_tile);
+      const uint8_t* at = mine + static_cast<uint64_t>(off) * 16;
+#pragma unroll
+      for (int x = 0; x < DT / 2; ++x)
+        __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(at + skip[x]),
+                                         (__attribute__((address_space(3))) void*)(to + (2 * DT * p + x) * 1024),
+                                         16, 0, 0);
+    }
+  };
+  if (SHARED) {
+#pragma unroll
+    for (int i = 0; i < RING - 1; ++i)
+      if (i < n) stage(i, 0);
+  } else if (n > 0) {
+    load_k(0, 0);
+    load_v(0, 0);
+  }
+  if (Q8B && n > 0) {
+    ksl = a.ks[ids.bh];
+    vsl = a.vs[ids.bh];
+  }
+
+  float rf[MT];  // score -> exponent of 2
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    rf[mt] = a.scale_log2;
+    if constexpr (Q8B) {
+      float x[NF][8];
+      float top = 0.0f;
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if constexpr (QBF)
+            x[f][e] = __uint_as_float(e & 1 ? qraw[mt][f][e >> 1] & 0xffff0000u : qraw[mt][f][e >> 1] << 16);
+          else
+            x[f][e] = __uint_as_float(qraw[mt][2 * f + (e >> 2)][e & 3]);
+          top = fmaxf(top, fabsf(x[f][e]));
+        }
+      }
+      top = max_across_groups(top);
+      // the row's largest value to [2^13, 2^14): what falls below fp16's steps of 2^-24
+      // there is below 2^-37 of it
+      const int ex = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
+      rf[mt] = ldexpf(a.scale_log2, ex - 14);
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[f][e] = ldexpf(x[f][e], 14 - ex);
+#pragma unroll
+        for (int p = 0; p < QP; ++p) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            qf[mt][p][f][e] = p + 1 < QP ? split_f16x2(x[f][2 * e], x[f][2 * e + 1])
+                                         : pack_f16x2(x[f][2 * e], x[f][2 * e + 1]);
+        }
+      }
+    }
+  }
 
   f32x4 acc[MT][DT];
   float m[MT], lsum[MT];
-  int qpos[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
@@ -247,313 +446,291 @@ __global__ __launch_bounds__(kWinThreads, 2) void window_attn_kernel(WindowArgs 
     m[mt] = kNone;
     lsum[mt] = 0.0f;
   }
-  float ref = kMinScale;  // acc is in units of it: a power of two that no s_v seen so far exceeds
+  // 8-bit: acc is in units of ref 2^-14, ref a power of two that no s_v of a tile seen so far
+  // exceeds
+  float ref = kMinScale;
+  const auto raise_ref = [&](int i) {  // the batch that starts at step i has become the current one
+    const int k0 = tile_of(i) * 16;
+    const bool seen = k0 + 15 > w.p0 - a.window || k0 < a.sinks;
+    float top = seen && vsl < INFINITY ? vsl : 0.0f;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+    top = max_across_groups(top);
+    if (top > ref) {  // (the same in every lane)
+      const float to = ldexpf(1.0f, min(__builtin_amdgcn_frexp_expf(top), 127)), f = ref / to;
+      ref = to;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[mt][dt] *= f;
+      }
+    }
+  };
+  if (Q8B && n > 0) raise_ref(0);
 
-  if (c * a.chunk + kw < end) {
-    // q: the lane's channels of row lr of each tile, in the order of its K pieces
-    u32x4 qf[MT][QP][NF];
-    float rf[MT];  // score -> exponent of 2
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int r = min(row0 + mt * 16 + lr, R - 1);
-      const int t = div_magic(r, a.G, a.g_magic), h = kvh * a.G + r - t * a.G;
-      qpos[mt] = s.start + t;
-      const size_t at = ((static_cast<size_t>(b) * a.Tq + t) * a.Hq + h) * D;
-      rf[mt] = a.scale_log2;
-      if constexpr (!Q8B) {
-        const uint8_t* qp = static_cast<const uint8_t*>(a.q) + at * ES + lg * 16;
-#pragma unroll
-        for (int j = 0; j < NF; ++j) qf[mt][0][j] = *reinterpret_cast<const u32x4*>(qp + j * 64);
-      } else {
-        // channels 64 j + 16 lg + 8 f .. of fragment 2 j + f
-        float x[NF][8];
-        float top = 0.0f;
-#pragma unroll
-        for (int f = 0; f < NF; ++f) {
-          const size_t ch = at + (f >> 1) * 64 + lg * 16 + (f & 1) * 8;
-          if constexpr (QBF) {
-            const u32x4 raw = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + ch);
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              x[f][e] = __uint_as_float(e & 1 ? raw[e >> 1] & 0xffff0000u : raw[e >> 1] << 16);
-          } else {
-            const float* qp = static_cast<const float*>(a.q) + ch;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[f][e] = qp[e];
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[f][e]));
+  for (int i = 0; i < n; ++i) {
+    if (n > BATCH && i % (BATCH / 2) == 0) {
+      if (i % BATCH == 0) {
+        if (i > 0) {
+          ids = ids1;
+          ksl = ks1;
+          vsl = vs1;
+          if (Q8B) raise_ref(i);
+          if (i + BATCH < n) raw1 = read_table(i + BATCH);
         }
-        top = max_across_groups(top);
-        // the row's largest value to [2^13, 2^14): what falls below fp16's steps of 2^-24
-        // there is below 2^-38 of it
-        int ex = 0;
-        if (top > 0.0f && top < INFINITY) frexpf(top, &ex);
-        rf[mt] = ldexpf(a.scale_log2, ex - 14);
-#pragma unroll
-        for (int f = 0; f < NF; ++f) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[f][e] = ldexpf(x[f][e], 14 - ex);
-#pragma unroll
-          for (int p = 0; p < QP; ++p) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              qf[mt][p][f][e] = p + 1 < QP ? split_f16x2(x[f][2 * e], x[f][2 * e + 1])
-                                           : pack_f16x2(x[f][2 * e], x[f][2 * e + 1]);
-          }
+      } else if (i + BATCH / 2 < n) {
+        ids1 = place(raw1, i + BATCH / 2);
+        if (Q8B) {
+          ks1 = a.ks[ids1.bh];
+          vs1 = a.vs[ids1.bh];
         }
       }
     }
-
-    const int32_t* table = a.tables + static_cast<size_t>(s.row) * a.max_blocks;
-    const int last_tile = w.p1 >> 4;
-    // the lane's K row and V keys within a step
-    const int kk = 4 * NT * (lr >> 2) + (lr & 3), vk = 4 * NT * lg;
-    const int ktile = kk >> 4, vtile = vk >> 4;
-    const size_t kin = static_cast<size_t>(kk & 15) * D * ES + lg * 16;
-    const size_t vrow = static_cast<size_t>(a.bs) * ES;
-    const size_t vin = lr * vrow + (vk & 15) * ES;
-    const size_t tile_bytes = static_cast<size_t>(a.bs) * D * ES;  // a (block, head)
-
-    u32x4 kf[NT * NJ], vf[DT];
-    int ids = 0;              // of the batch: tile lane's (block * Hkv + kvh) * tpb + part of it
-    float ksl = 0, vsl = 0;   // its scales
-    const auto tile_at = [&](int i, int tile) {  // (block, head) and the tile's place in it
-      const int id = __shfl(ids, i * NT + tile);
-      return id;
+    const uint8_t* here = ring + (i % RING) * (FRAGS * 1024) + l * 16;
+    if (SHARED) {
+      // step i has landed for every wave, and all are done with step i - 1, whose place
+      // takes step i + RING - 1
+      barrier_after_chunks<LPW, RING - 2>(min(RING - 2, n - 1 - i));
+      if (i + RING - 1 < n) stage(i + RING - 1, i);
+    }
+    const int k0 = w.step(at + i * KW) * SK;
+    // (a wave whose rows see nothing of a shared step sits it out)
+    if (SHARED && (!active || k0 > p1 || (k0 + SK - 1 <= p0 - a.window && k0 >= a.sinks))) continue;
+    // Fragments are taken NT (of K) and four (of V) at a time, the next ones on their way from
+    // LDS while some are multiplied (the compiler left to itself reads each right before its
+    // products and waits for it), and products that add to one sum are kept apart.
+    const auto k_frag = [&](int j, int t) {
+      const int f = t % NS * NJ + j;
+      return SHARED ? *reinterpret_cast<const u32x4*>(here + (2 * DT * (t / NS) + f) * 1024)
+                    : kf[t / NS][SHARED ? 0 : f];
     };
-    const auto load_k = [&](int i) {
-      const int id = tile_at(i, ktile);
-      const int bh = a.tpb == 1 ? id : id / a.tpb, part = a.tpb == 1 ? 0 : id - bh * a.tpb;
-      const uint8_t* p = a.k + static_cast<size_t>(bh) * tile_bytes +
-                         static_cast<size_t>(part) * 16 * D * ES + kin;
+    const auto v_frag = [&](int g, int x) {
+      const int dt = g % (DT / 4) * 4 + x, p = g / (DT / 4);
+      return SHARED ? *reinterpret_cast<const u32x4*>(here + (2 * DT * p + DT + dt) * 1024)
+                    : vf[p][SHARED ? 0 : dt];
+    };
+    f32x4 sc[MT][NT];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
+    for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
-          kf[t * NJ + j] = *reinterpret_cast<const u32x4*>(p + t * 4 * D * ES + j * 64);
+      for (int t = 0; t < NT; ++t) sc[mt][t] = f32x4{0, 0, 0, 0};
+    }
+    u32x4 kn[NT], vn[4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) kn[t] = k_frag(0, t);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      u32x4 kc[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) kc[t] = kn[t];
+      if (j + 1 < NJ) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) kn[t] = k_frag(j + 1, t);
+      } else {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) vn[x] = v_frag(0, x);
       }
-    };
-    const auto load_v = [&](int i) {
-      const int id = tile_at(i, vtile);
-      const int bh = a.tpb == 1 ? id : id / a.tpb, part = a.tpb == 1 ? 0 : id - bh * a.tpb;
-      const uint8_t* p = a.v + static_cast<size_t>(bh) * tile_bytes +
-                         static_cast<size_t>(part) * 16 * ES + vin;
+      if (SHARED) __builtin_amdgcn_sched_barrier(0);
+      if constexpr (F32) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-        vf[dt] = *reinterpret_cast<const u32x4*>(p + dt * 16 * vrow);
-    };
-
-    for (int i0 = c * a.chunk + kw; i0 < end; i0 += BATCH * KW) {
-      const int steps = min(BATCH, cdiv(end - i0, KW));
-      {
-        // lane: tile l % NT of the batch's step l / NT (past the last: it again)
-        const int st = w.step(i0 + min(l / NT, steps - 1) * KW);
-        const int tile = min(st * NT + l % NT, last_tile);
-        const int lb = a.tpb == 1 ? tile : tile / a.tpb;
-        const int blk = table[lb];  // within the table: start + T <= max_ctx <= its blocks
-        const int bh = (static_cast<unsigned>(blk) < static_cast<unsigned>(a.num_blocks) ? blk : 0) * a.Hkv + kvh;
-        ids = bh * a.tpb + tile - lb * a.tpb;
-        if constexpr (Q8B) {
-          ksl = a.ks[bh];
-          vsl = a.vs[bh];
-          const int k0 = tile * 16;
-          const bool seen = k0 + 15 > w.p0 - a.window || k0 < a.sinks;
-          float top = seen && vsl < INFINITY ? vsl : 0.0f;
+        for (int e = 0; e < 4; ++e) {
 #pragma unroll
-          for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
-          top = max_across_groups(top);
-          if (top > ref) {  // (the same in every lane)
-            int ex;
-            frexpf(top, &ex);
-            const float to = ldexpf(1.0f, min(ex, 127)), f = ref / to;
-            ref = to;
+          for (int t = 0; t < NT; ++t) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
+            for (int mt = 0; mt < MT; ++mt)
+              sc[mt][t] = mfma16x16x4_f32(__uint_as_float(kc[t][e]), __uint_as_float(qf[mt][0][j][e]),
+                                          sc[mt][t]);
+          }
+        }
+      } else if constexpr (Q8B) {
+        u32x4 f[NT][2];
 #pragma unroll
-              for (int dt = 0; dt < DT; ++dt) acc[mt][dt] *= f;
+        for (int t = 0; t < NT; ++t) codes_to_frags<P>(kc[t], f[t]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int q = 0; q < QP; ++q) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt)
+                sc[mt][t] = mfma16x16x32_f16(f[t][e], qf[mt][q][2 * j + e], sc[mt][t]);
             }
           }
         }
-      }
-      load_k(0);
-      load_v(0);
-      for (int i = 0; i < steps; ++i) {
-        const int k0 = w.step(i0 + i * KW) * SK;
-        f32x4 sc[MT][NT];
+      } else {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) sc[mt][t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) {
-            if constexpr (F32) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-                  sc[mt][t] = mfma16x16x4_f32(__uint_as_float(kf[t * NJ + j][e]),
-                                              __uint_as_float(qf[mt][0][j][e]), sc[mt][t]);
-              }
-            } else if constexpr (Q8B) {
-              u32x4 f[2];
-              codes_to_frags<P>(kf[t * NJ + j], f);
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-                  for (int p = 0; p < QP; ++p)
-                    sc[mt][t] = mfma16x16x32_f16(f[e], qf[mt][p][2 * j + e], sc[mt][t]);
-                }
-              }
-            } else {
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt)
-                sc[mt][t] = mfma16x16x32_bf16(kf[t * NJ + j], qf[mt][0][j], sc[mt][t]);
-            }
-          }
+          for (int mt = 0; mt < MT; ++mt) sc[mt][t] = mfma16x16x32_bf16(kc[t], qf[mt][0][j], sc[mt][t]);
         }
-        const bool more = i + 1 < steps;
-        if (more) load_k(i + 1);
-        float ks = 1.0f, vs = 1.0f;
-        if constexpr (Q8B) {
-          ks = __shfl(ksl, i * NT + lg);
-          vs = __shfl(vsl, i * NT + lg) * (0x1p14f / ref);
-        }
-        // seen whole by every row of the wave
-        const bool whole = k0 + SK - 1 <= w.p0 && (k0 > w.p1 - a.window || k0 + SK <= a.sinks);
-        bool dropped = false;
-        if (!whole && P != Pool::kInt8) {
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) dropped |= drop_nonfinite<P>(vf[dt]);
-        }
-        u32x4 pf[MT][PARTS][F32 ? 1 : NT / 2];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          const float f = Q8B ? rf[mt] * ks : rf[mt];
-          float x[4 * NT];
-          float top = kNone;
-#pragma unroll
-          for (int n = 0; n < 4 * NT; ++n) x[n] = sc[mt][n >> 2][n & 3] * f;
-          if (!whole) {
-#pragma unroll
-            for (int n = 0; n < 4 * NT; ++n) {
-              const int key = k0 + 4 * NT * lg + n;
-              const bool sees = key <= qpos[mt] && (key > qpos[mt] - a.window || key < a.sinks);
-              x[n] = sees ? x[n] : -INFINITY;
-            }
-          }
-#pragma unroll
-          for (int n = 0; n < 4 * NT; ++n) top = fmaxf(top, x[n]);
-          top = max_across_groups(top);
-          if (__any(top > m[mt])) {
-            const float to = fmaxf(m[mt], top), al = __builtin_amdgcn_exp2f(m[mt] - to);
-            m[mt] = to;
-            lsum[mt] *= al;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) acc[mt][dt] *= al;
-          }
-          float add = 0.0f;
-#pragma unroll
-          for (int n = 0; n < 4 * NT; ++n) {
-            x[n] = __builtin_amdgcn_exp2f(x[n] - m[mt]);
-            add += x[n];
-            // (0 * s_v of a block whose scale is no number stays 0)
-            if constexpr (Q8B) x[n] = whole || x[n] > 0.0f || x[n] != x[n] ? x[n] * vs : 0.0f;
-          }
-          lsum[mt] += add;
-          if constexpr (F32) {
-#pragma unroll
-            for (int n = 0; n < 4; ++n) pf[mt][0][0][n] = __float_as_uint(x[n]);
-          } else {
-#pragma unroll
-            for (int n = 0; n < 2 * NT; ++n) {
-#pragma unroll
-              for (int p = 0; p < PARTS; ++p) {
-                uint32_t h;
-                if constexpr (Q8B)
-                  h = p + 1 < PARTS ? split_f16x2(x[2 * n], x[2 * n + 1]) : pack_f16x2(x[2 * n], x[2 * n + 1]);
-                else
-                  h = p + 1 < PARTS ? split_bf16x2(x[2 * n], x[2 * n + 1]) : pack_bf16x2(x[2 * n], x[2 * n + 1]);
-                pf[mt][p][n >> 2][n & 3] = h;
-              }
-            }
-          }
-        }
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          if constexpr (F32) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt)
-                acc[mt][dt] = mfma16x16x4_f32(__uint_as_float(vf[dt][e]),
-                                              __uint_as_float(pf[mt][0][0][e]), acc[mt][dt]);
-            }
-          } else if constexpr (Q8B) {
-            u32x4 f[2];
-            codes_to_frags<P>(vf[dt], f);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-                for (int p = 0; p < PARTS; ++p)
-                  acc[mt][dt] = mfma16x16x32_f16(f[e], pf[mt][p][e], acc[mt][dt]);
-              }
-            }
-          } else {
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-              for (int p = 0; p < PARTS; ++p)
-                acc[mt][dt] = mfma16x16x32_bf16(vf[dt], pf[mt][p][0], acc[mt][dt]);
-            }
-          }
-        }
-        if (__any(dropped)) {
-          // rare: the step's keys one by one, their non-finite values to the rows that see them
-#pragma unroll 1
-          for (int n = 0; n < SK; ++n) {
-            const int key = k0 + n;
-            if (key > w.p1) break;
-            const int id = __shfl(ids, i * NT + (n >> 4));
-            const int bh = id / a.tpb, part = id - bh * a.tpb;
-            const uint8_t* p = a.v + static_cast<size_t>(bh) * tile_bytes +
-                               static_cast<size_t>(4 * lg) * vrow + (part * 16 + (n & 15)) * ES;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float v = nonfinite_of<P>(p + (dt * 16 + e) * vrow);
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                  const bool sees = key <= qpos[mt] && (key > qpos[mt] - a.window || key < a.sinks);
-                  acc[mt][dt][e] += sees ? v : 0.0f;
-                }
-              }
-            }
-          }
-        }
-        if (more) load_v(i + 1);
       }
+      if (SHARED) __builtin_amdgcn_sched_barrier(0);
     }
+    if (SHARED) __asm__ volatile("" ::: "memory");  // the first of V stays ahead of the softmax
+    if (!SHARED && i + 1 < n) load_k(i + 1, i);
+    float ks = 1.0f, vs = 1.0f;
+    if constexpr (Q8B) {
+      ks = __shfl(ksl, i % BATCH * NT + lg);
+      vs = __shfl(vsl, i % BATCH * NT + lg) * (0x1p14f / ref);
+    }
+    // seen whole by every row of the wave
+    const bool whole = k0 + SK - 1 <= p0 && (k0 > p1 - a.window || k0 + SK <= a.sinks);
+    u32x4 pf[MT][U][PP][Q8B ? 2 : 1];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      lsum[mt] = sum_across_groups(lsum[mt]);
-      if constexpr (Q8B) {
+      float f = Q8B ? rf[mt] * ks : rf[mt];
+      float top = -INFINITY;
+      if (whole) {
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) acc[mt][dt] *= ref * 0x1p-14f;
+        for (int x = 0; x < 4 * NT; ++x) top = fmaxf(top, sc[mt][x >> 2][x & 3]);
+        top *= f;
+      } else {
+        // the exponents themselves, so that nothing of a masked key or its scale stays
+#pragma unroll
+        for (int x = 0; x < 4 * NT; ++x) {
+          const int key = k0 + x / (4 * NS) * SP + 4 * NS * lg + x % (4 * NS);
+          const bool sees = (key <= qpos[mt]) & ((key > qpos[mt] - a.window) | (key < a.sinks));
+          const float y = sees ? sc[mt][x >> 2][x & 3] * f : -INFINITY;
+          sc[mt][x >> 2][x & 3] = y;
+          top = fmaxf(top, y);
+        }
+        f = 1.0f;
       }
+      top = max_across_groups(top);
+      const bool grow = top > m[mt] + kLag<Q8B>;
+      if (__any(grow)) {
+        const float to = grow ? top : m[mt], al = __builtin_amdgcn_exp2f(m[mt] - to);
+        m[mt] = to;
+        lsum[mt] *= al;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[mt][dt] *= al;
+      }
+      float x[4 * NT];
+      float add = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4 * NT; ++e) {
+        x[e] = __builtin_amdgcn_exp2f(fmaf(sc[mt][e >> 2][e & 3], f, -m[mt]));
+        add += x[e];
+      }
+      lsum[mt] += add;
+      if constexpr (Q8B) {
+        // (0 * s_v of a block whose scale is no number stays 0)
+#pragma unroll
+        for (int e = 0; e < 4 * NT; ++e) x[e] = whole || x[e] != 0.0f ? x[e] * vs : 0.0f;
+      }
+      if constexpr (F32) {
+#pragma unroll
+        for (int e = 0; e < 4 * NT; ++e) pf[mt][e >> 2][0][0][e & 3] = __float_as_uint(x[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 2 * NT; ++e) {
+#pragma unroll
+          for (int p = 0; p < PP; ++p) {
+            uint32_t h;
+            if constexpr (Q8B)
+              h = p + 1 < PP ? split_f16x2(x[2 * e], x[2 * e + 1]) : pack_f16x2(x[2 * e], x[2 * e + 1]);
+            else
+              h = p + 1 < PP ? split_bf16x2(x[2 * e], x[2 * e + 1]) : pack_bf16x2(x[2 * e], x[2 * e + 1]);
+            pf[mt][e / (2 * NS)][p][e % (2 * NS) >> 2][e & 3] = h;
+          }
+        }
+      }
+    }
+    bool dropped = false;
+#pragma unroll
+    for (int g = 0; g < U * DT / 4; ++g) {
+      const int p = g / (DT / 4), d0 = g % (DT / 4) * 4;
+      u32x4 vc[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) vc[x] = vn[x];
+      if (g + 1 < U * DT / 4) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) vn[x] = v_frag(g + 1, x);
+      }
+      if (SHARED) __builtin_amdgcn_sched_barrier(0);
+      if (P != Pool::kInt8 && !whole) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) dropped |= drop_nonfinite<P>(vc[x]);
+      }
+      if constexpr (F32) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+              acc[mt][d0 + x] = mfma16x16x4_f32(__uint_as_float(vc[x][e]),
+                                                __uint_as_float(pf[mt][p][0][0][e]), acc[mt][d0 + x]);
+          }
+        }
+      } else if constexpr (Q8B) {
+        u32x4 f[4][2];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) codes_to_frags<P>(vc[x], f[x]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int q = 0; q < PP; ++q) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt)
+                acc[mt][d0 + x] = mfma16x16x32_f16(f[x][e], pf[mt][p][q][e], acc[mt][d0 + x]);
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < PP; ++q) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+              acc[mt][d0 + x] = mfma16x16x32_bf16(vc[x], pf[mt][p][q][0], acc[mt][d0 + x]);
+          }
+        }
+      }
+      if (SHARED) __builtin_amdgcn_sched_barrier(0);
+    }
+    if (__any(dropped)) {
+      // rare: the step's keys one by one, their non-finite values to the rows that see them
+#pragma unroll 1
+      for (int x = 0; x < SK; ++x) {
+        const int key = k0 + x;
+        if (key > p1) break;
+        const uint32_t off = __shfl(static_cast<int>(ids.v), i % BATCH * NT + (x >> 4));
+        const uint8_t* p = a.v + static_cast<uint64_t>(off) * 16 + 4 * lg * vrow + (x & 15) * ES;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float v = nonfinite_of<P>(p + (dt * 16 + e) * vrow);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              const bool sees = key <= qpos[mt] && (key > qpos[mt] - a.window || key < a.sinks);
+              acc[mt][dt][e] += sees ? v : 0.0f;
+            }
+          }
+        }
+      }
+    }
+    if (!SHARED && i + 1 < n) load_v(i + 1, i);
+  }
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    lsum[mt] = sum_across_groups(lsum[mt]);
+    if constexpr (Q8B) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) acc[mt][dt] *= ref * 0x1p-14f;
     }
   }
 
-  // the key waves of a row wave, in order, into its first
-  if (KW > 1) {
+  if constexpr (!SHARED) {
+    // the waves' states, in order, into the first's
     constexpr int WAVE = MT * (DT * 256 + 32);  // floats a wave leaves
-    float* mine = sm + static_cast<size_t>(rwi * (KW - 1) + kw - 1) * WAVE;
-    if (kw > 0) {
+    float* mine = sm + (wid - 1) * WAVE;
+    if (wid > 0) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         if (lg == 0) {
@@ -566,9 +743,10 @@ __global__ __launch_bounds__(kWinThreads, 2) void window_attn_kernel(WindowArgs 
       }
     }
     __syncthreads();
-    if (kw > 0) return;
-    for (int o = 0; o < KW - 1; ++o) {
-      const float* other = sm + static_cast<size_t>(rwi * (KW - 1) + o) * WAVE;
+    if (wid > 0) return;
+#pragma unroll
+    for (int o = 0; o < 3; ++o) {
+      const float* other = sm + o * WAVE;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         const float mo = other[MT * DT * 256 + mt * 32 + 2 * lr];
@@ -584,77 +762,89 @@ __global__ __launch_bounds__(kWinThreads, 2) void window_attn_kernel(WindowArgs 
       }
     }
   }
-  if (c >= chunks) return;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     const int r = row0 + mt * 16 + lr;
     if (r >= R) continue;
     if (chunks == 1) {
       const int t = div_magic(r, a.G, a.g_magic), h = kvh * a.G + r - t * a.G;
-      const size_t at = ((static_cast<size_t>(b) * a.Tq + t) * a.Hq + h) * D + 4 * lg;
+      const size_t to = ((static_cast<size_t>(b) * a.Tq + t) * a.Hq + h) * D + 4 * lg;
       const float inv = 1.0f / lsum[mt];
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const f32x4 y = acc[mt][dt] * inv;
         if constexpr (QBF)
-          *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + at + dt * 16) =
+          *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + to + dt * 16) =
               u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
         else
-          *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at + dt * 16) = y;
+          *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + to + dt * 16) = y;
       }
     } else {
       const size_t slot =
-          ((static_cast<size_t>(b) * a.Hkv + kvh) * a.splits + c) * a.row_groups * rows + r;
+          ((static_cast<size_t>(b) * a.Hkv + kvh) * a.splits + c) * a.row_groups * ROWS + r;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
         *reinterpret_cast<f32x4*>(a.part_o + slot * D + dt * 16 + 4 * lg) = acc[mt][dt];
-      if (lg == 0) {
-        a.part_ml[slot * 2] = m[mt];
-        a.part_ml[slot * 2 + 1] = lsum[mt];
-      }
+      if (lg == 0) *reinterpret_cast<float2*>(a.part_ml + slot * 2) = float2{m[mt], lsum[mt]};
     }
   }
 }
 
 // Rows whose walk has several chunks: the chunks' states joined in chunk order, a wave
-// per row, lane l channels l, l + 64.
+// per row, D / 64 channels a lane. The first chunks are asked for before the row's walk
+// is known (the workspace holds them whatever it is), the others four at a time.
 template <int SK, int D, bool OUT_BF16>
-__global__ __launch_bounds__(kWinThreads) void window_merge_kernel(WindowArgs a, int wave_rows) {
+__global__ __launch_bounds__(kWinThreads) void window_merge_kernel(WindowArgs a, int unit_rows) {
+  constexpr int N = D / 64, AHEAD = 4;
+  struct alignas(4 * N) Vec { float v[N]; };
   const int l = threadIdx.x & 63;
   const int rmax = a.G * a.Tq;
   const int64_t u = static_cast<int64_t>(blockIdx.x) * (kWinThreads / 64) + (threadIdx.x >> 6);
   if (u >= static_cast<int64_t>(a.B) * a.Hkv * rmax) return;
   const int r = static_cast<int>(u % rmax), bh = static_cast<int>(u / rmax);
   const int b = bh / a.Hkv, kvh = bh - b * a.Hkv;
+  const size_t per = static_cast<size_t>(a.row_groups) * unit_rows;
+  const size_t slot0 = static_cast<size_t>(bh) * a.splits * per + r;
+  float2 ml[AHEAD];
+  Vec po[AHEAD];
+  const auto load = [&](int c0) {
+#pragma unroll
+    for (int x = 0; x < AHEAD; ++x) {
+      const size_t slot = slot0 + min(c0 + x, a.splits - 1) * per;
+      ml[x] = *reinterpret_cast<const float2*>(a.part_ml + slot * 2);
+      po[x] = *reinterpret_cast<const Vec*>(a.part_o + slot * D + l * N);
+    }
+  };
+  load(0);
   const WinSeq s = win_seq(a, b);
   const int R = a.G * s.T;
   if (r >= R) return;
-  const int row0 = r / wave_rows * wave_rows;
-  const Walk w = walk_of<SK>(a, s, row0, min(R, row0 + wave_rows));
+  const int row0 = r / unit_rows * unit_rows;
+  const Walk w = walk_of<SK>(a, s, row0, min(R, row0 + unit_rows));
   const int chunks = cdiv(w.total, a.chunk);
   if (chunks == 1) return;
-  const size_t per = static_cast<size_t>(a.row_groups) * wave_rows * a.rw;
-  const size_t slot0 = static_cast<size_t>(bh) * a.splits * per + r;
-  constexpr int N = D / 64;
-  float m = kNone, sum = 0.0f, o[N];
+  float m = kNone, sum = 0.0f;
+  Vec o{};
+  for (int c0 = 0; c0 < chunks; c0 += AHEAD) {
+    if (c0) load(c0);
 #pragma unroll
-  for (int e = 0; e < N; ++e) o[e] = 0.0f;
-  for (int c = 0; c < chunks; ++c) {
-    const size_t slot = slot0 + c * per;
-    const float mc = a.part_ml[slot * 2], lc = a.part_ml[slot * 2 + 1];
-    const float to = fmaxf(m, mc), al = __builtin_amdgcn_exp2f(m - to), be = __builtin_amdgcn_exp2f(mc - to);
-    m = to;
-    sum = sum * al + lc * be;
+    for (int x = 0; x < AHEAD; ++x) {
+      if (c0 + x >= chunks) break;
+      const float to = fmaxf(m, ml[x].x), al = __builtin_amdgcn_exp2f(m - to),
+                  be = __builtin_amdgcn_exp2f(ml[x].x - to);
+      m = to;
+      sum = sum * al + ml[x].y * be;
 #pragma unroll
-    for (int e = 0; e < N; ++e) o[e] = o[e] * al + a.part_o[slot * D + e * 64 + l] * be;
+      for (int e = 0; e < N; ++e) o.v[e] = o.v[e] * al + po[x].v[e] * be;
+    }
   }
   const int t = div_magic(r, a.G, a.g_magic), h = kvh * a.G + r - t * a.G;
-  const size_t at = ((static_cast<size_t>(b) * a.Tq + t) * a.Hq + h) * D + l;
+  const size_t to = ((static_cast<size_t>(b) * a.Tq + t) * a.Hq + h) * D + l * N;
 #pragma unroll
   for (int e = 0; e < N; ++e) {
-    const float y = o[e] / sum;
-    if constexpr (OUT_BF16) static_cast<uint16_t*>(a.out)[at + e * 64] = f32_to_bf16(y);
-    else static_cast<float*>(a.out)[at + e * 64] = y;
+    const float y = o.v[e] / sum;
+    if constexpr (OUT_BF16) static_cast<uint16_t*>(a.out)[to + e] = f32_to_bf16(y);
+    else static_cast<float*>(a.out)[to + e] = y;
   }
 }
 
@@ -662,77 +852,81 @@ __global__ __launch_bounds__(kWinThreads) void window_merge_kernel(WindowArgs a,
 
 // Workgroups that a launch should have before walks are cut: two per compute unit.
 constexpr int kFill = 512;
-// Steps of a key wave below which a walk is not cut further.
-constexpr int kMinSteps = 2;
+// Workgroups from which on a wave takes two tiles of rows.
+constexpr int kTwoTiles = 48;
 
 struct WindowCfg {
-  int mt, rw, row_groups, chunk, splits;
+  int mt, rows, row_groups, chunk, splits;  // mt 0: up to 16 rows
   size_t ml, bytes;  // offset of part_ml, the workspace's size
 };
 
-// sk: keys of a step
+// Walks are not cut below `least` steps, where a chunk's own start and its part of the
+// join outweigh the steps it takes over (window 1024 of 32 sequences x 5 rows in bf16 at 1 / 2 /
+// 4 / 8 steps 18.9 / 19.0 / 19.4 / 22.8 us, 8-bit 20.4 / 20.4 / 18.4 / 23.9; up to 16 rows, where
+// four waves share them, 4 / 8 / 16 steps of 8 long histories 23.1 / 17.5 / 18.3 us; fp32 pools,
+// bound by their products, 1 / 2 / 4 steps 11.7 / 14.0 / 19.2). Two tiles a wave halve the
+// LDS reads per product and pay where the workgroups fill the chip all the same (bf16, 1 / 2
+// tiles: prompts 291 / 191 us, 32 x 9 rows 25.5 / 23.0, 4 x 33 17.5 / 19.8, 1 x 100 18.4 / 21.4);
+// fp32 queries, bound by products or registers, keep one (prompt of 1025 242 / 275 us).
 static WindowCfg window_cfg(int B, int Tq, int Hq, int Hkv, int D, int max_ctx, int window,
-                            int sinks, int sk) {
+                            int sinks, int elem_bytes, bool f32) {
   WindowCfg c{};
-  const int R = Hq / Hkv * Tq;
-  const int most = D == 64 ? 4 : 2;  // tiles whose state stays in a wave's registers
-  c.mt = R <= 16 ? 1 : R <= 32 ? 2 : most;
-  c.rw = R <= 16 * c.mt ? 1 : R <= 32 * c.mt ? 2 : 4;
-  c.row_groups = cdiv(R, 16 * c.mt * c.rw);
-  const int kw = 4 / c.rw;
-  // the longest walk: the window of a wave's first query to its last
-  const int64_t keys = std::min<int64_t>(
-      max_ctx, static_cast<int64_t>(window) + cdiv(16 * c.mt, Hq / Hkv) + 1);
+  const int R = Hq / Hkv * Tq, sk = step_keys(elem_bytes, D);
+  const bool two = !f32 && R > 64 && static_cast<int64_t>(B) * Hkv * cdiv(R, 128) >= kTwoTiles;
+  c.mt = R <= 16 ? 0 : two ? 2 : 1;
+  c.rows = c.mt ? 64 * c.mt : 16;
+  c.row_groups = cdiv(R, c.rows);
+  // the longest walk: the window of a workgroup's first query to its last
+  const int64_t keys =
+      std::min<int64_t>(max_ctx, static_cast<int64_t>(window) + cdiv(c.rows, Hq / Hkv) + 1);
   int64_t steps = keys / sk + 2;
   if (keys < max_ctx) steps += cdiv(std::min(sinks, max_ctx), sk);
+  const int least = c.mt == 0 ? 8 : elem_bytes == 4 ? 1 : 4;
   const int64_t units = static_cast<int64_t>(B) * Hkv * c.row_groups;
   const int64_t want = std::max<int64_t>(1, kFill / units);
-  int64_t chunk = std::max<int64_t>((steps + want - 1) / want, kMinSteps * kw);
-  chunk = (chunk + kw - 1) / kw * kw;
+  const int64_t chunk = std::max<int64_t>((steps + want - 1) / want, least);
   c.splits = static_cast<int>((steps + chunk - 1) / chunk);
   c.chunk = static_cast<int>(chunk);
   if (c.splits > 1) {
-    const size_t slots = static_cast<size_t>(B) * Hkv * c.splits * c.row_groups * 16 * c.mt * c.rw;
+    const size_t slots = static_cast<size_t>(B) * Hkv * c.splits * c.row_groups * c.rows;
     c.ml = slots * D * sizeof(float);
     c.bytes = c.ml + slots * 2 * sizeof(float);
   }
   return c;
 }
 
-template <Pool P, int PARTS, int D, int MT>
-static int launch_walk(const WindowArgs& a, int64_t grid, hipStream_t st) {
-  const auto kernel = window_attn_kernel<P, PARTS, D, MT>;
-  const int kw = 4 / a.rw;
-  const size_t lds = static_cast<size_t>(a.rw) * (kw - 1) * MT * (D * 16 + 32) * sizeof(float);
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(kWinThreads), lds, st, a);
-  return KVE_OK;
+template <Pool P, int QP, int PP, int D, int MT, bool SHARED>
+static void launch_walk(const WindowArgs& a, hipStream_t st) {
+  const int64_t grid = static_cast<int64_t>(a.B) * a.Hkv * a.splits * a.row_groups;
+  const size_t lds = SHARED ? kRingBytes : 3 * MT * (D * 16 + 32) * sizeof(float);
+  hipLaunchKernelGGL((window_attn_kernel<P, QP, PP, D, MT, SHARED>), dim3(static_cast<unsigned>(grid)),
+                     dim3(kWinThreads), lds, st, a);
 }
 
-template <Pool P, int PARTS, int D>
+template <Pool P, int QP, int PP, int D>
 static int launch_window(const WindowArgs& a, const WindowCfg& c, hipStream_t st) {
-  const int64_t grid = static_cast<int64_t>(a.B) * a.Hkv * c.splits * c.row_groups;
-  int rc = KVE_OK;
-  if (c.mt == 1) rc = launch_walk<P, PARTS, D, 1>(a, grid, st);
-  else if (c.mt == 2) rc = launch_walk<P, PARTS, D, 2>(a, grid, st);
-  else if constexpr (D == 64) rc = launch_walk<P, PARTS, D, 4>(a, grid, st);
-  if (rc) return rc;
+  // bf16 pools: one part of P from two tiles a wave on
+  constexpr int PM = P == Pool::kBf16 ? 1 : PP;
+  constexpr bool kTwo = P != Pool::kF32 && QP == 1;  // bf16 queries
+  if (c.mt == 0) launch_walk<P, QP, PP, D, 1, false>(a, st);
+  else if (c.mt == 1) launch_walk<P, QP, PP, D, 1, true>(a, st);
+  else if constexpr (kTwo) launch_walk<P, QP, PM, D, 2, true>(a, st);
   if (c.splits > 1) {
-    constexpr bool bf = P == Pool::kBf16 || (PoolOf<P>::Q8B && PARTS == 1);
+    constexpr bool bf = P == Pool::kBf16 || (PoolOf<P, D>::Q8B && QP == 1);
     const int64_t rows = static_cast<int64_t>(a.B) * a.Hkv * a.G * a.Tq;
-    hipLaunchKernelGGL((window_merge_kernel<PoolOf<P>::SK, D, bf>),
-                       dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(kWinThreads), 0, st, a,
-                       16 * c.mt);
+    hipLaunchKernelGGL((window_merge_kernel<PoolOf<P, D>::SK, D, bf>),
+                       dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(kWinThreads), 0, st, a, c.rows);
   }
-  return check_launch("paged window attention");
+  return check_launch("kve_paged_window_attn");
 }
 
-template <Pool P, int PARTS>
+template <Pool P, int QP, int PP>
 static int launch_window_d(const WindowArgs& a, const WindowCfg& c, int D, hipStream_t st) {
-  return D == 64 ? launch_window<P, PARTS, 64>(a, c, st) : launch_window<P, PARTS, 128>(a, c, st);
+  return D == 64 ? launch_window<P, QP, PP, 64>(a, c, st) : launch_window<P, QP, PP, 128>(a, c, st);
 }
 
-static int step_keys(int pool_dtype) {
-  return pool_dtype == KVE_DTYPE_F32 ? 16 : pool_dtype == KVE_DTYPE_BF16 ? 32 : 64;
+static int elem_bytes(int pool_dtype) {
+  return pool_dtype == KVE_DTYPE_F32 ? 4 : pool_dtype == KVE_DTYPE_BF16 ? 2 : 1;
 }
 
 static bool window_sizes_ok(int B, int Tq, int Hq, int Hkv, int D, int max_ctx, int window, int sinks) {
@@ -746,11 +940,12 @@ using namespace kve;
 
 extern "C" size_t kve_window_workspace_bytes(int num_seqs, int q_len, int num_q_heads,
                                              int num_kv_heads, int head_dim, int max_ctx,
-                                             int window, int sinks, int pool_dtype) {
+                                             int window, int sinks, int dtype, int pool_dtype) {
   if (!window_sizes_ok(num_seqs, q_len, num_q_heads, num_kv_heads, head_dim, max_ctx, window, sinks))
     return 0;
   return window_cfg(num_seqs, q_len, num_q_heads, num_kv_heads, head_dim, max_ctx,
-                    window > 0 ? window : INT32_MAX, sinks, step_keys(pool_dtype))
+                    window > 0 ? window : INT32_MAX, sinks, elem_bytes(pool_dtype),
+                    dtype == KVE_DTYPE_F32)
       .bytes;
 }
 
@@ -777,7 +972,11 @@ extern "C" int kve_paged_window_attn(const void* q, const void* k_layer, const v
                   static_cast<int64_t>(max_blocks) * block_size >= max_ctx,
               "kve_paged_window_attn: %d blocks of %d do not hold max_ctx %d", max_blocks,
               block_size, max_ctx);
-  KVE_REQUIRE(static_cast<int64_t>(num_blocks) * num_kv_heads * (block_size / 16) < (1ll << 31),
+  // (offsets in units of 16 bytes are 32-bit, and so is a block's number times the heads)
+  KVE_REQUIRE(static_cast<int64_t>(num_blocks) * num_kv_heads < (1ll << 31) &&
+                  static_cast<int64_t>(num_blocks) * num_kv_heads * (block_size / 16) * head_dim *
+                          elem_bytes(pool_dtype) <
+                      (1ll << 32),
               "kve_paged_window_attn: pool of %d blocks too large", num_blocks);
   KVE_REQUIRE(scale > 0.0f && scale < INFINITY, "kve_paged_window_attn: scale %g", scale);
   const bool q8 = pool_dtype == KVE_DTYPE_I8 || pool_dtype == KVE_DTYPE_E4M3;
@@ -789,7 +988,7 @@ extern "C" int kve_paged_window_attn(const void* q, const void* k_layer, const v
               "kve_paged_window_attn: q, pools and out must be 16-byte aligned");
   const int win = window > 0 ? window : INT32_MAX;
   const WindowCfg c = window_cfg(num_seqs, q_len, num_q_heads, num_kv_heads, head_dim, max_ctx, win,
-                                 sinks, step_keys(pool_dtype));
+                                 sinks, elem_bytes(pool_dtype), dtype == KVE_DTYPE_F32);
   KVE_REQUIRE(static_cast<int64_t>(num_seqs) * num_kv_heads * c.splits * c.row_groups < (1ll << 31) &&
                   static_cast<int64_t>(num_seqs) * num_q_heads * q_len < (1ll << 31),
               "kve_paged_window_attn: %d x %d tokens too large for one launch", num_seqs, q_len);
@@ -825,7 +1024,6 @@ extern "C" int kve_paged_window_attn(const void* q, const void* k_layer, const v
   a.max_ctx = max_ctx;
   a.window = win;
   a.sinks = sinks;
-  a.rw = c.rw;
   a.row_groups = c.row_groups;
   a.chunk = c.chunk;
   a.splits = c.splits;
@@ -833,13 +1031,13 @@ extern "C" int kve_paged_window_attn(const void* q, const void* k_layer, const v
   a.g_magic = static_cast<uint32_t>(((1ull << 32) + a.G - 1) / a.G);
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (pool_dtype) {
-    case KVE_DTYPE_BF16: return launch_window_d<Pool::kBf16, 2>(a, c, head_dim, st);
-    case KVE_DTYPE_F32: return launch_window_d<Pool::kF32, 1>(a, c, head_dim, st);
+    case KVE_DTYPE_BF16: return launch_window_d<Pool::kBf16, 1, 2>(a, c, head_dim, st);
+    case KVE_DTYPE_F32: return launch_window_d<Pool::kF32, 1, 1>(a, c, head_dim, st);
     case KVE_DTYPE_I8:
-      return dtype == KVE_DTYPE_BF16 ? launch_window_d<Pool::kInt8, 1>(a, c, head_dim, st)
-                                     : launch_window_d<Pool::kInt8, 2>(a, c, head_dim, st);
+      return dtype == KVE_DTYPE_BF16 ? launch_window_d<Pool::kInt8, 1, 1>(a, c, head_dim, st)
+                                     : launch_window_d<Pool::kInt8, 2, 2>(a, c, head_dim, st);
     default:
-      return dtype == KVE_DTYPE_BF16 ? launch_window_d<Pool::kE4m3, 1>(a, c, head_dim, st)
-                                     : launch_window_d<Pool::kE4m3, 2>(a, c, head_dim, st);
+      return dtype == KVE_DTYPE_BF16 ? launch_window_d<Pool::kE4m3, 1, 1>(a, c, head_dim, st)
+                                     : launch_window_d<Pool::kE4m3, 2, 2>(a, c, head_dim, st);
   }
 }

@@ -1192,7 +1192,7 @@ def _window_attn(q, k_layer, v_layer, k_scale, v_scale, block_tables, start_pos,
     lib = _lib.lib()
     # (a window of 2^30 tokens sees what none does)
     window, sinks = min(window, 1 << 30), min(sinks, 1 << 30)
-    nbytes = lib.kve_window_workspace_bytes(B, T, Hq, Hkv, D, max_ctx, window, sinks, pool)
+    nbytes = lib.kve_window_workspace_bytes(B, T, Hq, Hkv, D, max_ctx, window, sinks, code, pool)
     # the call's own, so that captured graphs share none
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _call(lib.kve_paged_window_attn, "kve_paged_window_attn", dev, q.data_ptr(), k_layer.data_ptr(),

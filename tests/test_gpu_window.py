@@ -7,7 +7,8 @@ inputs:
   fp16 of 11 bits), and is rounded a few times more on its way into the exponent (8
   roundings of values up to max|score|): =: a. A weight is then off by a relative 2 a
   (itself and the sum that divides it), exp2 and the sums over L keys add 2^-21 + 2 L 2^-24;
-* a weight keeps 16 bits over a bf16 pool (2^-16), and over 8-bit ones fp16's 11 (2^-11, bf16
+* a weight keeps 16 bits over a bf16 pool (2^-16; 8, 2^-8, in passes of more than 64 rows a
+  kv head), and over 8-bit ones fp16's 11 (2^-11, bf16
   queries) or 22 (2^-22); in units of the largest scale that a walk has seen (less than
   twice it), 2^14 of them, it has steps of 2^-24 at the least: 2^-38 of that scale, over L keys,
   times a code;
@@ -100,7 +101,7 @@ class Case:
         if e8:
             rel += 2.0 ** -11 if self.dtype == "bf16" else 2.0 ** -22
         elif self.dtype == "bf16":
-            rel += 2.0 ** -16
+            rel += 2.0 ** -16 if self.T * G <= 64 else 2.0 ** -8
         half = 2.0 ** -8 if self.dtype == "bf16" else 2.0 ** -24
         bound = rel * float(V.abs().max()) + half * out.abs() + len(see) * 2.0 ** -38 * unit
         return out, bound * (1 + half)
@@ -158,6 +159,24 @@ def test_q8_without_a_window(starts, T, Hq, Hkv, D, bs, pool, dtype):
     rows = {(b, t, h) for b in range(len(starts)) for t in range(T) for h in range(Hq)
             if t < 3 or t >= T - 3 or t % 17 == 0}
     c.check(c.run(), None, 0, rows=rows)
+
+
+@pytest.mark.parametrize("pool,dtype", POOLS)
+@pytest.mark.parametrize("T,G,bs", [(1, 1, 16), (9, 2, 32)])
+def test_walks_of_many_steps(T, G, bs, pool, dtype):
+    """So many sequences that no walk is cut: 64 with one history (and block table), one of
+    them shorter, over scales that grow along it."""
+    c = Case(20 + T, [5000], T, 8 * G, 8, 64, pool, dtype, bs)
+    if c.ks is not None:
+        for i, n in enumerate(c.tables[0]):
+            c.vs[n] *= 2.0 ** (i * 16 // (5000 // bs))
+    c.starts, c.tables, c.counts = [5000] * 63 + [4990], c.tables * 64, [T] * 64
+    g = torch.Generator().manual_seed(T)
+    c.q = torch.randn(64, T, 8 * G, 64, generator=g).to(c.q.dtype)
+    rows = {(b, t, (b + t) % (8 * G)) for b in (0, 17, 62, 63) for t in (0, T - 1)}
+    c.check(c.run(4900, 33), 4900, 33, rows=rows)
+    if c.ks is not None:
+        c.check(c.run(), None, 0, rows=rows)
 
 
 @pytest.mark.parametrize("pool,dtype", POOLS)

@@ -34,7 +34,7 @@ def test_attention_refuses(change, text):
 
 
 def test_attention_workspace():
-    need = _lib.lib().kve_window_workspace_bytes(1, 1, 14, 2, 64, 8000, 0, 0, 1)
+    need = _lib.lib().kve_window_workspace_bytes(1, 1, 14, 2, 64, 8000, 0, 0, 1, 1)
     assert need > 0
     long = dict(T=1, max_blocks=500, max_ctx=8000, window=0)
     assert call_attn(**long, wsb=need - 1)[0] == -2
@@ -42,7 +42,7 @@ def test_attention_workspace():
     rc, msg = call_attn(**long, ws=8, wsb=need)
     assert rc == -1 and "16-byte" in msg
     size = _lib.lib().kve_window_workspace_bytes
-    assert size(0, 1, 14, 2, 64, 8000, 0, 0, 1) == size(1, 1, 14, 2, 96, 8000, 0, 0, 1) == 0
+    assert size(0, 1, 14, 2, 64, 8000, 0, 0, 1, 1) == size(1, 1, 14, 2, 96, 8000, 0, 0, 1, 1) == 0
     assert call_attn(B=0)[0] == 0
 
 
