@@ -63,79 +63,215 @@ __global__ __launch_bounds__(kThreads) void logprob_stats_kernel(LogprobArgs a) 
     Piece<E> x = t;
     const int next = i + step;
     if (next < total) load(next);
-    float m = -INFINITY;
+    float f[NV * N], g[NV], m = -INFINITY, lo = INFINITY;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      float g = logit<E>(x.x[v], 0);
 #pragma unroll
-      for (int e = 1; e < N; ++e) g = max_nan(g, logit<E>(x.x[v], e));
-      if (a.top) {
-        g = row_max(g);
-        if ((l & 15) == 0)
-          a.groups[static_cast<size_t>(i) * kChunkGroups<E> + v * 4 + (l >> 4)] = order_key(g + 0.0f);
-      }
-      m = max_nan(m, g);
+      for (int e = 0; e < N; ++e) f[v * N + e] = logit<E>(x.x[v], e);
+      g[v] = f[v * N];
+#pragma unroll
+      for (int e = 1; e < N; ++e) g[v] = max_nan(g[v], f[v * N + e]);
+#pragma unroll
+      for (int e = 0; e < N; ++e) lo = fminf(lo, f[v * N + e]);
     }
+    if (a.top) {
+      // the 16 lanes' maxima of each vector; lane v of them keeps the v-th, for one store
+#pragma unroll
+      for (int v = 0; v < NV; ++v) g[v] = row_max(g[v]);
+      float mine = g[0];
+#pragma unroll
+      for (int v = 1; v < NV; ++v) mine = (l & 15) == v ? g[v] : mine;
+      if ((l & 15) < NV)
+        a.groups[static_cast<size_t>(i) * kChunkGroups<E> + (l & 15) * 4 + (l >> 4)] = order_key(mine + 0.0f);
+    }
+#pragma unroll
+    for (int v = 0; v < NV; ++v) m = max_nan(m, g[v]);
     m = wave_max(m);
-    // (the difference first: a maximum at the type's lowest value times log2(e) is -inf)
-    const float mc = m == -INFINITY ? 0.0f : m;
     float s = 0.0f, w = 0.0f;
+    if (__all(lo > -1e30f) && fabsf(m) < 1000.0f) {
+      // y = x log2(e) - k in one rounding, k = m log2(e) rounded; what that lost, d, is made
+      // good on the sums
+      const float k = m * kLog2e, d = fmaf(m, kLog2e, -k);
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      x.hide(v);
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float y = max_nan((logit<E>(x.x[v], e) - mc) * kLog2e, -1000.0f);
+      for (int e = 0; e < NV * N; ++e) {
+        const float y = fmaf(f[e], kLog2e, -k);
         const float p = __builtin_amdgcn_exp2f(y);
         s += p;
         w = fmaf(y, p, w);
       }
+      s = wave_sum(s);
+      w = wave_sum(w);
+      const float r = __builtin_amdgcn_exp2f(-d);
+      w = (w - d * s) * r;
+      s *= r;
+    } else {
+      // any values: an id of no mass adds nothing to w; the difference comes first, for a
+      // maximum at the type's lowest value times log2(e) is -inf
+      const float c = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int e = 0; e < NV * N; ++e) {
+        const float y = max_nan((f[e] - c) * kLog2e, -1000.0f);
+        const float p = __builtin_amdgcn_exp2f(y);
+        s += p;
+        w = fmaf(y, p, w);
+      }
+      s = wave_sum(s);
+      w = wave_sum(w);
     }
-    s = wave_sum(s);
-    w = wave_sum(w);
     if (l == 0) a.stats[i] = float4{m, s, w, 0.0f};
     if (next >= total) return;
     i = next;
   }
 }
 
-// The largest key of the workgroup below `under`, keys held by the threads; every
-// thread gets it. sm: 2 * kWaves, halves used in turn so that one barrier is enough.
-__device__ __forceinline__ uint64_t block_max(uint64_t v, uint64_t* sm, int tid) {
+// Sums of two doubles over a wave, by moves inside the vector unit.
+__device__ __forceinline__ double dpp_mov64(double v, int step) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  uint32_t lo = static_cast<uint32_t>(u), hi = static_cast<uint32_t>(u >> 32);
+  const auto mov = [&](uint32_t x) {
+    const int y = static_cast<int>(x);
+    return static_cast<uint32_t>(
+        step == 0   ? __builtin_amdgcn_mov_dpp(y, 0xB1, 0xf, 0xf, false)
+        : step == 1 ? __builtin_amdgcn_mov_dpp(y, 0x4E, 0xf, 0xf, false)
+        : step == 2 ? __builtin_amdgcn_mov_dpp(y, 0x141, 0xf, 0xf, false)
+                    : __builtin_amdgcn_mov_dpp(y, 0x140, 0xf, 0xf, false));
+  };
+  lo = mov(lo);
+  hi = mov(hi);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ void wave_sums(double& a, double& b) {
 #pragma unroll
-  for (int o = 1; o < 16; o <<= 1) v = umax64(v, __shfl_xor(v, o));
-  v = max_across_groups_u64(v);
-  if ((tid & 63) == 0) sm[tid >> 6] = v;
-  __syncthreads();
-  v = sm[0];
-#pragma unroll
-  for (int q = 1; q < kWaves; ++q) v = umax64(v, sm[q]);
-  return v;
+  for (int s = 0; s < 4; ++s) {
+    a += dpp_mov64(a, s);
+    b += dpp_mov64(b, s);
+  }
+  a += __shfl_xor(a, 16);
+  b += __shfl_xor(b, 16);
+  a += __shfl_xor(a, 32);
+  b += __shfl_xor(b, 32);
 }
 
-__device__ __forceinline__ double block_sum(double v, double* sm, int tid) {
-  v = wave_sum64(v);
-  if ((tid & 63) == 0) sm[tid >> 6] = v;
-  __syncthreads();
-  double t = 0.0;
+// A key ranks a value by itself, then by its place: the later the smaller.
+__device__ __forceinline__ uint64_t rank_key(uint32_t order, int place) {
+  return static_cast<uint64_t>(order) << 32 | ~static_cast<uint32_t>(place);
+}
+__device__ __forceinline__ int place_of(uint64_t key) { return static_cast<int>(~static_cast<uint32_t>(key)); }
+
+// The n largest of `count` keys by a workgroup: found(i, key) for i = 0 .. n - 1 (n <= kMaxTop
+// of them are not 0, which stands for none). Four threads' keys are a set, 64 sets; the n-th
+// largest of the sets' maxima is no larger than the n-th largest key, so only what reaches
+// it (n and a few more where the keys lie at random) is listed and ranked by counting. Where
+// the list does not hold that, the largest is taken n times. key(i): key i.
+constexpr int kList = 1024;
+struct Select {
+  uint64_t sets[64], list[kList];
+  uint64_t least;
+  int listed;
+};
+
+constexpr int KEEP = 16;  // keys a thread holds on to: 4096 in all
+
+template <typename K>
+__device__ __forceinline__ void hold_keys(uint64_t (&held)[KEEP], int count, int tid, K key) {
 #pragma unroll
-  for (int q = 0; q < kWaves; ++q) t += sm[q];
+  for (int e = 0; e < KEEP; ++e) {
+    const int i = tid + e * kThreads;
+    held[e] = i < count ? key(i) : 0;
+  }
+}
+
+// held: hold_keys of them
+template <typename K, typename F>
+__device__ __forceinline__ void select_largest(Select& sm, const uint64_t (&held)[KEEP], int n,
+                                               int count, int tid, K key, F found) {
+  uint64_t set = 0;
+#pragma unroll
+  for (int e = 0; e < KEEP; ++e) set = umax64(set, held[e]);
+  for (int i = tid + KEEP * kThreads; i < count; i += kThreads) set = umax64(set, key(i));
+  set = umax64(set, __shfl_xor(set, 1));
+  set = umax64(set, __shfl_xor(set, 2));
+  if ((tid & 3) == 0) sm.sets[tid >> 2] = set;
+  if (tid == 0) {
+    sm.listed = 0;
+    sm.least = 1;  // fewer than n sets hold anything: every key reaches it
+  }
   __syncthreads();
-  return t;
+  if (tid < 64) {
+    const uint64_t mine = sm.sets[tid];
+    int above = 0;
+#pragma unroll 16
+    for (int q = 0; q < 64; ++q) above += sm.sets[q] > mine;
+    if (above == n - 1 && mine) sm.least = mine;
+  }
+  __syncthreads();
+  const uint64_t least = sm.least;
+  const auto list = [&](uint64_t k) {
+    if (k >= least) {
+      const int at = atomicAdd(&sm.listed, 1);
+      if (at < kList) sm.list[at] = k;
+    }
+  };
+#pragma unroll
+  for (int e = 0; e < KEEP; ++e) list(held[e]);
+  for (int i = tid + KEEP * kThreads; i < count; i += kThreads) list(key(i));
+  __syncthreads();
+  const int listed = sm.listed;
+  if (listed <= kList) {
+    for (int x = tid; x < listed; x += kThreads) {
+      const uint64_t mine = sm.list[x];
+      int above = 0;
+#pragma unroll 8
+      for (int q = 0; q < listed; ++q) above += sm.list[q] > mine;
+      if (above < n) found(above, mine);
+    }
+  } else {
+    uint64_t under = ~0ull;
+    for (int x = 0; x < n; ++x) {
+      uint64_t best = 0;
+      for (int i = tid; i < count; i += kThreads) {
+        const uint64_t k = key(i);
+        if (k < under) best = umax64(best, k);
+      }
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) best = umax64(best, __shfl_xor(best, o));
+      best = max_across_groups_u64(best);
+      __syncthreads();
+      if ((tid & 63) == 0) sm.sets[tid >> 6] = best;
+      __syncthreads();
+      under = sm.sets[0];
+#pragma unroll
+      for (int q = 1; q < kWaves; ++q) under = umax64(under, sm.sets[q]);
+      if (tid == 0) found(x, under);
+    }
+  }
+  __syncthreads();
 }
 
 template <typename E>
 __global__ __launch_bounds__(kThreads) void logprob_finish_kernel(LogprobArgs a) {
   constexpr double kLn2 = 0.69314718055994530942;
-  __shared__ double sm_d[kWaves];
+  __shared__ double sm_d[2 * kWaves];
   __shared__ float sm_m[kWaves];
-  __shared__ uint64_t sm_k[2 * kWaves];
   __shared__ int sm_groups[kMaxTop];
+  __shared__ Select sm_select;
   const int r = blockIdx.x, tid = threadIdx.x;
   const E* row = static_cast<const E*>(a.logits) + r * a.stride;
   const float4* st = a.stats + static_cast<size_t>(r) * a.chunks;
-  float M = -INFINITY;
-  for (int c = tid; c < a.chunks; c += kThreads) M = max_nan(M, st[c].x);
+  const int t = a.tokens[r];
+  const bool inside = t >= 0 && t < a.V;
+  const float given = to_f32(row[inside ? t : 0]);
+  // the groups' keys, asked for with the statistics
+  const int G = cdiv(a.V, kGroup<E>);
+  const uint32_t* gk = a.groups + static_cast<size_t>(r) * a.chunks * kChunkGroups<E>;
+  const auto group_key = [&](int g) { return rank_key(gk[g], g); };
+  uint64_t held[KEEP];
+  hold_keys(held, a.top ? G : 0, tid, group_key);
+  // every thread's first chunk stays in registers: 256 are a vocabulary of 524288
+  const float4 none = {-INFINITY, 0.0f, 0.0f, 0.0f};
+  const float4 own = tid < a.chunks ? st[tid] : none;
+  float M = own.x;
+  for (int c = tid + kThreads; c < a.chunks; c += kThreads) M = max_nan(M, st[c].x);
   M = wave_max(M);
   if ((tid & 63) == 0) sm_m[tid >> 6] = M;
   __syncthreads();
@@ -143,58 +279,52 @@ __global__ __launch_bounds__(kThreads) void logprob_finish_kernel(LogprobArgs a)
 #pragma unroll
   for (int q = 1; q < kWaves; ++q) M = max_nan(M, sm_m[q]);
   double S = 0.0, T = 0.0;
-  for (int c = tid; c < a.chunks; c += kThreads) {
-    const float4 p = st[c];
-    if (p.x == -INFINITY) continue;  // no mass
+  const auto join = [&](const float4& p) {
+    if (p.x == -INFINITY) return;  // no mass
     const double d = (static_cast<double>(p.x) - M) * static_cast<double>(kLog2e);
-    const double f = exp2(d);
-    S += f * p.y;
-    if (f > 0.0) T += f * (p.z + d * p.y);
+    const float f = __builtin_amdgcn_exp2f(static_cast<float>(d));
+    S += static_cast<double>(f) * p.y;
+    if (f != 0.0f) T += f * (p.z + d * p.y);
+  };
+  join(own);
+  for (int c = tid + kThreads; c < a.chunks; c += kThreads) join(st[c]);
+  wave_sums(S, T);
+  if ((tid & 63) == 0) {
+    sm_d[tid >> 6] = S;
+    sm_d[kWaves + (tid >> 6)] = T;
   }
-  S = block_sum(S, sm_d, tid);
-  T = block_sum(T, sm_d, tid);
+  __syncthreads();
+  S = T = 0.0;
+#pragma unroll
+  for (int q = 0; q < kWaves; ++q) {
+    S += sm_d[q];
+    T += sm_d[kWaves + q];
+  }
   const double logS = log(S);  // a row of no mass: -inf, and NaN below
   // (M off first: beside a maximum of 3e38 log S would be lost)
-  const auto logprob = [&](E x) {
-    return static_cast<float>(static_cast<double>(to_f32(x)) - M - logS);
+  const auto logprob = [&](float x) {
+    return static_cast<float>(static_cast<double>(x) - M - logS);
   };
   if (tid == 0) {
-    const int t = a.tokens[r];
-    a.logprobs[r] = t >= 0 && t < a.V ? logprob(row[t]) : NAN;
+    a.logprobs[r] = inside ? logprob(given) : NAN;
     a.entropy[r] = static_cast<float>(logS - kLn2 * T / S);
   }
   if (!a.top) return;
-  // the groups of the likeliest ids
-  const int G = cdiv(a.V, kGroup<E>), ng = min(a.top, G);
-  const uint32_t* gk = a.groups + static_cast<size_t>(r) * a.chunks * kChunkGroups<E>;
-  uint64_t under = ~0ull;
-  for (int n = 0; n < ng; ++n) {
-    uint64_t best = 0;
-    for (int g = tid; g < G; g += kThreads) {
-      const uint64_t k = static_cast<uint64_t>(gk[g]) << 32 | ~static_cast<uint32_t>(g);
-      if (k < under) best = umax64(best, k);
-    }
-    under = block_max(best, sm_k + (n & 1) * kWaves, tid);
-    if (tid == 0) sm_groups[n] = static_cast<int>(~static_cast<uint32_t>(under));
-  }
-  __syncthreads();
-  under = ~0ull;
-  for (int n = 0; n < a.top; ++n) {
-    uint64_t best = 0;
-    for (int c = tid; c < ng * kGroup<E>; c += kThreads) {
-      const int id = sm_groups[c / kGroup<E>] * kGroup<E> + c % kGroup<E>;
-      if (id >= a.V) continue;
-      const uint64_t k = static_cast<uint64_t>(order_key(to_f32(row[id]) + 0.0f)) << 32 |
-                         ~static_cast<uint32_t>(id);
-      if (k < under) best = umax64(best, k);
-    }
-    under = block_max(best, sm_k + (n & 1) * kWaves, tid);
-    if (tid == 0) {
-      const int id = static_cast<int>(~static_cast<uint32_t>(under));
-      a.top_ids[static_cast<size_t>(r) * a.top + n] = id;
-      a.top_logprobs[static_cast<size_t>(r) * a.top + n] = logprob(row[id]);
-    }
-  }
+  // the groups of the likeliest ids, then the ids
+  const int groups = min(a.top, G);
+  select_largest(sm_select, held, groups, G, tid, group_key,
+                 [&](int n, uint64_t key) { sm_groups[n] = place_of(key); });
+  const auto id_key = [&](int i) -> uint64_t {
+    const int id = sm_groups[i / kGroup<E>] * kGroup<E> + i % kGroup<E>;
+    return id < a.V ? rank_key(order_key(to_f32(row[id]) + 0.0f), id) : 0;
+  };
+  hold_keys(held, groups * kGroup<E>, tid, id_key);
+  select_largest(sm_select, held, a.top, groups * kGroup<E>, tid, id_key, [&](int n, uint64_t key) {
+    const size_t at = static_cast<size_t>(r) * a.top + n;
+    a.top_ids[at] = place_of(key);
+    // the logit, out of the order it was ranked by
+    a.top_logprobs[at] = logprob(unorder_key(static_cast<uint32_t>(key >> 32)));
+  });
 }
 
 // Workgroups of the stats launch: 8 per compute unit.
@@ -217,8 +347,9 @@ static LogprobCfg logprob_cfg(int rows, int V, int top, int dtype) {
 
 template <typename E>
 static void launch_logprobs(const LogprobArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL(logprob_stats_kernel<E>, dim3(std::min(kStatGrid, cdiv(a.rows * a.chunks, kWaves))),
-                     dim3(kThreads), 0, st, a);
+  // every wave the same number of chunks
+  const int total = a.rows * a.chunks, each = cdiv(total, kStatGrid * kWaves);
+  hipLaunchKernelGGL(logprob_stats_kernel<E>, dim3(cdiv(total, each * kWaves)), dim3(kThreads), 0, st, a);
   hipLaunchKernelGGL(logprob_finish_kernel<E>, dim3(a.rows), dim3(kThreads), 0, st, a);
 }
 

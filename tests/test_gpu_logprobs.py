@@ -128,6 +128,24 @@ def test_rows_without_a_distribution_and_ids_outside(dtype):
     check(x[3:], torch.tensor([5, 6, 7], dtype=torch.int32), 4)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [151936, 700001])
+def test_likely_ids_that_lie_together(dtype, V):
+    """The likeliest ids spread evenly, in one place, ascending and descending, and in places
+    that a selection by parts would find in one part: every 4th, 64th, 1024th, 32768th id."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(9, V, generator=g)
+    i = torch.arange(V)
+    x[0, V // 2:V // 2 + 100] += 10
+    x[1] = i / V * 30
+    x[2] = -i / V * 30
+    for r, step in enumerate((4, 64, 1024, 32768), start=3):
+        x[r, step - 1::step] += 8
+    x[7] += 5.0 * (i // 128 % 1024 < 500)
+    x[8] += 5.0 * (i // 64 % 256 < 128)
+    check(x.to(dtype), torch.arange(9, dtype=torch.int32), 32)
+
+
 def test_strided_and_unaligned_rows():
     g = torch.Generator().manual_seed(2)
     for dtype in (torch.bfloat16, torch.float32):
