@@ -124,32 +124,27 @@ __global__ __launch_bounds__(kThreads) void logprob_stats_kernel(LogprobArgs a) 
   }
 }
 
-// Sums of two doubles over a wave, by moves inside the vector unit.
-__device__ __forceinline__ double dpp_mov64(double v, int step) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, v);
-  uint32_t lo = static_cast<uint32_t>(u), hi = static_cast<uint32_t>(u >> 32);
-  const auto mov = [&](uint32_t x) {
-    const int y = static_cast<int>(x);
-    return static_cast<uint32_t>(
-        step == 0   ? __builtin_amdgcn_mov_dpp(y, 0xB1, 0xf, 0xf, false)
-        : step == 1 ? __builtin_amdgcn_mov_dpp(y, 0x4E, 0xf, 0xf, false)
-        : step == 2 ? __builtin_amdgcn_mov_dpp(y, 0x141, 0xf, 0xf, false)
-                    : __builtin_amdgcn_mov_dpp(y, 0x140, 0xf, 0xf, false));
-  };
-  lo = mov(lo);
-  hi = mov(hi);
-  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+// Reductions of 64-bit values over the 16 lanes of a row, by moves inside the vector unit
+// (swap neighbours, swap pairs, mirror halves, mirror the row).
+template <int CTRL>
+__device__ __forceinline__ uint64_t dpp_mov64(uint64_t u) {
+  const uint32_t lo = static_cast<uint32_t>(u), hi = static_cast<uint32_t>(u >> 32);
+  return static_cast<uint64_t>(static_cast<uint32_t>(
+             __builtin_amdgcn_mov_dpp(static_cast<int>(hi), CTRL, 0xf, 0xf, false))) << 32 |
+         static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(lo), CTRL, 0xf, 0xf, false));
 }
-__device__ __forceinline__ void wave_sums(double& a, double& b) {
-#pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    a += dpp_mov64(a, s);
-    b += dpp_mov64(b, s);
-  }
-  a += __shfl_xor(a, 16);
-  b += __shfl_xor(b, 16);
-  a += __shfl_xor(a, 32);
-  b += __shfl_xor(b, 32);
+template <typename Op>
+__device__ __forceinline__ uint64_t row_reduce64(uint64_t v, Op op) {
+  v = op(v, dpp_mov64<0xB1>(v));
+  v = op(v, dpp_mov64<0x4E>(v));
+  v = op(v, dpp_mov64<0x141>(v));
+  return op(v, dpp_mov64<0x140>(v));
+}
+__device__ __forceinline__ double row_add(double v) {
+  return __builtin_bit_cast(
+      double, row_reduce64(__builtin_bit_cast(uint64_t, v), [](uint64_t a, uint64_t b) {
+        return __builtin_bit_cast(uint64_t, __builtin_bit_cast(double, a) + __builtin_bit_cast(double, b));
+      }));
 }
 
 // A key ranks a value by itself, then by its place: the later the smaller.
@@ -159,39 +154,49 @@ __device__ __forceinline__ uint64_t rank_key(uint32_t order, int place) {
 __device__ __forceinline__ int place_of(uint64_t key) { return static_cast<int>(~static_cast<uint32_t>(key)); }
 
 // The n largest of `count` keys by a workgroup: found(i, key) for i = 0 .. n - 1 (n <= kMaxTop
-// of them are not 0, which stands for none). Four threads' keys are a set, 64 sets; the n-th
+// of them are not 0, which stands for none). 16 threads' keys are a set, 64 sets; the n-th
 // largest of the sets' maxima is no larger than the n-th largest key, so only what reaches
 // it (n and a few more where the keys lie at random) is listed and ranked by counting. Where
 // the list does not hold that, the largest is taken n times. key(i): key i.
+constexpr int kFinishThreads = 1024;
 constexpr int kList = 1024;
 struct Select {
-  uint64_t sets[64], list[kList];
+  alignas(16) uint64_t sets[64], list[kList];
   uint64_t least;
   int listed;
 };
 
-constexpr int KEEP = 16;  // keys a thread holds on to: 4096 in all
-
-template <typename K>
-__device__ __forceinline__ void hold_keys(uint64_t (&held)[KEEP], int count, int tid, K key) {
-#pragma unroll
-  for (int e = 0; e < KEEP; ++e) {
-    const int i = tid + e * kThreads;
-    held[e] = i < count ? key(i) : 0;
+// keys of sm[0, count) above `mine`, count even
+__device__ __forceinline__ int keys_above(const uint64_t* sm, int count, uint64_t mine) {
+  int above = 0;
+#pragma unroll 16
+  for (int q = 0; q < count; q += 2) {
+    const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(sm + q);
+    above += (k.x > mine) + (k.y > mine);
   }
+  return above;
 }
 
-// held: hold_keys of them
 template <typename K, typename F>
-__device__ __forceinline__ void select_largest(Select& sm, const uint64_t (&held)[KEEP], int n,
-                                               int count, int tid, K key, F found) {
-  uint64_t set = 0;
+__device__ __forceinline__ void select_largest(Select& sm, int n, int count, int tid, K key, F found) {
+  constexpr int KEEP = 4;  // keys a thread holds on to: 4096 in all
+  uint64_t held[KEEP], set = 0;
 #pragma unroll
-  for (int e = 0; e < KEEP; ++e) set = umax64(set, held[e]);
-  for (int i = tid + KEEP * kThreads; i < count; i += kThreads) set = umax64(set, key(i));
-  set = umax64(set, __shfl_xor(set, 1));
-  set = umax64(set, __shfl_xor(set, 2));
-  if ((tid & 3) == 0) sm.sets[tid >> 2] = set;
+  for (int e = 0; e < KEEP; ++e) held[e] = key(min(tid + e * kFinishThreads, count - 1));
+#pragma unroll
+  for (int e = 0; e < KEEP; ++e) {
+    held[e] = tid + e * kFinishThreads < count ? held[e] : 0;
+    set = umax64(set, held[e]);
+  }
+  const auto each = [&](auto put) {
+#pragma unroll
+    for (int e = 0; e < KEEP; ++e) put(held[e]);
+    for (int i0 = KEEP * kFinishThreads; i0 < count; i0 += kFinishThreads)
+      put(i0 + tid < count ? key(i0 + tid) : 0);
+  };
+  if (count > KEEP * kFinishThreads) each([&](uint64_t k) { set = umax64(set, k); });
+  set = row_reduce64(set, umax64);
+  if ((tid & 15) == 0) sm.sets[tid >> 4] = set;
   if (tid == 0) {
     sm.listed = 0;
     sm.least = 1;  // fewer than n sets hold anything: every key reaches it
@@ -199,49 +204,49 @@ __device__ __forceinline__ void select_largest(Select& sm, const uint64_t (&held
   __syncthreads();
   if (tid < 64) {
     const uint64_t mine = sm.sets[tid];
-    int above = 0;
-#pragma unroll 16
-    for (int q = 0; q < 64; ++q) above += sm.sets[q] > mine;
-    if (above == n - 1 && mine) sm.least = mine;
+    if (keys_above(sm.sets, 64, mine) == n - 1 && mine) sm.least = mine;
   }
   __syncthreads();
   const uint64_t least = sm.least;
-  const auto list = [&](uint64_t k) {
-    if (k >= least) {
-      const int at = atomicAdd(&sm.listed, 1);
-      if (at < kList) sm.list[at] = k;
-    }
-  };
-#pragma unroll
-  for (int e = 0; e < KEEP; ++e) list(held[e]);
-  for (int i = tid + KEEP * kThreads; i < count; i += kThreads) list(key(i));
+  // a wave counts what it will list, takes that many places and fills them
+  int places = 0;
+  each([&](uint64_t k) { places += __popcll(__ballot(k >= least)); });
+  if (places) {
+    int at = 0;
+    if ((tid & 63) == 0) at = atomicAdd(&sm.listed, places);
+    at = __builtin_amdgcn_readfirstlane(at);
+    each([&](uint64_t k) {
+      const uint64_t here = __ballot(k >= least);
+      if (!here) return;
+      const int x = at + __popcll(here & ((1ull << (tid & 63)) - 1));
+      if (k >= least && x < kList) sm.list[x] = k;
+      at += __popcll(here);
+    });
+  }
   __syncthreads();
   const int listed = sm.listed;
   if (listed <= kList) {
-    for (int x = tid; x < listed; x += kThreads) {
-      const uint64_t mine = sm.list[x];
-      int above = 0;
-#pragma unroll 8
-      for (int q = 0; q < listed; ++q) above += sm.list[q] > mine;
+    if (tid == 0 && listed < kList) sm.list[listed] = 0;
+    __syncthreads();
+    if (tid < listed) {
+      const uint64_t mine = sm.list[tid];
+      const int above = keys_above(sm.list, (listed + 1) & ~1, mine);
       if (above < n) found(above, mine);
     }
   } else {
     uint64_t under = ~0ull;
     for (int x = 0; x < n; ++x) {
       uint64_t best = 0;
-      for (int i = tid; i < count; i += kThreads) {
+      for (int i = tid; i < count; i += kFinishThreads) {
         const uint64_t k = key(i);
         if (k < under) best = umax64(best, k);
       }
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) best = umax64(best, __shfl_xor(best, o));
-      best = max_across_groups_u64(best);
+      best = max_across_groups_u64(row_reduce64(best, umax64));
       __syncthreads();
       if ((tid & 63) == 0) sm.sets[tid >> 6] = best;
       __syncthreads();
       under = sm.sets[0];
-#pragma unroll
-      for (int q = 1; q < kWaves; ++q) under = umax64(under, sm.sets[q]);
+      for (int q = 1; q < kFinishThreads / 64; ++q) under = umax64(under, sm.sets[q]);
       if (tid == 0) found(x, under);
     }
   }
@@ -249,10 +254,11 @@ __device__ __forceinline__ void select_largest(Select& sm, const uint64_t (&held
 }
 
 template <typename E>
-__global__ __launch_bounds__(kThreads) void logprob_finish_kernel(LogprobArgs a) {
+__global__ __launch_bounds__(kFinishThreads) void logprob_finish_kernel(LogprobArgs a) {
   constexpr double kLn2 = 0.69314718055994530942;
-  __shared__ double sm_d[2 * kWaves];
-  __shared__ float sm_m[kWaves];
+  constexpr int kFinishWaves = kFinishThreads / 64;
+  __shared__ double sm_s[kFinishThreads / 16], sm_t[kFinishThreads / 16];
+  __shared__ float sm_m[kFinishWaves];
   __shared__ int sm_groups[kMaxTop];
   __shared__ Select sm_select;
   const int r = blockIdx.x, tid = threadIdx.x;
@@ -261,23 +267,17 @@ __global__ __launch_bounds__(kThreads) void logprob_finish_kernel(LogprobArgs a)
   const int t = a.tokens[r];
   const bool inside = t >= 0 && t < a.V;
   const float given = to_f32(row[inside ? t : 0]);
-  // the groups' keys, asked for with the statistics
-  const int G = cdiv(a.V, kGroup<E>);
-  const uint32_t* gk = a.groups + static_cast<size_t>(r) * a.chunks * kChunkGroups<E>;
-  const auto group_key = [&](int g) { return rank_key(gk[g], g); };
-  uint64_t held[KEEP];
-  hold_keys(held, a.top ? G : 0, tid, group_key);
-  // every thread's first chunk stays in registers: 256 are a vocabulary of 524288
+  // every thread's first chunk stays in registers: 1024 are a vocabulary of 2097152
   const float4 none = {-INFINITY, 0.0f, 0.0f, 0.0f};
   const float4 own = tid < a.chunks ? st[tid] : none;
   float M = own.x;
-  for (int c = tid + kThreads; c < a.chunks; c += kThreads) M = max_nan(M, st[c].x);
+  for (int c = tid + kFinishThreads; c < a.chunks; c += kFinishThreads) M = max_nan(M, st[c].x);
   M = wave_max(M);
   if ((tid & 63) == 0) sm_m[tid >> 6] = M;
   __syncthreads();
   M = sm_m[0];
 #pragma unroll
-  for (int q = 1; q < kWaves; ++q) M = max_nan(M, sm_m[q]);
+  for (int q = 1; q < kFinishWaves; ++q) M = max_nan(M, sm_m[q]);
   double S = 0.0, T = 0.0;
   const auto join = [&](const float4& p) {
     if (p.x == -INFINITY) return;  // no mass
@@ -287,19 +287,17 @@ __global__ __launch_bounds__(kThreads) void logprob_finish_kernel(LogprobArgs a)
     if (f != 0.0f) T += f * (p.z + d * p.y);
   };
   join(own);
-  for (int c = tid + kThreads; c < a.chunks; c += kThreads) join(st[c]);
-  wave_sums(S, T);
-  if ((tid & 63) == 0) {
-    sm_d[tid >> 6] = S;
-    sm_d[kWaves + (tid >> 6)] = T;
+  for (int c = tid + kFinishThreads; c < a.chunks; c += kFinishThreads) join(st[c]);
+  S = row_add(S);
+  T = row_add(T);
+  if ((tid & 15) == 0) {
+    sm_s[tid >> 4] = S;
+    sm_t[tid >> 4] = T;
   }
   __syncthreads();
-  S = T = 0.0;
-#pragma unroll
-  for (int q = 0; q < kWaves; ++q) {
-    S += sm_d[q];
-    T += sm_d[kWaves + q];
-  }
+  // 64 rows' sums, four to a lane of 16
+  S = row_add((sm_s[tid & 15] + sm_s[16 + (tid & 15)]) + (sm_s[32 + (tid & 15)] + sm_s[48 + (tid & 15)]));
+  T = row_add((sm_t[tid & 15] + sm_t[16 + (tid & 15)]) + (sm_t[32 + (tid & 15)] + sm_t[48 + (tid & 15)]));
   const double logS = log(S);  // a row of no mass: -inf, and NaN below
   // (M off first: beside a maximum of 3e38 log S would be lost)
   const auto logprob = [&](float x) {
@@ -310,21 +308,30 @@ __global__ __launch_bounds__(kThreads) void logprob_finish_kernel(LogprobArgs a)
     a.entropy[r] = static_cast<float>(logS - kLn2 * T / S);
   }
   if (!a.top) return;
-  // the groups of the likeliest ids, then the ids
-  const int groups = min(a.top, G);
-  select_largest(sm_select, held, groups, G, tid, group_key,
-                 [&](int n, uint64_t key) { sm_groups[n] = place_of(key); });
-  const auto id_key = [&](int i) -> uint64_t {
-    const int id = sm_groups[i / kGroup<E>] * kGroup<E> + i % kGroup<E>;
-    return id < a.V ? rank_key(order_key(to_f32(row[id]) + 0.0f), id) : 0;
-  };
-  hold_keys(held, groups * kGroup<E>, tid, id_key);
-  select_largest(sm_select, held, a.top, groups * kGroup<E>, tid, id_key, [&](int n, uint64_t key) {
-    const size_t at = static_cast<size_t>(r) * a.top + n;
-    a.top_ids[at] = place_of(key);
-    // the logit, out of the order it was ranked by
-    a.top_logprobs[at] = logprob(unorder_key(static_cast<uint32_t>(key >> 32)));
-  });
+  // the groups of the likeliest ids, then the ids: one code for both
+  const int G = cdiv(a.V, kGroup<E>), groups = min(a.top, G);
+  const uint32_t* gk = a.groups + static_cast<size_t>(r) * a.chunks * kChunkGroups<E>;
+#pragma unroll 1
+  for (int ids = 0; ids < 2; ++ids) {
+    select_largest(
+        sm_select, ids ? a.top : groups, ids ? groups * kGroup<E> : G, tid,
+        [&](int i) -> uint64_t {
+          if (!ids) return rank_key(gk[i], i);
+          const int id = sm_groups[i / kGroup<E>] * kGroup<E> + i % kGroup<E>;
+          const E x = row[min(id, a.V - 1)];
+          return id < a.V ? rank_key(order_key(to_f32(x) + 0.0f), id) : 0;
+        },
+        [&](int n, uint64_t key) {
+          if (!ids) {
+            sm_groups[n] = place_of(key);
+            return;
+          }
+          const size_t at = static_cast<size_t>(r) * a.top + n;
+          a.top_ids[at] = place_of(key);
+          // the logit, out of the order it was ranked by
+          a.top_logprobs[at] = logprob(unorder_key(static_cast<uint32_t>(key >> 32)));
+        });
+  }
 }
 
 // Workgroups of the stats launch: 8 per compute unit.
@@ -350,7 +357,7 @@ static void launch_logprobs(const LogprobArgs& a, hipStream_t st) {
   // every wave the same number of chunks
   const int total = a.rows * a.chunks, each = cdiv(total, kStatGrid * kWaves);
   hipLaunchKernelGGL(logprob_stats_kernel<E>, dim3(cdiv(total, each * kWaves)), dim3(kThreads), 0, st, a);
-  hipLaunchKernelGGL(logprob_finish_kernel<E>, dim3(a.rows), dim3(kThreads), 0, st, a);
+  hipLaunchKernelGGL(logprob_finish_kernel<E>, dim3(a.rows), dim3(kFinishThreads), 0, st, a);
 }
 
 }  // namespace kve
