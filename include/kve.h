@@ -264,7 +264,7 @@ int kve_sample_verify(const void* target, int64_t target_seq_stride, int64_t tar
  * Rows behind the pass's last keep their codes. A sequence's row may stand once in a
  * launch, and no two sequences of it may share a block that they write.
  * k_new, v_new, src_token_stride, dtype: as for kve_kv_write; block_size % 16 == 0,
- * head_dim % 8 == 0 and <= 1024; rows and pools 16-byte aligned.
+ * head_dim 64 or 128; rows and pools 16-byte aligned.
  */
 int kve_kv_write_q8(const void* k_new, const void* v_new, int64_t src_token_stride, void* k_pool,
                     void* v_pool, float* k_scale, float* v_scale, const int32_t* block_tables,

@@ -84,7 +84,7 @@ def same(p, c):
 @pytest.mark.parametrize("starts,T,Hkv,D,bs,counts", [
     ([0], 1, 1, 64, 16, None), ([5, 15, 16, 31], 1, 2, 128, 16, None),
     ([0, 3, 14, 40], 5, 2, 64, 16, [5, 0, 3, 1]), ([7, 100], 33, 2, 128, 32, None),
-    ([1, 47, 48], 50, 1, 64, 48, [50, 49, 2]), ([9], 200, 3, 72, 16, None)])
+    ([1, 47, 48], 50, 1, 64, 48, [50, 49, 2]), ([9], 200, 3, 64, 16, None), ([130], 90, 1, 128, 64, None), ([3, 40], 9, 2, 64, 32, None)])
 def test_write(starts, T, Hkv, D, bs, counts, dtype, pool):
     r, g = random.Random(T), torch.Generator().manual_seed(D + T)
     B = len(starts)

@@ -59,7 +59,7 @@ def call_write(**kw):
     (dict(k=None), "null pointer"), (dict(vs=None), "null pointer"), (dict(start=None), "null pointer"),
     (dict(T=0), "bad sizes"), (dict(B=-1), "bad sizes"), (dict(num_blocks=0), "bad sizes"),
     (dict(bs=8), "block_size"), (dict(bs=0), "block_size"), (dict(D=60), "head_dim"),
-    (dict(D=2048), "head_dim"), (dict(dtype=2), "dtype"), (dict(pool=1), "pool dtype"),
+    (dict(D=256), "head_dim"), (dict(dtype=2), "dtype"), (dict(pool=1), "pool dtype"),
     (dict(stride=120), "stride"), (dict(stride=132), "stride"), (dict(k=8), "aligned"),
     (dict(vp=20), "aligned"), (dict(B=1 << 28, T=1 << 10), "too large"),
 ])
