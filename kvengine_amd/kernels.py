@@ -1115,18 +1115,42 @@ def _q8_code(t: torch.Tensor) -> int:
     return code
 
 
+def _fits(t: torch.Tensor, dtype, shape: tuple, at: int) -> bool:
+    """_check_on's condition for a tensor on GPU `at`. A decode step's calls take less time
+    on the card than its checks would as calls that raise: they are tested together, and
+    looked at one by one (_check_on) only for the message."""
+    return t.dtype is dtype and t.shape == shape and t.get_device() == at and t.is_contiguous()
+
+
 def _check_paged(block_tables, start_pos, seq_rows, q_lens, B: int, dev) -> tuple[int, int]:
     """-> (rows, blocks per row) of the tables."""
+    i32, at = torch.int32, dev.index
     _need(block_tables.dim() == 2 and start_pos.dim() == 1,
           "block_tables [rows, max_blocks], start_pos [rows]")
     num_rows, max_blocks = block_tables.shape
-    _check_on(block_tables, "block_tables", torch.int32, (num_rows, max_blocks), dev)
-    _check_on(start_pos, "start_pos", torch.int32, start_pos.shape, dev)
-    _check_on(seq_rows, "seq_rows", torch.int32, (B,), dev)
-    _check_on(q_lens, "q_lens", torch.int32, (B,), dev)
-    _need(start_pos.numel() >= num_rows, "start_pos needs one entry per table row")
-    _need(seq_rows is not None or num_rows >= B, "too few table rows")
+    n = start_pos.shape
+    if not (_fits(block_tables, i32, (num_rows, max_blocks), at) and _fits(start_pos, i32, n, at)
+            and n[0] >= num_rows
+            and (num_rows >= B if seq_rows is None else _fits(seq_rows, i32, (B,), at))
+            and (q_lens is None or _fits(q_lens, i32, (B,), at))):
+        _check_on(block_tables, "block_tables", i32, (num_rows, max_blocks), dev)
+        _check_on(start_pos, "start_pos", i32, n, dev)
+        _check_on(seq_rows, "seq_rows", i32, (B,), dev)
+        _check_on(q_lens, "q_lens", i32, (B,), dev)
+        _need(n[0] >= num_rows, "start_pos needs one entry per table row")
+        _need(False, "too few table rows")
     return num_rows, max_blocks
+
+
+def _check_pool(k_layer, v_layer, k_scale, v_scale, NB, Hkv, bs, D, dev) -> None:
+    dtype, f32, at = k_layer.dtype, torch.float32, dev.index
+    if not (_fits(k_layer, dtype, (NB, Hkv, bs, D), at) and _fits(v_layer, dtype, (NB, Hkv, D, bs), at)
+            and (k_scale is None or _fits(k_scale, f32, (NB, Hkv), at)
+                 and _fits(v_scale, f32, (NB, Hkv), at))):
+        _check_on(k_layer, "k_layer", dtype, (NB, Hkv, bs, D), dev)
+        _check_on(v_layer, "v_layer", dtype, (NB, Hkv, D, bs), dev)
+        _check_on(k_scale, "k_scale", f32, (NB, Hkv), dev)
+        _check_on(v_scale, "v_scale", f32, (NB, Hkv), dev)
 
 
 def kv_write_q8(k_new: torch.Tensor, v_new: torch.Tensor, k_layer: torch.Tensor,
@@ -1148,10 +1172,7 @@ def kv_write_q8(k_new: torch.Tensor, v_new: torch.Tensor, k_layer: torch.Tensor,
     _need(k_layer.dim() == 4, "k layer must be [NB, Hkv, bs, D]")
     NB, _, bs, _ = k_layer.shape
     pool = _q8_code(k_layer)
-    _check_on(k_layer, "k_layer", k_layer.dtype, (NB, Hkv, bs, D), dev)
-    _check_on(v_layer, "v_layer", k_layer.dtype, (NB, Hkv, D, bs), dev)
-    _check_on(k_scale, "k_scale", torch.float32, (NB, Hkv), dev)
-    _check_on(v_scale, "v_scale", torch.float32, (NB, Hkv), dev)
+    _check_pool(k_layer, v_layer, k_scale, v_scale, NB, Hkv, bs, D, dev)
     num_rows, max_blocks = _check_paged(block_tables, start_pos, seq_rows, q_lens, B, dev)
     code = _dtype_code(k_new)
     if B == 0 or T == 0:
@@ -1166,13 +1187,15 @@ def kv_write_q8(k_new: torch.Tensor, v_new: torch.Tensor, k_layer: torch.Tensor,
           bs, max_blocks, num_rows, NB, code, pool)
 
 
+_WINDOW_WS: dict[tuple, int] = {}  # workspace bytes by sizes
+
+
 def _window_attn(q, k_layer, v_layer, k_scale, v_scale, block_tables, start_pos, max_ctx, window,
                  sinks, seq_rows, q_lens, scale, out, code: int, pool: int):
     dev, dtype = q.device, q.dtype
     B, T, Hq, D = q.shape
     NB, Hkv, bs, _ = k_layer.shape
-    _check_on(k_layer, "k_layer", k_layer.dtype, (NB, Hkv, bs, D), dev)
-    _check_on(v_layer, "v_layer", k_layer.dtype, (NB, Hkv, D, bs), dev)
+    _check_pool(k_layer, v_layer, k_scale, v_scale, NB, Hkv, bs, D, dev)
     if Hkv < 1 or Hq % Hkv:
         raise ValueError(f"{Hq} q heads not a multiple of {Hkv} kv heads")
     num_rows, max_blocks = _check_paged(block_tables, start_pos, seq_rows, q_lens, B, dev)
@@ -1192,7 +1215,12 @@ def _window_attn(q, k_layer, v_layer, k_scale, v_scale, block_tables, start_pos,
     lib = _lib.lib()
     # (a window of 2^30 tokens sees what none does)
     window, sinks = min(window, 1 << 30), min(sinks, 1 << 30)
-    nbytes = lib.kve_window_workspace_bytes(B, T, Hq, Hkv, D, max_ctx, window, sinks, code, pool)
+    key = (B, T, Hq, Hkv, D, max_ctx, window, sinks, code, pool)
+    nbytes = _WINDOW_WS.get(key)
+    if nbytes is None:
+        if len(_WINDOW_WS) >= 4096:  # (max_ctx grows with every step)
+            _WINDOW_WS.clear()
+        nbytes = _WINDOW_WS[key] = lib.kve_window_workspace_bytes(*key)
     # the call's own, so that captured graphs share none
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _call(lib.kve_paged_window_attn, "kve_paged_window_attn", dev, q.data_ptr(), k_layer.data_ptr(),
@@ -1235,10 +1263,8 @@ def paged_q8_attn(q: torch.Tensor, k_layer: torch.Tensor, v_layer: torch.Tensor,
     _need(k_layer.dim() == 4, "k layer must be [NB, Hkv, bs, D]")
     if window is not None and window < 1:
         raise ValueError(f"window {window}, at least 1 (None: no window)")
-    NB, Hkv = k_layer.shape[:2]
     pool = _q8_code(k_layer)
-    _check_on(k_scale, "k_scale", torch.float32, (NB, Hkv), q.device)
-    _check_on(v_scale, "v_scale", torch.float32, (NB, Hkv), q.device)
+    _need(k_scale is not None and v_scale is not None, "an 8-bit pool needs scales")
     return _window_attn(q, k_layer, v_layer, k_scale, v_scale, block_tables, start_pos, max_ctx,
                         window or 0, sinks, seq_rows, q_lens, scale, out, _dtype_code(q), pool)
 
