@@ -11,13 +11,14 @@
 //
 // Work. Rows: the G = Hq / Hkv query heads of a kv head times the new tokens (row r =
 // t G + head). Rows walk the keys they see in steps of 64 (32 in fp32 at head_dim 128): first
-// the steps that hold sinks, then those of the window; what lies between is not read. A workgroup is four waves, in one of two forms:
-//  * up to 16 rows (decoding): one tile of 16 rows, the waves take the walk's steps in turn,
-//    each K/V byte goes into the registers of the one wave that multiplies it, and the four
-//    states are folded through LDS;
-//  * more rows (drafts, prompts): every wave has MT tiles of its own and all walk together;
-//    a step's K/V comes into LDS once, by direct loads into a ring of 64 KB (two workgroups
-//    a CU), RING - 1 steps ahead, and one barrier a step hands it over.
+// the steps that hold sinks, then those of the window; what lies between is not read. A
+// workgroup takes one of two forms:
+//  * up to 16 rows (decoding): eight waves with one tile of 16 rows between them, which take
+//    the walk's steps in turn; each K/V byte goes into the registers of the one wave that
+//    multiplies it, and the eight states are folded through LDS;
+//  * more rows (drafts, prompts): four waves, each with one or two tiles of its own, that
+//    walk together; a step's K/V comes into LDS once, by direct loads into a ring of 64 KB
+//    (two workgroups a CU), RING - 1 steps ahead, and one barrier a step hands it over.
 // A long walk is cut into chunks of steps, a workgroup each, that a second launch joins in
 // chunk order.
 //
@@ -30,11 +31,13 @@
 // as an operand of O^T = V^T P^T without leaving the lane. A direct load writes its 64 lanes'
 // 16 bytes one after another, so a fragment is read back from LDS without bank conflicts.
 //
-// Numbers. bf16: products in bf16, P as the sum of two bf16 (16 bits of it). fp32: fp32
-// products. 8 bits: codes are exact in fp16, so the products are fp16's: q is scaled to the
-// fp16 range by a power of two per row (exact for bf16; fp32 as the sum of two fp16, 22
-// bits), P s_v by one per walk (11 bits of it for bf16 queries, 22 for fp32). Sums, m and l
-// are fp32.
+// Numbers. bf16: products in bf16, P as the sum of two bf16 (16 bits of it), but as one (8
+// bits) where a wave has two tiles: there matrix products bound the pass, and the second
+// part costs a third of them; outputs then lie 2.3e-3 from 64 bits instead of 1.7e-3, of which
+// the output's own rounding is 1.7e-3. fp32: fp32 products. 8 bits: codes are exact in
+// fp16, so the products are fp16's: q is scaled to the fp16 range by a power of two per row
+// (exact for bf16; fp32 as the sum of two fp16, 22 bits), P s_v by one per walk (11 bits of
+// it for bf16 queries, 22 for fp32). Sums, m and l are fp32.
 //
 // Values that a row must not see. A masked score is replaced, not added to, so that nothing
 // of its key remains. In V a masked infinity or NaN would be 0 * inf: steps that some
@@ -70,7 +73,9 @@ struct WindowArgs {
   uint32_t g_magic;
 };
 
-constexpr int kWinThreads = 256;
+constexpr int kKeyWaves = 8;  // waves of a workgroup that share up to 16 rows' steps
+constexpr int kMergeThreads = 256;
+__host__ __device__ constexpr int win_threads(bool shared) { return shared ? 256 : 64 * kKeyWaves; }
 constexpr float kNone = -1.0e30f;  // the maximum of a row that has seen no key
 
 // n / d for 0 <= n < 2^16 with magic = ceil(2^32 / d), d >= 2 (the host checks the range)
@@ -225,13 +230,13 @@ constexpr float kLag = F16 ? 1.0f : 8.0f;
 // QP: fp16 parts that q is taken as over 8-bit pools (1: bf16 queries, 2: fp32; else 1).
 // PP: 16-bit parts of P (fp32 pools: 1, whole).
 template <Pool P, int QP, int PP, int D, int MT, bool SHARED>
-__global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void window_attn_kernel(WindowArgs a) {
+__global__ __launch_bounds__(win_threads(SHARED)) __attribute__((amdgpu_waves_per_eu(2, 2))) void window_attn_kernel(WindowArgs a) {
   using X = PoolOf<P, D>;
   constexpr int ES = X::ES, NS = X::NS, U = X::U, NT = X::NT, SK = X::SK, SP = 16 * NS;
   constexpr bool Q8B = X::Q8B, F32 = P == Pool::kF32;
   constexpr bool QBF = P == Pool::kBf16 || (Q8B && QP == 1);  // q and out in bf16
-  constexpr int KW = SHARED ? 1 : 4;
-  constexpr int ROWS = 16 * MT * (4 / KW);
+  constexpr int KW = SHARED ? 1 : kKeyWaves;
+  constexpr int ROWS = 16 * MT * (SHARED ? 4 : 1);
   constexpr int NJ = D * ES / 64;  // fragments of a K row
   constexpr int DT = D / 16;
   constexpr int NF = F32 ? D / 16 : D / 32;  // fragments of q
@@ -745,7 +750,7 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
     __syncthreads();
     if (wid > 0) return;
 #pragma unroll
-    for (int o = 0; o < 3; ++o) {
+    for (int o = 0; o < KW - 1; ++o) {
       const float* other = sm + o * WAVE;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
@@ -794,12 +799,12 @@ __global__ __launch_bounds__(kWinThreads) __attribute__((amdgpu_waves_per_eu(2, 
 // per row, D / 64 channels a lane. The first chunks are asked for before the row's walk
 // is known (the workspace holds them whatever it is), the others four at a time.
 template <int SK, int D, bool OUT_BF16>
-__global__ __launch_bounds__(kWinThreads) void window_merge_kernel(WindowArgs a, int unit_rows) {
+__global__ __launch_bounds__(kMergeThreads) void window_merge_kernel(WindowArgs a, int unit_rows) {
   constexpr int N = D / 64, AHEAD = 4;
   struct alignas(4 * N) Vec { float v[N]; };
   const int l = threadIdx.x & 63;
   const int rmax = a.G * a.Tq;
-  const int64_t u = static_cast<int64_t>(blockIdx.x) * (kWinThreads / 64) + (threadIdx.x >> 6);
+  const int64_t u = static_cast<int64_t>(blockIdx.x) * (kMergeThreads / 64) + (threadIdx.x >> 6);
   if (u >= static_cast<int64_t>(a.B) * a.Hkv * rmax) return;
   const int r = static_cast<int>(u % rmax), bh = static_cast<int>(u / rmax);
   const int b = bh / a.Hkv, kvh = bh - b * a.Hkv;
@@ -850,8 +855,8 @@ __global__ __launch_bounds__(kWinThreads) void window_merge_kernel(WindowArgs a,
 
 // ---- launch -------------------------------------------------------------------------
 
-// Workgroups that a launch should have before walks are cut: two per compute unit.
-constexpr int kFill = 512;
+// Waves that a launch should have before walks are cut: eight per compute unit.
+constexpr int kFillWaves = 2048;
 // Workgroups from which on a wave takes two tiles of rows.
 constexpr int kTwoTiles = 48;
 
@@ -861,13 +866,16 @@ struct WindowCfg {
 };
 
 // Walks are not cut below `least` steps, where a chunk's own start and its part of the
-// join outweigh the steps it takes over (window 1024 of 32 sequences x 5 rows in bf16 at 1 / 2 /
-// 4 / 8 steps 18.9 / 19.0 / 19.4 / 22.8 us, 8-bit 20.4 / 20.4 / 18.4 / 23.9; up to 16 rows, where
-// four waves share them, 4 / 8 / 16 steps of 8 long histories 23.1 / 17.5 / 18.3 us; fp32 pools,
-// bound by their products, 1 / 2 / 4 steps 11.7 / 14.0 / 19.2). Two tiles a wave halve the
-// LDS reads per product and pay where the workgroups fill the chip all the same (bf16, 1 / 2
-// tiles: prompts 291 / 191 us, 32 x 9 rows 25.5 / 23.0, 4 x 33 17.5 / 19.8, 1 x 100 18.4 / 21.4);
-// fp32 queries, bound by products or registers, keep one (prompt of 1025 242 / 275 us).
+// join outweigh the steps it takes over: more than 16 rows, 1 / 2 / 4 / 8 steps, bf16 (32 x 5
+// rows, window 1024) 18.9 / 19.0 / 19.4 / 22.8 us, 8-bit (16 x 5) 20.4 / 20.4 / 18.4 / 23.9, fp32
+// pools, bound by their products, 11.7 / 14.0 / 19.2 / 26.2. Up to 16 rows, 8 / 16 / 32 steps: 8 long
+// histories in bf16 18.1 / 20.9 / 28.5, 32 under a window of 1024 15.2 / 19.5 / 18.2; where
+// all waves are done in two turns, the join costs more than it gains (1000 keys 9.7 us, 8.7
+// in one piece). Eight waves for four: 32 long 8-bit histories 28.3 -> 25.9 us.
+// Two tiles a wave halve the LDS reads per product and pay where the workgroups fill the chip
+// all the same (bf16, 1 / 2 tiles: prompts 291 / 191 us, 32 x 9 rows 25.5 / 23.0, 4 x 33 17.5 /
+// 19.8, 1 x 100 18.4 / 21.4); fp32 queries, bound by products or registers, keep one
+// (prompt of 1025 242 / 275 us).
 static WindowCfg window_cfg(int B, int Tq, int Hq, int Hkv, int D, int max_ctx, int window,
                             int sinks, int elem_bytes, bool f32) {
   WindowCfg c{};
@@ -881,10 +889,13 @@ static WindowCfg window_cfg(int B, int Tq, int Hq, int Hkv, int D, int max_ctx, 
       std::min<int64_t>(max_ctx, static_cast<int64_t>(window) + cdiv(c.rows, Hq / Hkv) + 1);
   int64_t steps = keys / sk + 2;
   if (keys < max_ctx) steps += cdiv(std::min(sinks, max_ctx), sk);
-  const int least = c.mt == 0 ? 8 : elem_bytes == 4 ? 1 : 4;
+  const int waves = c.mt == 0 ? kKeyWaves : 4;
+  int64_t least = c.mt == 0 ? kKeyWaves : elem_bytes == 4 ? 1 : 4;
+  if (c.mt == 0 && steps <= 2 * kKeyWaves + 1) least = steps;
   const int64_t units = static_cast<int64_t>(B) * Hkv * c.row_groups;
-  const int64_t want = std::max<int64_t>(1, kFill / units);
-  const int64_t chunk = std::max<int64_t>((steps + want - 1) / want, least);
+  const int64_t want = std::max<int64_t>(1, kFillWaves / waves / units);
+  int64_t chunk = std::max<int64_t>((steps + want - 1) / want, least);
+  if (c.mt == 0) chunk = (chunk + kKeyWaves - 1) / kKeyWaves * kKeyWaves;
   c.splits = static_cast<int>((steps + chunk - 1) / chunk);
   c.chunk = static_cast<int>(chunk);
   if (c.splits > 1) {
@@ -898,9 +909,9 @@ static WindowCfg window_cfg(int B, int Tq, int Hq, int Hkv, int D, int max_ctx, 
 template <Pool P, int QP, int PP, int D, int MT, bool SHARED>
 static void launch_walk(const WindowArgs& a, hipStream_t st) {
   const int64_t grid = static_cast<int64_t>(a.B) * a.Hkv * a.splits * a.row_groups;
-  const size_t lds = SHARED ? kRingBytes : 3 * MT * (D * 16 + 32) * sizeof(float);
+  const size_t lds = SHARED ? kRingBytes : (kKeyWaves - 1) * MT * (D * 16 + 32) * sizeof(float);
   hipLaunchKernelGGL((window_attn_kernel<P, QP, PP, D, MT, SHARED>), dim3(static_cast<unsigned>(grid)),
-                     dim3(kWinThreads), lds, st, a);
+                     dim3(win_threads(SHARED)), lds, st, a);
 }
 
 template <Pool P, int QP, int PP, int D>
@@ -915,7 +926,7 @@ static int launch_window(const WindowArgs& a, const WindowCfg& c, hipStream_t st
     constexpr bool bf = P == Pool::kBf16 || (PoolOf<P, D>::Q8B && QP == 1);
     const int64_t rows = static_cast<int64_t>(a.B) * a.Hkv * a.G * a.Tq;
     hipLaunchKernelGGL((window_merge_kernel<PoolOf<P, D>::SK, D, bf>),
-                       dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(kWinThreads), 0, st, a, c.rows);
+                       dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(kMergeThreads), 0, st, a, c.rows);
   }
   return check_launch("kve_paged_window_attn");
 }
