@@ -15,7 +15,7 @@ from dataclasses import dataclass, field
 import torch
 
 from . import kernels
-from .forward import forward_hidden
+from .forward import forward_hidden, forward_with_own_cache
 from .model import lm_head_weight
 
 AUTO_EOS = "auto"
@@ -124,6 +124,29 @@ def greedy_paged(model, input_ids: torch.Tensor, pool, max_new_tokens: int = 32,
             seq.free()
     r.sequence = None if free_on_finish else seq
     return r
+
+
+# Rows of logits that scoring holds at once (151936 ids in bf16: 156 MB).
+SCORE_ROWS = 512
+
+
+@torch.no_grad()
+def score_tokens(model, input_ids: torch.Tensor, cache, top: int = 0):
+    """Log probabilities of a text: input_ids [1, T] (T >= 2) are appended to `cache` in one
+    pass; -> kernels.token_logprobs of each token after the first given those before it
+    (logprobs [T - 1], entropy [T - 1], top_ids [T - 1, top], top_logprobs [T - 1, top]).
+    The mean of -logprobs over one text, with the cache in the model's type and in 8 bits or
+    with and without a window, is what either costs."""
+    T = input_ids.shape[1]
+    if T < 2:
+        raise ValueError(f"{T} tokens: the first one has no probability")
+    hidden = forward_with_own_cache(model, input_ids, cache, all_logits=True, return_hidden=True)[0]
+    nxt = input_ids[0, 1:].to(device=hidden.device, dtype=torch.int32).contiguous()
+    parts = []
+    for a in range(0, T - 1, SCORE_ROWS):
+        b = min(a + SCORE_ROWS, T - 1)
+        parts.append(kernels.token_logprobs(model.lm_head(hidden[a:b]), nxt[a:b], top=top))
+    return tuple(torch.cat(x) for x in zip(*parts))
 
 
 @torch.no_grad()

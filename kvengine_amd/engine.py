@@ -47,7 +47,7 @@ import torch
 from . import kernels
 from .capture import no_gc
 from .forward import (SPLITK_MAX_ROWS, _fusable, forward_hidden, forward_packed,
-                      forward_packed_wide, invariant_gemm_rows, blocked_forward)
+                      forward_packed_wide, invariant_gemm_rows, blocked_forward, windowed)
 from .model import lm_head_blocked
 from .paged import PagedKVCache, PagedSequenceCache
 
@@ -228,6 +228,9 @@ class SpecEngine:
                  prefix_sharing: bool = False, narrow_batches: bool | None = None,
                  events: list | None = None):
         assert k >= 1
+        for m in (target, draft):
+            if windowed(m):
+                raise NotImplementedError("the engine's passes take no sliding window")
         self.target, self.draft = target, draft
         # Admission adopts the published full blocks of a prompt's prefix
         # (refcounted, content-addressed: kvengine/paged.py:209-279) and

@@ -17,12 +17,13 @@ LM head to the caller (the spec loop fuses it with argmax).
 
 from __future__ import annotations
 
+import functools
 import os
 
 import torch
 
 from . import kernels
-from .paged import DeviceKV
+from .paged import DeviceKV, write_kv
 
 USE_SDPA = os.environ.get("KVENGINE_EAGER_ATTN", "0") != "1"
 
@@ -81,20 +82,37 @@ class LayerAttention:
     (kve_attn_plan) shared by every layer, and the summation order `attn` =
     (unit_blocks, key_waves) of kve_paged_verify_attn ((0, 0): chosen per
     launch; fixed values make a row's result independent of the batch). tree: the
-    (masks, depths) of a pass over trees (kernels.tree_masks)."""
+    (masks, depths) of a pass over trees (kernels.tree_masks). Layers with a window
+    (kernels.paged_window_attn) and 8-bit pools (kernels.paged_q8_attn) take neither plan nor
+    order."""
 
     def __init__(self, kv: DeviceKV, rows, B: int, T: int, Hq: int, max_ctx: int, q_lens,
                  dtype, attn: tuple[int, int] = (0, 0), tree=None):
         self.kv, self.rows, self.q_lens, self.max_ctx = kv, rows, q_lens, max_ctx
         self.masks = None if tree is None else tree[0]
         self.unit_blocks, self.key_waves = attn
-        _, NB, Hkv, bs, D = kv.k.shape
-        self.plan = kernels.attn_plan(kv.tables, kv.lens, B, T, Hq, Hkv, D, bs, NB, max_ctx, dtype,
-                                      seq_rows=rows, q_lens=q_lens, unit_blocks=self.unit_blocks,
-                                      key_waves=self.key_waves)
+        self.sizes = B, T, Hq, dtype
 
-    def __call__(self, q, li: int, scale: float, out=None, blocked: bool = False):
+    @functools.cached_property
+    def plan(self):
+        """Made by the first layer that needs it."""
+        kv, (B, T, Hq, dtype) = self.kv, self.sizes
+        _, NB, Hkv, bs, D = kv.k.shape
+        return kernels.attn_plan(kv.tables, kv.lens, B, T, Hq, Hkv, D, bs, NB, self.max_ctx, dtype,
+                                 seq_rows=self.rows, q_lens=self.q_lens, unit_blocks=self.unit_blocks,
+                                 key_waves=self.key_waves)
+
+    def __call__(self, q, li: int, scale: float, out=None, blocked: bool = False,
+                 window: int | None = None, sinks: int = 0):
         kv = self.kv
+        if kv.k_scale is not None:
+            return kernels.paged_q8_attn(q, kv.k[li], kv.v[li], kv.k_scale[li], kv.v_scale[li],
+                                         kv.tables, kv.lens, self.max_ctx, window=window, sinks=sinks,
+                                         seq_rows=self.rows, q_lens=self.q_lens, scale=scale, out=out)
+        if window is not None:
+            return kernels.paged_window_attn(q, kv.k[li], kv.v[li], kv.tables, kv.lens, self.max_ctx,
+                                             window, sinks, seq_rows=self.rows, q_lens=self.q_lens,
+                                             scale=scale, out=out)
         if self.masks is not None:
             return kernels.paged_tree_attn(q, kv.k[li], kv.v[li], kv.tables, kv.lens, self.max_ctx,
                                            self.masks, seq_rows=self.rows, q_lens=self.q_lens,
@@ -105,6 +123,24 @@ class LayerAttention:
                                          seq_rows=self.rows, q_lens=self.q_lens, scale=scale,
                                          unit_blocks=self.unit_blocks, key_waves=self.key_waves,
                                          plan=self.plan, out=out, blocked=blocked)
+
+
+def _window(attn) -> tuple[int | None, int]:
+    """A layer's (sliding_window, sinks), as transformers names the first; the second is
+    this framework's own (window_sinks, 0 where a module has none)."""
+    return getattr(attn, "sliding_window", None), getattr(attn, "window_sinks", 0)
+
+
+def windows(model) -> tuple:
+    """(sliding_window, sinks) of each layer."""
+    return tuple(_window(layer.self_attn) for layer in model.model.layers)
+
+
+def windowed(model) -> bool:
+    """Some layer of the model has a sliding window."""
+    # (out of the module's dictionary: nn.Module's attribute lookup costs a microsecond a layer)
+    return any(layer._modules["self_attn"].__dict__.get("sliding_window") is not None
+               for layer in model.model.layers)
 
 
 def _q_heads(model, kv: DeviceKV) -> int:
@@ -225,6 +261,11 @@ def forward_hidden(model, input_ids: torch.Tensor, kv: DeviceKV, rows: torch.Ten
     The fp32 pass of one host call (kernels.f32_pass) takes chains only: trees run
     the library GEMMs there, whose sums have another order. After the commit
     kernels.tree_accept picks the path and makes its K/V consecutive.
+
+    Layers whose self_attn.sliding_window is set attend to that many latest tokens and
+    the first self_attn.window_sinks; an 8-bit pool (PagedKVCache of int8 or
+    float8_e4m3fn) is written with kernels.kv_write_q8. Both run the library-GEMM layer,
+    whose attention order is its own (attn_order and gemm_rows do not apply).
     """
     if tree is not None:
         masks, depths = tree
@@ -234,6 +275,11 @@ def forward_hidden(model, input_ids: torch.Tensor, kv: DeviceKV, rows: torch.Ten
     if fused is None:
         fused = _fusable(model)
     n = input_ids.numel()
+    if kv.k_scale is not None or windowed(model):
+        if tree is not None or blocked_out:
+            raise NotImplementedError("trees and blocked hidden states over a window or an 8-bit cache")
+        run = _forward_fused if fused else _forward_modules
+        return run(model, input_ids, kv, rows, max_ctx, q_lens, attn_order)
     if blocked_out:
         if not (fused and blocked_forward(model, n, gemm_rows)):
             raise ValueError("blocked_out needs the blocked split-K layer (blocked_forward)")
@@ -253,6 +299,11 @@ def forward_hidden(model, input_ids: torch.Tensor, kv: DeviceKV, rows: torch.Ten
         if tree is None and _f32_ok(model, n) and _plain_tokens(model, input_ids):
             return _forward_f32(model, input_ids, kv, rows, max_ctx, q_lens, attn_order)
         return _forward_fused(model, input_ids, kv, rows, max_ctx, q_lens, attn_order, tree)
+    return _forward_modules(model, input_ids, kv, rows, max_ctx, q_lens, attn_order, tree)
+
+
+def _forward_modules(model, input_ids, kv: DeviceKV, rows, max_ctx, q_lens, attn_order, tree=None):
+    """The layer loop as transformers-style module calls."""
     inner = model.model
     B, T = input_ids.shape
     hidden = inner.embed_tokens(input_ids)
@@ -261,8 +312,6 @@ def forward_hidden(model, input_ids: torch.Tensor, kv: DeviceKV, rows: torch.Ten
                                 attn_order, tree)
     for layer in inner.layers:
         attn = layer.self_attn
-        if getattr(attn, "sliding_window", None) is not None:
-            raise NotImplementedError("sliding-window attention needs a windowed mask; this model uses it")
         li = attn.layer_idx
         D = attn.head_dim
         residual = hidden
@@ -271,9 +320,9 @@ def forward_hidden(model, input_ids: torch.Tensor, kv: DeviceKV, rows: torch.Ten
         k = attn.k_proj(h).view(B, T, -1, D)
         v = attn.v_proj(h).view(B, T, -1, D)
         q, k = apply_rope(q, k, cos, sin, unsqueeze_dim=2)
-        kernels.kv_write(k, v, kv.k[li], kv.v[li], kv.tables, kv.lens, seq_rows=rows,
-                         q_lens=q_lens)
-        out = layer_attn(q, li, attn.scaling)
+        write_kv(kv, li, k, v, rows, q_lens)
+        window, sinks = _window(attn)
+        out = layer_attn(q, li, attn.scaling, window=window, sinks=sinks)
         hidden = residual + attn.o_proj(out.view(B, T, -1))
         residual = hidden
         hidden = residual + layer.mlp(layer.post_attention_layernorm(hidden))
@@ -372,14 +421,19 @@ def _forward_fused(model, input_ids, kv: DeviceKV, rows, max_ctx, q_lens, attn_o
                                 attn_order, tree)
     for i, layer in enumerate(layers):
         attn = layer.self_attn
-        if getattr(attn, "sliding_window", None) is not None:
-            raise NotImplementedError("sliding-window attention needs a windowed mask; this model uses it")
         li = attn.layer_idx
         qkv = torch.nn.functional.linear(h, attn.qkv_weight, attn.qkv_bias)
-        q = kernels.rope_kv_write(qkv, cos, sin, kv.k[li], kv.v[li], kv.tables, kv.lens,
-                                  attn.num_key_value_groups * kv.k.shape[2], seq_rows=rows,
-                                  q_lens=q_lens)
-        out = layer_attn(q, li, attn.scaling)
+        if kv.k_scale is None:
+            q = kernels.rope_kv_write(qkv, cos, sin, kv.k[li], kv.v[li], kv.tables, kv.lens,
+                                      attn.num_key_value_groups * kv.k.shape[2], seq_rows=rows,
+                                      q_lens=q_lens)
+        else:
+            Hkv, D = kv.k.shape[2], kv.k.shape[4]
+            q, k, v = qkv.view(B, T, -1, D).split([attn.num_key_value_groups * Hkv, Hkv, Hkv], dim=2)
+            q, k = apply_rope(q, k, cos, sin, unsqueeze_dim=2)
+            write_kv(kv, li, k, v.contiguous(), rows, q_lens)
+        window, sinks = _window(attn)
+        out = layer_attn(q, li, attn.scaling, window=window, sinks=sinks)
         post = layer.post_attention_layernorm
         if splitk:
             part = kernels.linear_splitk(out.view(B * T, -1), attn.o_proj.weight)
@@ -403,6 +457,11 @@ def _forward_fused(model, input_ids, kv: DeviceKV, rows, max_ctx, q_lens, attn_o
     return h
 
 
+def _need_plain(model, kv: DeviceKV) -> None:
+    if kv.k_scale is not None or windowed(model):
+        raise NotImplementedError("packed prefills take neither a sliding window nor an 8-bit pool")
+
+
 def forward_packed(model, ids: torch.Tensor, dst: torch.Tensor, B: int, T: int, kv: DeviceKV,
                    rows: torch.Tensor, max_ctx: int, q_lens: torch.Tensor,
                    attn_order: tuple[int, int] = (0, 0)) -> torch.Tensor:
@@ -413,7 +472,8 @@ def forward_packed(model, ids: torch.Tensor, dst: torch.Tensor, B: int, T: int, 
     on the padded [B, T] layout, which packed rows are scattered into and
     gathered back from. Same per-sequence semantics as forward_hidden over the
     padded [B, T] batch; the caller commits lengths afterwards. Models whose
-    shapes fit (_wide_ok) take forward_packed_wide."""
+    shapes fit (_wide_ok) take forward_packed_wide. Pools of the model's type only."""
+    _need_plain(model, kv)
     if _wide_ok(model, ids.numel()):
         return forward_packed_wide(model, ids, dst, B, T, kv, rows, max_ctx, q_lens, attn_order)
     inner = model.model
@@ -433,8 +493,6 @@ def forward_packed(model, ids: torch.Tensor, dst: torch.Tensor, B: int, T: int, 
                                 attn_order)
     for i, layer in enumerate(layers):
         attn = layer.self_attn
-        if getattr(attn, "sliding_window", None) is not None:
-            raise NotImplementedError("sliding-window attention needs a windowed mask; this model uses it")
         li = attn.layer_idx
         qkv = torch.nn.functional.linear(h, attn.qkv_weight, attn.qkv_bias)
         qkv_pad.index_copy_(0, dst, qkv)
@@ -493,6 +551,7 @@ def forward_packed_wide(model, ids: torch.Tensor, dst: torch.Tensor, B: int, T: 
     tokens recomputed here, therefore continue exactly as if every token had
     come from a verify pass (the reference recomputes the same way,
     kvengine/engine.py:425-440)."""
+    _need_plain(model, kv)
     inner = model.model
     layers = inner.layers
     N = ids.numel()
@@ -518,8 +577,6 @@ def forward_packed_wide(model, ids: torch.Tensor, dst: torch.Tensor, B: int, T: 
     layer_attn = LayerAttention(kv, rows, B, T, Hq, max_ctx, q_lens, kv.k.dtype, attn_order)
     for i, layer in enumerate(layers):
         attn = layer.self_attn
-        if getattr(attn, "sliding_window", None) is not None:
-            raise NotImplementedError("sliding-window attention needs a windowed mask; this model uses it")
         li = attn.layer_idx
         mlp = layer.mlp
         part = _wide_proj(xn, attn.qkv_weight_blk if blk else attn.qkv_weight, kernels.ROWS_QKV,
@@ -601,8 +658,6 @@ def _pass_layers(model, blk: bool = False):
     for layer in model.model.layers:
         sub = layer._modules  # (nn.Module's attribute lookup costs a microsecond each)
         attn, mlp = sub["self_attn"], sub["mlp"]
-        if getattr(attn, "sliding_window", None) is not None:
-            raise NotImplementedError("sliding-window attention needs a windowed mask; this model uses it")
         norm, post = sub["input_layernorm"], sub["post_attention_layernorm"]
         layers.append((attn.layer_idx, norm.weight, attn.qkv_weight_blk if blk else attn.qkv_weight,
                        attn.qkv_bias, attn.o_weight_blk if blk else attn.o_proj.weight, post.weight,
@@ -667,7 +722,7 @@ def _has_blocked(model) -> bool:
 def blocked_forward(model, n: int, gemm_rows: int | None = None) -> bool:
     """forward_hidden of n rows (with this gemm_rows) runs the split-K layer on
     blocked operands, so it can return its hidden states blocked."""
-    if not (_fusable(model) and _has_blocked(model) and n <= SPLITK_MAX_ROWS):
+    if not (_fusable(model) and _has_blocked(model) and n <= SPLITK_MAX_ROWS) or windowed(model):
         return False
     if gemm_rows is not None and n <= gemm_rows and _wide_ok(model, gemm_rows):
         return True
@@ -705,8 +760,6 @@ def _forward_splitk(model, input_ids, kv: DeviceKV, rows, max_ctx, q_lens, attn_
                                 attn_order, tree)
     for i, layer in enumerate(layers):
         attn = layer.self_attn
-        if getattr(attn, "sliding_window", None) is not None:
-            raise NotImplementedError("sliding-window attention needs a windowed mask; this model uses it")
         li = attn.layer_idx
         Hq = attn.num_key_value_groups * kv.k.shape[2]
         mlp = layer.mlp

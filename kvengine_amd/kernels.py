@@ -1177,12 +1177,14 @@ def kv_write_q8(k_new: torch.Tensor, v_new: torch.Tensor, k_layer: torch.Tensor,
     code = _dtype_code(k_new)
     if B == 0 or T == 0:
         return
-    st = k_new.stride()
-    if st != v_new.stride() or st[3] != 1 or st[2] != D or (B > 1 and st[0] != T * st[1]):
-        raise ValueError(f"k_new/v_new layouts {st}, {v_new.stride()} not [B, T, Hkv, D] with "
-                         "contiguous heads")
+    tok = k_new.stride(1) if T > 1 else k_new.stride(0) if B > 1 else Hkv * D
+    for st in (k_new.stride(), v_new.stride()):  # (of dimensions longer than one)
+        if (st[3] != 1 or (Hkv > 1 and st[2] != D) or (T > 1 and st[1] != tok)
+                or (B > 1 and st[0] != T * tok)):
+            raise ValueError(f"k_new/v_new layouts {k_new.stride()}, {v_new.stride()} not [B, T, Hkv, D] "
+                             "with contiguous heads and one stride for all tokens")
     _call(_lib.lib().kve_kv_write_q8, "kve_kv_write_q8", dev, k_new.data_ptr(), v_new.data_ptr(),
-          st[1], k_layer.data_ptr(), v_layer.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+          tok, k_layer.data_ptr(), v_layer.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
           block_tables.data_ptr(), _ptr(seq_rows), start_pos.data_ptr(), _ptr(q_lens), B, T, Hkv, D,
           bs, max_blocks, num_rows, NB, code, pool)
 

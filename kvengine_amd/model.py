@@ -96,7 +96,8 @@ class Attention(nn.Module):
         self.num_key_value_heads = arch.num_kv_heads
         self.num_key_value_groups = arch.group
         self.scaling = arch.head_dim ** -0.5
-        self.sliding_window = None
+        self.sliding_window = None  # tokens a query sees, itself included (None: all)
+        self.window_sinks = 0       # first tokens that stay visible behind the window
         self.q_proj = nn.Linear(arch.hidden, arch.q_dim, bias=True)
         self.k_proj = nn.Linear(arch.hidden, arch.kv_dim, bias=True)
         self.v_proj = nn.Linear(arch.hidden, arch.kv_dim, bias=True)

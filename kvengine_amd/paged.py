@@ -37,6 +37,20 @@ class DeviceKV:
     tables: torch.Tensor     # [rows, max_blocks] int32
     lens: torch.Tensor       # [rows] int32, committed length per row
     block_size: int
+    k_scale: torch.Tensor | None = None  # [L, NB, Hkv] float32: k and v hold 8-bit codes
+    v_scale: torch.Tensor | None = None
+
+
+def write_kv(kv: DeviceKV, layer_idx: int, k_new: torch.Tensor, v_new: torch.Tensor,
+             rows: torch.Tensor, q_lens: torch.Tensor | None = None) -> None:
+    """New K/V rows [B, T, Hkv, D] of a layer behind the rows' committed lengths, in the
+    pool's type."""
+    if kv.k_scale is None:
+        kernels.kv_write(k_new, v_new, kv.k[layer_idx], kv.v[layer_idx], kv.tables, kv.lens,
+                         seq_rows=rows, q_lens=q_lens)
+    else:
+        kernels.kv_write_q8(k_new, v_new, kv.k[layer_idx], kv.v[layer_idx], kv.k_scale[layer_idx],
+                            kv.v_scale[layer_idx], kv.tables, kv.lens, seq_rows=rows, q_lens=q_lens)
 
 
 def _model_info(model) -> dict:
@@ -51,7 +65,14 @@ def _model_info(model) -> dict:
 
 
 class PagedKVCache:
-    """The shared pool: block tensors, the allocator, device tables and lengths."""
+    """The shared pool: block tensors, the allocator, device tables and lengths.
+
+    dtype int8 or float8_e4m3fn: the pool holds 8-bit codes with a scale for each block
+    and head (kernels.kv_write_q8), half the bytes of bf16 and a quarter of fp32; blocks of
+    a multiple of 16 tokens, head_dim 64 or 128. Passes over it run through forward_hidden
+    (greedy and speculative decoding, chains only); the batched engine needs a pool of the
+    model's type. A block's scale only grows while the block holds rows, so tokens that a
+    rejected draft wrote may leave a coarser scale behind."""
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_blocks: int,
                  block_size: int, dtype: torch.dtype, device, max_seqs: int = 64,
@@ -67,6 +88,14 @@ class PagedKVCache:
                              dtype=dtype, device=self.device)
         self.v = torch.zeros((num_layers, num_blocks, num_kv_heads, head_dim, block_size),
                              dtype=dtype, device=self.device)
+        self.k_scale = self.v_scale = None
+        if dtype in kernels.Q8_DTYPES:
+            if block_size % 16 or head_dim not in (64, 128):
+                raise ValueError(f"an 8-bit pool needs blocks of a multiple of 16 tokens and heads of 64 "
+                                 f"or 128, not {block_size} and {head_dim}")
+            self.k_scale, self.v_scale = (
+                torch.zeros((num_layers, num_blocks, num_kv_heads), dtype=torch.float32,
+                            device=self.device) for _ in range(2))
         self.max_blocks = max_blocks_per_seq or num_blocks
         self.max_seqs = max_seqs
         self.tables = torch.full((max_seqs, self.max_blocks), -1, dtype=torch.int32,
@@ -77,11 +106,12 @@ class PagedKVCache:
 
     @classmethod
     def for_model(cls, model, num_blocks: int, block_size: int = DEFAULT_BLOCK_SIZE,
-                  max_seqs: int = 64) -> "PagedKVCache":
+                  max_seqs: int = 64, dtype: torch.dtype | None = None) -> "PagedKVCache":
+        """dtype: the pool's (default the model's)."""
         info = _model_info(model)
         p = next(model.parameters())
         return cls(info["num_layers"], info["num_key_value_heads"], info["head_dim"], num_blocks,
-                   block_size, p.dtype, p.device, max_seqs=max_seqs)
+                   block_size, dtype or p.dtype, p.device, max_seqs=max_seqs)
 
     # --- rows of the device tables ---
 
@@ -96,12 +126,14 @@ class PagedKVCache:
         self._free_rows.append(row)
 
     def device_kv(self) -> DeviceKV:
-        return DeviceKV(self.k, self.v, self.tables, self.lens, self.block_size)
+        return DeviceKV(self.k, self.v, self.tables, self.lens, self.block_size, self.k_scale,
+                        self.v_scale)
 
     # --- capacity accounting (kvengine/paged.py:92-113) ---
 
     def nbytes(self) -> int:
-        return self.k.numel() * self.k.element_size() * 2
+        scales = 0 if self.k_scale is None else self.k_scale.numel() * 4
+        return (self.k.numel() * self.k.element_size() + scales) * 2
 
     def bytes_per_block(self) -> int:
         return self.nbytes() // self.num_blocks
@@ -226,18 +258,20 @@ class PagedSequenceCache:
             "reserve() must be called with this pass's token count before write()")
         self.write_rows(layer_idx, k[0].transpose(0, 1).unsqueeze(0).contiguous(),
                         v[0].transpose(0, 1).unsqueeze(0).contiguous())
-        return self._gather(layer_idx, start + n)
+        return tuple(t.to(k.dtype) for t in self._gather(layer_idx, start + n))
 
     def write_rows(self, layer_idx: int, k_new: torch.Tensor, v_new: torch.Tensor) -> None:
         """k_new/v_new [1, T, Hkv, D] at positions length..length+T-1 (kernel scatter)."""
-        kernels.kv_write(k_new, v_new, self.pool.k[layer_idx], self.pool.v[layer_idx],
-                         self.pool.tables, self.pool.lens, seq_rows=self.row_dev)
+        write_kv(self.device_kv(), layer_idx, k_new, v_new, self.row_dev)
 
     def _gather(self, layer_idx: int, end: int):
         nb = self.pool.manager.blocks_needed(end)
         ids = torch.tensor(self.blocks[:nb], dtype=torch.long, device=self.pool.device)
         k = self.pool.k[layer_idx][ids]            # [nb, Hkv, bs, D]
         v = self.pool.v[layer_idx][ids]            # [nb, Hkv, D, bs]
+        if self.pool.k_scale is not None:          # what the codes stand for, in float32
+            k = k.float() * self.pool.k_scale[layer_idx][ids][..., None, None]
+            v = v.float() * self.pool.v_scale[layer_idx][ids][..., None, None]
         Hkv, D, bs = self.pool.num_kv_heads, self.pool.head_dim, self.block_size
         k_all = k.permute(1, 0, 2, 3).reshape(Hkv, nb * bs, D)[:, :end]
         v_all = v.permute(1, 0, 3, 2).reshape(Hkv, nb * bs, D)[:, :end]

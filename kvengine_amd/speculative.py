@@ -46,7 +46,7 @@ import torch
 from . import kernels
 from .capture import no_gc
 from .decode import AUTO_EOS, _resolve_eos, _sync, argmax_rows
-from .forward import forward_hidden
+from .forward import forward_hidden, windows
 from .model import lm_head_weight
 from .paged import PagedSequenceCache
 
@@ -139,9 +139,13 @@ class _IterationGraphs:
         when any of them is freed), bound to this call's caches."""
         tp, dp = t_cache.pool, d_cache.pool
         # every address a replay reads: a model whose weights or a pool whose
-        # tables were replaced since the capture gets new graphs
+        # tables were replaced since the capture gets new graphs; so does one
+        # whose windows were set since, which the launches hold by value
         key = (id(target), id(draft), id(tp), id(dp), k, _addresses(target), _addresses(draft),
-               tuple(t.data_ptr() for p in (tp, dp) for t in (p.tables, p.lens, p.k, p.v)))
+               _windows(target), _windows(draft),
+               tuple(None if t is None else t.data_ptr() for p in (tp, dp)
+                     for t in (p.tables, p.lens, p.k, p.v, getattr(p, "k_scale", None),
+                               getattr(p, "v_scale", None))))
         g = _GRAPHS.get(key)
         if g is None:
             g = _GRAPHS[key] = _IterationGraphs(t_cache.pool, k)
@@ -259,6 +263,11 @@ def _addresses(model) -> int:
             if isinstance(t, torch.Tensor):
                 ptrs.append(t.data_ptr())
     return hash(tuple(ptrs))
+
+
+def _windows(model) -> tuple:
+    """windows() of a model with layers."""
+    return windows(model) if hasattr(model, "model") else ()
 
 
 def _feed(model, cache, ids: torch.Tensor) -> torch.Tensor:
