@@ -388,7 +388,8 @@ extern "C" int kve_token_logprobs(const void* logits, int64_t row_stride, const 
   KVE_REQUIRE((reinterpret_cast<uintptr_t>(logits) & (esz - 1)) == 0,
               "kve_token_logprobs: logits are not aligned to their type");
   const LogprobCfg c = logprob_cfg(rows, vocab, top, dtype);
-  KVE_REQUIRE(static_cast<long long>(rows) * c.chunks < (1ll << 30),
+  // (chunks are counted in 32 bits, and a launch has below 2^32 threads)
+  KVE_REQUIRE(rows < (1 << 22) && static_cast<long long>(rows) * c.chunks < (1ll << 30),
               "kve_token_logprobs: %d rows of %d too large for one launch", rows, vocab);
   KVE_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
               "kve_token_logprobs: workspace required (16-byte aligned)");

@@ -286,7 +286,8 @@ extern "C" int kve_kv_write_q8(const void* k_new, const void* v_new, int64_t src
   // tokens o .. o + q_len - 1 of a block offset o <= block_size - 1
   a.spans = static_cast<int>((static_cast<int64_t>(q_len) + block_size - 2) / block_size) + 1;
   a.units = static_cast<int64_t>(num_seqs) * a.spans * num_kv_heads * 2;
-  KVE_REQUIRE(a.units < (1ll << 31), "kve_kv_write_q8: %d x %d tokens too large for one launch",
+  // (a launch has below 2^32 threads)
+  KVE_REQUIRE(a.units < (1ll << 26), "kve_kv_write_q8: %d x %d tokens too large for one launch",
               num_seqs, q_len);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == KVE_DTYPE_BF16) launch_write_q8<uint16_t>(a, pool_dtype, st);

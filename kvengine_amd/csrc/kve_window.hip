@@ -48,7 +48,7 @@
 #include "kve_q8.h"
 
 #include <algorithm>
-#include <mutex>
+#include <cfloat>
 #include <type_traits>
 
 namespace kve {
@@ -71,16 +71,20 @@ struct WindowArgs {
   int row_groups, chunk, splits;  // chunk: steps of a workgroup
   float scale_log2;
   uint32_t g_magic;
+  int g_shift;
 };
 
 constexpr int kKeyWaves = 8;  // waves of a workgroup that share up to 16 rows' steps
 constexpr int kMergeThreads = 256;
 __host__ __device__ constexpr int win_threads(bool shared) { return shared ? 256 : 64 * kKeyWaves; }
-constexpr float kNone = -1.0e30f;  // the maximum of a row that has seen no key
+// The maximum of a row that has seen no key. Finite, for -inf less itself is NaN, and no
+// score is lower but -inf.
+constexpr float kNone = -FLT_MAX;
 
-// n / d for 0 <= n < 2^16 with magic = ceil(2^32 / d), d >= 2 (the host checks the range)
-__device__ __forceinline__ int div_magic(int n, int d, uint32_t magic) {
-  return d == 1 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), magic));
+// Token of row r: r / G for 0 <= r < 2^31. With 2^(s - 1) < G <= 2^s the product with
+// ceil(2^(31 + s) / G) is over by r (G - 1) / G / 2^(31 + s) < 1 / G at most.
+__device__ __forceinline__ int token_of(const WindowArgs& a, int r) {
+  return a.G == 1 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), a.g_magic) >> a.g_shift);
 }
 
 struct WinSeq {
@@ -108,8 +112,8 @@ struct Walk {
 template <int SK>
 __device__ __forceinline__ Walk walk_of(const WindowArgs& a, const WinSeq& s, int row0, int row1) {
   Walk w;
-  w.p0 = s.start + div_magic(row0, a.G, a.g_magic);
-  w.p1 = s.start + div_magic(row1 - 1, a.G, a.g_magic);
+  w.p0 = s.start + token_of(a, row0);
+  w.p1 = s.start + token_of(a, row1 - 1);
   w.first = w.p0 >= a.window ? (w.p0 - a.window + 1) / SK : 0;
   w.sinks = min((a.sinks + SK - 1) / SK, w.first);
   w.total = w.sinks + w.p1 / SK - w.first + 1;
@@ -266,8 +270,8 @@ __global__ __launch_bounds__(win_threads(SHARED)) __attribute__((amdgpu_waves_pe
   const int kw = SHARED ? 0 : wid, at = c * a.chunk + kw;
   const int n = cdiv(max(min(w.total, (c + 1) * a.chunk) - at, 0), KW);
   const bool active = row0 < R;
-  const int p0 = active ? s.start + div_magic(row0, a.G, a.g_magic) : w.p0;
-  const int p1 = active ? s.start + div_magic(row1 - 1, a.G, a.g_magic) : w.p1;
+  const int p0 = active ? s.start + token_of(a, row0) : w.p0;
+  const int p1 = active ? s.start + token_of(a, row1 - 1) : w.p1;
 
   // q as it lies in memory: the lane's channels of row lr of each tile, in the order of its
   // K fragments. Asked for first, for behind the first K and V it would wait for all of them.
@@ -277,7 +281,7 @@ __global__ __launch_bounds__(win_threads(SHARED)) __attribute__((amdgpu_waves_pe
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     const int r = min(row0 + mt * 16 + lr, R - 1);
-    const int t = div_magic(r, a.G, a.g_magic), h = kvh * a.G + r - t * a.G;
+    const int t = token_of(a, r), h = kvh * a.G + r - t * a.G;
     qpos[mt] = s.start + t;
     const size_t qat = ((static_cast<size_t>(b) * a.Tq + t) * a.Hq + h) * D;
     if constexpr (!Q8B) {
@@ -772,7 +776,7 @@ __global__ __launch_bounds__(win_threads(SHARED)) __attribute__((amdgpu_waves_pe
     const int r = row0 + mt * 16 + lr;
     if (r >= R) continue;
     if (chunks == 1) {
-      const int t = div_magic(r, a.G, a.g_magic), h = kvh * a.G + r - t * a.G;
+      const int t = token_of(a, r), h = kvh * a.G + r - t * a.G;
       const size_t to = ((static_cast<size_t>(b) * a.Tq + t) * a.Hq + h) * D + 4 * lg;
       const float inv = 1.0f / lsum[mt];
 #pragma unroll
@@ -843,7 +847,7 @@ __global__ __launch_bounds__(kMergeThreads) void window_merge_kernel(WindowArgs 
       for (int e = 0; e < N; ++e) o.v[e] = o.v[e] * al + po[x].v[e] * be;
     }
   }
-  const int t = div_magic(r, a.G, a.g_magic), h = kvh * a.G + r - t * a.G;
+  const int t = token_of(a, r), h = kvh * a.G + r - t * a.G;
   const size_t to = ((static_cast<size_t>(b) * a.Tq + t) * a.Hq + h) * D + l * N;
 #pragma unroll
   for (int e = 0; e < N; ++e) {
@@ -942,7 +946,8 @@ static int elem_bytes(int pool_dtype) {
 
 static bool window_sizes_ok(int B, int Tq, int Hq, int Hkv, int D, int max_ctx, int window, int sinks) {
   return B > 0 && Tq > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && (D == 64 || D == 128) &&
-         max_ctx > 0 && window >= 0 && sinks >= 0 && static_cast<int64_t>(Hq / Hkv) * Tq < 65536;
+         max_ctx > 0 && max_ctx <= (1 << 30) && window >= 0 && sinks >= 0 &&
+         static_cast<int64_t>(Hq / Hkv) * Tq < (1 << 30);
 }
 
 }  // namespace kve
@@ -1000,8 +1005,9 @@ extern "C" int kve_paged_window_attn(const void* q, const void* k_layer, const v
   const int win = window > 0 ? window : INT32_MAX;
   const WindowCfg c = window_cfg(num_seqs, q_len, num_q_heads, num_kv_heads, head_dim, max_ctx, win,
                                  sinks, elem_bytes(pool_dtype), dtype == KVE_DTYPE_F32);
-  KVE_REQUIRE(static_cast<int64_t>(num_seqs) * num_kv_heads * c.splits * c.row_groups < (1ll << 31) &&
-                  static_cast<int64_t>(num_seqs) * num_q_heads * q_len < (1ll << 31),
+  // (a launch has below 2^32 threads: 512 a workgroup, 64 a row in the join)
+  KVE_REQUIRE(static_cast<int64_t>(num_seqs) * num_kv_heads * c.splits * c.row_groups < (1ll << 23) &&
+                  static_cast<int64_t>(num_seqs) * num_q_heads * q_len < (1ll << 26),
               "kve_paged_window_attn: %d x %d tokens too large for one launch", num_seqs, q_len);
   if (workspace_bytes < c.bytes || (c.bytes && !workspace)) {
     set_error("kve_paged_window_attn: workspace %zu bytes, need %zu", workspace_bytes, c.bytes);
@@ -1039,7 +1045,10 @@ extern "C" int kve_paged_window_attn(const void* q, const void* k_layer, const v
   a.chunk = c.chunk;
   a.splits = c.splits;
   a.scale_log2 = scale * 1.44269504088896340736f;
-  a.g_magic = static_cast<uint32_t>(((1ull << 32) + a.G - 1) / a.G);
+  int s = 1;
+  while ((1ll << s) < a.G) ++s;
+  a.g_magic = static_cast<uint32_t>(((1ull << (31 + s)) + a.G - 1) / a.G);
+  a.g_shift = s - 1;
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (pool_dtype) {
     case KVE_DTYPE_BF16: return launch_window_d<Pool::kBf16, 1, 2>(a, c, head_dim, st);

@@ -138,8 +138,8 @@ def windows(model) -> tuple:
 
 def windowed(model) -> bool:
     """Some layer of the model has a sliding window."""
-    # (out of the module's dictionary: nn.Module's attribute lookup costs a microsecond a layer)
-    return any(layer._modules["self_attn"].__dict__.get("sliding_window") is not None
+    # (nn.Module's lookup of a submodule costs a microsecond a layer)
+    return any(getattr(layer._modules["self_attn"], "sliding_window", None) is not None
                for layer in model.model.layers)
 
 

@@ -1201,7 +1201,7 @@ def _window_attn(q, k_layer, v_layer, k_scale, v_scale, block_tables, start_pos,
     if Hkv < 1 or Hq % Hkv:
         raise ValueError(f"{Hq} q heads not a multiple of {Hkv} kv heads")
     num_rows, max_blocks = _check_paged(block_tables, start_pos, seq_rows, q_lens, B, dev)
-    if max_ctx < 1 or max_blocks * bs < max_ctx:
+    if not 1 <= max_ctx <= min(max_blocks * bs, 1 << 30):
         raise ValueError(f"max_ctx {max_ctx} exceeds table capacity {max_blocks * bs}")
     if sinks < 0:
         raise ValueError(f"{sinks} sinks")

@@ -197,3 +197,36 @@ def test_strided_rows_and_another_stream(pool):
     write(c, k, v, 0, [5, 4], 0, 20, pool)
     write(c, k, v, 3, [0, 2], 1, 20, pool)
     same(p, c)
+
+
+def test_offsets_past_32_bits():
+    """Pools of more than 4 GiB of codes, the sequence in the last blocks."""
+    nb, Hkv, D = 1_100_000, 2, 128
+    p = dict(k=torch.zeros(nb, Hkv, 16, D, dtype=torch.int8, device=DEV),
+             v=torch.zeros(nb, Hkv, D, 16, dtype=torch.int8, device=DEV),
+             ks=torch.zeros(nb, Hkv, device=DEV), vs=torch.zeros(nb, Hkv, device=DEV))
+    assert p["k"].numel() > 1 << 32
+    c = {n: t[:4].cpu().double() for n, t in p.items()}
+    x = torch.randn(1, 40, Hkv, D, generator=torch.Generator().manual_seed(6)).to(torch.bfloat16)
+    kernels.kv_write_q8(x.to(DEV), x.to(DEV), p["k"], p["v"], p["ks"], p["vs"],
+                        i32([[nb - 1, nb - 3, nb - 2]]), i32([0]))
+    write(c, x, x, 0, [3, 1, 2], 0, 40, "int8")
+    same({n: t[nb - 4:] for n, t in p.items()}, c)
+    assert not any(bool(t[:nb - 4].any()) for t in p.values())
+
+
+@pytest.mark.parametrize("B,T,Hkv", [(1, 1, 2), (3, 1, 2), (1, 5, 1), (2, 1, 1), (1, 1, 1)])
+def test_strides_of_dimensions_of_one_do_not_matter(B, T, Hkv):
+    """K and V rows whose strides differ in dimensions of one element only."""
+    g = torch.Generator().manual_seed(7)
+    x = torch.randn(B, T, Hkv, 64, generator=g)
+    p = {n: t.to(DEV) for n, t in pools(8, 6, Hkv, 16, 64, "e4m3").items()}
+    c = {n: t.cpu().double() for n, t in p.items()}
+    k = x.to(DEV)
+    odd = [s if n > 1 else s + 8 * (i + 1) for i, (n, s) in enumerate(zip(x.shape, x.stride()))]
+    v = k.as_strided(x.shape, odd)
+    kernels.kv_write_q8(k, v, p["k"], p["v"], p["ks"], p["vs"], i32([[1, 0], [3, 2], [5, 4]]),
+                        i32([15, 0, 3]))
+    for b, (start, table) in enumerate([(15, [1, 0]), (0, [3, 2]), (3, [5, 4])][:B]):
+        write(c, x, x, start, table, b, T, "e4m3")
+    same(p, c)

@@ -300,6 +300,53 @@ def test_a_window_of_everything_is_verify_attention(pool, dtype):
     c.check(other, None, 0)
 
 
+@pytest.mark.parametrize("pool,dtype", POOLS)
+@pytest.mark.parametrize("T", [1, 40])
+def test_scores_far_below_zero(T, pool, dtype):
+    """Scores of -2^105 and lower: the first key's is the largest by more than 2^104, so the
+    rows are its V."""
+    c = Case(13, [60], T, 4, 2, 64, pool, dtype)
+    c.q.zero_()
+    c.q[..., 0] = 2.0 ** 52
+    c.k.zero_()
+    size = 2.0 ** 56
+    if c.ks is not None:
+        c.ks[:], c.vs[:] = 2.0 ** 50, 1.0
+        size = 64.0
+    c.k[:, :, :, 0] = -1.5 * size
+    c.k[c.tables[0][0], :, 0, 0] = -size
+    got = c.run(200, 0)
+    want = c.v[c.tables[0][0], :, :, 0].float().repeat_interleave(2, 0).to(c.q.dtype)
+    assert torch.equal(got, want.expand(1, T, 4, 64))
+
+
+@pytest.mark.parametrize("pool,dtype", [("bf16", "bf16"), ("int8", "fp32")])
+def test_prompts_of_more_than_2_16_rows(pool, dtype):
+    c = Case(14, [3], 8300, 16, 2, 64, pool, dtype)
+    r = random.Random(2)
+    rows = {(0, t, h) for t in [0, 1, 4094, 4095, 4096, 8190, 8191, 8192, 8299] + r.sample(range(8300), 12)
+            for h in (0, 7, 8, 15)}
+    got = c.run(50, 3)
+    for b, t, h in rows:
+        want, bound = c.exact(b, t, h, 50, 3)
+        assert bool(((got[b, t, h].double() - want).abs() <= bound).all()), (t, h)
+
+
+def test_a_bf16_pool_past_32_bits():
+    """More than 4 GiB of K and V each, the sequences in the last blocks; 16 rows and more."""
+    nb, Hkv, D = 550_000, 2, 128
+    for T in (2, 9):
+        c = Case(15, [100, 70], T, 16, Hkv, D)
+        n = c.k.shape[0]
+        k, v = (torch.zeros(s, dtype=torch.bfloat16, device=DEV) for s in ((nb, Hkv, 16, D), (nb, Hkv, D, 16)))
+        assert k.numel() * 2 > 1 << 32
+        for big, small in ((k, c.k), (v, c.v)):
+            big[nb - n:] = small.to(DEV)
+        table = torch.where(c.table() < 0, -1, c.table() + (nb - n))
+        got = kernels.paged_window_attn(c.q.to(DEV), k, v, table, i32(c.starts), 100 + T, 64, 5).cpu()
+        c.check(got, 64, 5)
+
+
 def test_offsets_past_32_bits():
     """A pool of more than 4 GiB of codes, the sequences in its last blocks."""
     nb, Hkv, D = 1_100_000, 2, 128

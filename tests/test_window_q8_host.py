@@ -20,7 +20,8 @@ def call_attn(**kw):
     (dict(q=None), "null pointer"), (dict(out=None), "null pointer"), (dict(tables=None), "null pointer"),
     (dict(T=0), "tokens"), (dict(B=-1), "tokens"), (dict(Hq=15), "heads"), (dict(D=96), "heads"),
     (dict(Hkv=0), "heads"), (dict(window=-1), "window"), (dict(sinks=-1), "sinks"),
-    (dict(T=9363), "tokens"), (dict(bs=24), "block_size"), (dict(bs=0), "block_size"),
+    (dict(T=1 << 28), "tokens"), (dict(max_blocks=1 << 27, max_ctx=(1 << 30) + 1), "max_ctx"),
+    (dict(B=1 << 22, T=1), "too large"), (dict(bs=24), "block_size"), (dict(bs=0), "block_size"),
     (dict(bs=1 << 21), "block_size"), (dict(max_ctx=129), "max_ctx"), (dict(max_ctx=0), "max_ctx"),
     (dict(num_blocks=0), "blocks"), (dict(num_blocks=1 << 30), "too large"),
     (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
@@ -62,6 +63,7 @@ def call_write(**kw):
     (dict(D=256), "head_dim"), (dict(dtype=2), "dtype"), (dict(pool=1), "pool dtype"),
     (dict(stride=120), "stride"), (dict(stride=132), "stride"), (dict(k=8), "aligned"),
     (dict(vp=20), "aligned"), (dict(B=1 << 28, T=1 << 10), "too large"),
+    (dict(B=1 << 24, T=1), "too large"),
 ])
 def test_write_refuses(change, text):
     rc, msg = call_write(**change)
@@ -88,6 +90,7 @@ def call_logprobs(**kw):
     (dict(x=17), -1, "aligned"), (dict(x=18, dtype=0), -1, "aligned"), (dict(ws=None), -1, "workspace"),
     (dict(ws=8), -1, "16-byte"), (dict(wsb=8), -2, "workspace"),
     (dict(rows=1 << 24, V=1 << 20), -1, "too large"),
+    (dict(rows=1 << 22, wsb=1 << 40), -1, "too large"),
 ])
 def test_logprobs_refuses(change, rc, text):
     got, msg = call_logprobs(**change)
