@@ -189,27 +189,40 @@ __device__ __forceinline__ uint32_t split_bf16x2(float& a, float& b) {
   return h;
 }
 
-// The non-finite values of 16 bytes set to 0; whether there were any.
+// Whether some value of four 16-byte vectors is not finite.
 template <Pool P>
-__device__ __forceinline__ bool drop_nonfinite(u32x4& x) {
-  uint32_t any = 0;
+__device__ __forceinline__ bool any_nonfinite(const u32x4 (&x)[4]) {
+  uint32_t top = 0;  // bf16: the largest magnitudes of the halves; fp32: of all; e4m3: flags
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int i = 0; i < 16; ++i) {
+    const uint32_t w = x[i >> 2][i & 3];
     if constexpr (P == Pool::kBf16) {
-      const uint32_t f = ((x[w] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-      x[w] &= ~((f >> 15) * 0xffffu);
-      any |= f;
+      typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+      top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, w & 0x7fff7fffu),
+                                                                   __builtin_bit_cast(u16x2, top)));
     } else if constexpr (P == Pool::kF32) {
-      const bool f = (x[w] & 0x7f800000u) == 0x7f800000u;
-      x[w] = f ? 0u : x[w];
-      any |= f;
-    } else if constexpr (P == Pool::kE4m3) {
-      const uint32_t f = ((x[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-      x[w] &= ~((f >> 7) * 0xffu);
-      any |= f;
+      top = max(top, w & 0x7fffffffu);
+    } else {
+      top |= (w & 0x7f7f7f7fu) + 0x01010101u;
     }
   }
-  return any != 0;
+  if constexpr (P == Pool::kBf16) return ((top + 0x00800080u) & 0x80008000u) != 0;
+  if constexpr (P == Pool::kF32) return top >= 0x7f800000u;
+  return (top & 0x80808080u) != 0;
+}
+
+// The non-finite values of 16 bytes set to 0.
+template <Pool P>
+__device__ __forceinline__ void drop_nonfinite(u32x4& x) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if constexpr (P == Pool::kBf16)
+      x[w] &= ~(((((x[w] & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 15) * 0xffffu);
+    else if constexpr (P == Pool::kF32)
+      x[w] = (x[w] & 0x7f800000u) == 0x7f800000u ? 0u : x[w];
+    else
+      x[w] &= ~(((((x[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu);
+  }
 }
 
 // A V value if it is not finite, else 0.
@@ -253,12 +266,14 @@ __global__ __launch_bounds__(win_threads(SHARED)) __attribute__((amdgpu_waves_pe
 
   const int tid = threadIdx.x, l = tid & 63, lr = l & 15, lg = l >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // The last rows of all sequences come first: their walks are the longest, and what is left
+  // at the end is short (prompt of 4 x 4097 tokens 167 -> 160 us).
   int u = blockIdx.x;
-  const int rg = u % a.row_groups;
-  u /= a.row_groups;
   const int c = u % a.splits;
   u /= a.splits;
-  const int kvh = u % a.Hkv, b = u / a.Hkv;
+  const int kvh = u % a.Hkv;
+  u /= a.Hkv;
+  const int b = u % a.B, rg = a.row_groups - 1 - u / a.B;
   const WinSeq s = win_seq(a, b);
   const int R = a.G * s.T, g0 = rg * ROWS;
   if (g0 >= R) return;
@@ -527,6 +542,8 @@ __global__ __launch_bounds__(win_threads(SHARED)) __attribute__((amdgpu_waves_pe
     u32x4 kn[NT], vn[4];
 #pragma unroll
     for (int t = 0; t < NT; ++t) kn[t] = k_frag(0, t);
+    // (a wave in its products goes before one in its softmax: 1 % of a prompt)
+    if (SHARED) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       u32x4 kc[NT];
@@ -576,6 +593,7 @@ __global__ __launch_bounds__(win_threads(SHARED)) __attribute__((amdgpu_waves_pe
       }
       if (SHARED) __builtin_amdgcn_sched_barrier(0);
     }
+    if (SHARED) __builtin_amdgcn_s_setprio(0);
     if (SHARED) __asm__ volatile("" ::: "memory");  // the first of V stays ahead of the softmax
     if (!SHARED && i + 1 < n) load_k(i + 1, i);
     float ks = 1.0f, vs = 1.0f;
@@ -589,24 +607,34 @@ __global__ __launch_bounds__(win_threads(SHARED)) __attribute__((amdgpu_waves_pe
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       float f = Q8B ? rf[mt] * ks : rf[mt];
-      float top = -INFINITY;
-      if (whole) {
+      if (!whole) {
+        if constexpr (Q8B) {  // the exponents themselves: a masked key's scale may be no number
 #pragma unroll
-        for (int x = 0; x < 4 * NT; ++x) top = fmaxf(top, sc[mt][x >> 2][x & 3]);
-        top *= f;
-      } else {
-        // the exponents themselves, so that nothing of a masked key or its scale stays
-#pragma unroll
-        for (int x = 0; x < 4 * NT; ++x) {
-          const int key = k0 + x / (4 * NS) * SP + 4 * NS * lg + x % (4 * NS);
-          const bool sees = (key <= qpos[mt]) & ((key > qpos[mt] - a.window) | (key < a.sinks));
-          const float y = sees ? sc[mt][x >> 2][x & 3] * f : -INFINITY;
-          sc[mt][x >> 2][x & 3] = y;
-          top = fmaxf(top, y);
+          for (int x = 0; x < 4 * NT; ++x) sc[mt][x >> 2][x & 3] *= f;
+          f = 1.0f;
         }
-        f = 1.0f;
+        // key k0 + 4 NS lg + (a constant of x) against the ends of what the row sees, the
+        // window's last and its first, each where the step reaches it
+        const int at = k0 + 4 * NS * lg;
+        if (k0 + SK - 1 > p0) {
+          const int last = qpos[mt] - at;
+#pragma unroll
+          for (int x = 0; x < 4 * NT; ++x)
+            sc[mt][x >> 2][x & 3] = x / (4 * NS) * SP + x % (4 * NS) <= last ? sc[mt][x >> 2][x & 3] : -INFINITY;
+        }
+        if (k0 <= p1 - a.window) {
+          const int before = qpos[mt] - a.window - at, sunk = a.sinks - at;
+#pragma unroll
+          for (int x = 0; x < 4 * NT; ++x) {
+            const int y = x / (4 * NS) * SP + x % (4 * NS);
+            sc[mt][x >> 2][x & 3] = (y > before) | (y < sunk) ? sc[mt][x >> 2][x & 3] : -INFINITY;
+          }
+        }
       }
-      top = max_across_groups(top);
+      float top = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < 4 * NT; ++x) top = fmaxf(top, sc[mt][x >> 2][x & 3]);
+      top = max_across_groups(top * f);
       const bool grow = top > m[mt] + kLag<Q8B>;
       if (__any(grow)) {
         const float to = grow ? top : m[mt], al = __builtin_amdgcn_exp2f(m[mt] - to);
@@ -647,6 +675,7 @@ __global__ __launch_bounds__(win_threads(SHARED)) __attribute__((amdgpu_waves_pe
       }
     }
     bool dropped = false;
+    if (SHARED) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int g = 0; g < U * DT / 4; ++g) {
       const int p = g / (DT / 4), d0 = g % (DT / 4) * 4;
@@ -658,9 +687,12 @@ __global__ __launch_bounds__(win_threads(SHARED)) __attribute__((amdgpu_waves_pe
         for (int x = 0; x < 4; ++x) vn[x] = v_frag(g + 1, x);
       }
       if (SHARED) __builtin_amdgcn_sched_barrier(0);
-      if (P != Pool::kInt8 && !whole) {
+      if constexpr (P != Pool::kInt8) {
+        if (!whole && __builtin_expect(__any(any_nonfinite<P>(vc)), 0)) {
+          dropped = true;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) dropped |= drop_nonfinite<P>(vc[x]);
+          for (int x = 0; x < 4; ++x) drop_nonfinite<P>(vc[x]);
+        }
       }
       if constexpr (F32) {
 #pragma unroll
@@ -702,7 +734,8 @@ __global__ __launch_bounds__(win_threads(SHARED)) __attribute__((amdgpu_waves_pe
       }
       if (SHARED) __builtin_amdgcn_sched_barrier(0);
     }
-    if (__any(dropped)) {
+    if (SHARED) __builtin_amdgcn_s_setprio(0);
+    if (dropped) {
       // rare: the step's keys one by one, their non-finite values to the rows that see them
 #pragma unroll 1
       for (int x = 0; x < SK; ++x) {
