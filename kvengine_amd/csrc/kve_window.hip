@@ -895,7 +895,7 @@ __global__ __launch_bounds__(kMergeThreads) void window_merge_kernel(WindowArgs 
 // Waves that a launch should have before walks are cut: eight per compute unit.
 constexpr int kFillWaves = 2048;
 // Workgroups from which on a wave takes two tiles of rows.
-constexpr int kTwoTiles = 48;
+constexpr int kTwoTiles = 96;
 
 struct WindowCfg {
   int mt, rows, row_groups, chunk, splits;  // mt 0: up to 16 rows
@@ -904,15 +904,16 @@ struct WindowCfg {
 
 // Walks are not cut below `least` steps, where a chunk's own start and its part of the
 // join outweigh the steps it takes over: more than 16 rows, 1 / 2 / 4 / 8 steps, bf16 (32 x 5
-// rows, window 1024) 18.9 / 19.0 / 19.4 / 22.8 us, 8-bit (16 x 5) 20.4 / 20.4 / 18.4 / 23.9, fp32
-// pools, bound by their products, 11.7 / 14.0 / 19.2 / 26.2. Up to 16 rows, 8 / 16 / 32 steps: 8 long
-// histories in bf16 18.1 / 20.9 / 28.5, 32 under a window of 1024 15.2 / 19.5 / 18.2; where
-// all waves are done in two turns, the join costs more than it gains (1000 keys 9.7 us, 8.7
+// tokens, window 1024) 16.8 / 16.9 / 17.1 / 20.0 us, 8-bit (16 x 5) 19.5 / 19.5 / 18.0 / 22.5, fp32
+// pools, bound by their products, 11.2 / 12.9 / 17.8 / 23.1. Up to 16 rows, 8 / 16 / 32 steps: 8 long
+// histories in bf16 17.9 / 20.5 / 28.3, 32 under a window of 1024 14.8 / 19.2 / 17.7; where
+// all waves are done in two turns, the join costs more than it gains (1000 keys 9.5 us, 8.4
 // in one piece). Eight waves for four: 32 long 8-bit histories 28.3 -> 25.9 us.
 // Two tiles a wave halve the LDS reads per product and pay where the workgroups fill the chip
-// all the same (bf16, 1 / 2 tiles: prompts 291 / 191 us, 32 x 9 rows 25.5 / 23.0, 4 x 33 17.5 /
-// 19.8, 1 x 100 18.4 / 21.4); fp32 queries, bound by products or registers, keep one
-// (prompt of 1025 242 / 275 us).
+// all the same (1 / 2 tiles, bf16: 4 x 4097 tokens 232 / 153 us, 48 x 9 28.0 / 24.9, 32 x 9
+// 19.5 / 20.6, 16 x 17 21.1 / 23.1, 4 x 33 14.7 / 18.4; 8-bit: 32 x 17 48.0 / 43.0, 16 x 17
+// 26.1 / 30.1); fp32 queries, bound by products or registers, keep one (prompt of 1025
+// 242 / 275 us).
 static WindowCfg window_cfg(int B, int Tq, int Hq, int Hkv, int D, int max_ctx, int window,
                             int sinks, int elem_bytes, bool f32) {
   WindowCfg c{};

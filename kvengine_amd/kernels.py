@@ -1189,7 +1189,18 @@ def kv_write_q8(k_new: torch.Tensor, v_new: torch.Tensor, k_layer: torch.Tensor,
           bs, max_blocks, num_rows, NB, code, pool)
 
 
-_WINDOW_WS: dict[tuple, int] = {}  # workspace bytes by sizes
+_WS_BYTES: dict[tuple, int] = {}  # by sizes
+
+
+def _ws_bytes(what: str, *sizes) -> int:
+    """What the library's function of this name says for these sizes."""
+    key = (what, sizes)
+    n = _WS_BYTES.get(key)
+    if n is None:
+        if len(_WS_BYTES) >= 4096:  # (max_ctx grows with every step)
+            _WS_BYTES.clear()
+        n = _WS_BYTES[key] = getattr(_lib.lib(), what)(*sizes)
+    return n
 
 
 def _window_attn(q, k_layer, v_layer, k_scale, v_scale, block_tables, start_pos, max_ctx, window,
@@ -1217,12 +1228,7 @@ def _window_attn(q, k_layer, v_layer, k_scale, v_scale, block_tables, start_pos,
     lib = _lib.lib()
     # (a window of 2^30 tokens sees what none does)
     window, sinks = min(window, 1 << 30), min(sinks, 1 << 30)
-    key = (B, T, Hq, Hkv, D, max_ctx, window, sinks, code, pool)
-    nbytes = _WINDOW_WS.get(key)
-    if nbytes is None:
-        if len(_WINDOW_WS) >= 4096:  # (max_ctx grows with every step)
-            _WINDOW_WS.clear()
-        nbytes = _WINDOW_WS[key] = lib.kve_window_workspace_bytes(*key)
+    nbytes = _ws_bytes("kve_window_workspace_bytes", B, T, Hq, Hkv, D, max_ctx, window, sinks, code, pool)
     # the call's own, so that captured graphs share none
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _call(lib.kve_paged_window_attn, "kve_paged_window_attn", dev, q.data_ptr(), k_layer.data_ptr(),
@@ -1282,18 +1288,19 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0):
     R, V = logits.shape
     stride, one = logits.stride()
     _need(one == 1 or V == 1, "logits need a contiguous vocabulary")
-    _check_on(tokens, "tokens", torch.int32, (R,), dev)
+    if not _fits(tokens, torch.int32, (R,), dev.index):
+        _check_on(tokens, "tokens", torch.int32, (R,), dev)
     if not 0 <= top <= min(LOGPROBS_MAX_TOP, V):
         raise ValueError(f"{top} alternatives of {V} ids, at most {LOGPROBS_MAX_TOP}")
     code = _dtype_code(logits)
     logprobs = torch.empty(R, dtype=torch.float32, device=dev)
-    entropy = torch.empty(R, dtype=torch.float32, device=dev)
+    entropy = torch.empty_like(logprobs)
     ids = torch.empty((R, top), dtype=torch.int32, device=dev)
-    tops = torch.empty((R, top), dtype=torch.float32, device=dev)
+    tops = torch.empty_like(ids, dtype=torch.float32)
     if R == 0:
         return logprobs, entropy, ids, tops
     lib = _lib.lib()
-    nbytes = lib.kve_logprobs_workspace_bytes(R, V, top, code)
+    nbytes = _ws_bytes("kve_logprobs_workspace_bytes", R, V, top, code)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _call(lib.kve_token_logprobs, "kve_token_logprobs", dev, logits.data_ptr(), stride,
           tokens.data_ptr(), R, V, top, code, logprobs.data_ptr(), entropy.data_ptr(),
