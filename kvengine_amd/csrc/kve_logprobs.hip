@@ -14,6 +14,10 @@
 // by logit, equal ones lowest first. The n likeliest ids lie in the n groups whose maxima
 // rank first (an id of another group has n group maxima before it), so the row is read
 // again in those groups alone.
+//
+// What bounds it, at 151936 ids in bf16. 160 rows and 20 alternatives: statistics 13.5 us (3.6
+// TB/s), the row's workgroup 10, two selections one after another with their dependent reads
+// (taking the largest n times 60 more). One row: 3.5 and 7.8, launches and round trips.
 
 #include "kve_logits.h"
 
