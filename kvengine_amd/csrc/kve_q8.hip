@@ -15,9 +15,9 @@
 // by two lane swaps, so that a lane stores 16 tokens of a channel at once.
 //
 // What bounds it: one decode step is launch and three dependent reads (length, block id, scale
-// and held codes): 32 sequences of 2 heads of 128 5.4 us. A prompt is bytes: 8 x 2049 tokens 9.0 us,
-// 2.8 TB/s (a workgroup a block with its codes turned in LDS 18); a tile's reads, its maximum and
-// its stores follow one another.
+// and held codes): 32 sequences of 2 heads of 128 5.4 us. A prompt is bytes: 8 x 2049 tokens 9.0
+// us, 2.8 TB/s; a tile's reads, its maximum and its stores follow one another (18 with a workgroup
+// a tile, whose waves meet for the maximum and whose reads of V jump from token to token).
 
 #include "kve_q8.h"
 

@@ -137,9 +137,9 @@ def score_tokens(model, input_ids: torch.Tensor, cache, top: int = 0):
     (logprobs [T - 1], entropy [T - 1], top_ids [T - 1, top], top_logprobs [T - 1, top]).
     The mean of -logprobs over one text, with the cache in the model's type and in 8 bits or
     with and without a window, is what either costs."""
+    if input_ids.dim() != 2 or input_ids.shape[0] != 1 or input_ids.shape[1] < 2:
+        raise ValueError(f"input_ids {list(input_ids.shape)}: one text of two tokens or more")
     T = input_ids.shape[1]
-    if T < 2:
-        raise ValueError(f"{T} tokens: the first one has no probability")
     hidden = forward_with_own_cache(model, input_ids, cache, all_logits=True, return_hidden=True)[0]
     nxt = input_ids[0, 1:].to(device=hidden.device, dtype=torch.int32).contiguous()
     parts = []

@@ -263,7 +263,7 @@ def forward_hidden(model, input_ids: torch.Tensor, kv: DeviceKV, rows: torch.Ten
     kernels.tree_accept picks the path and makes its K/V consecutive.
 
     Layers whose self_attn.sliding_window is set attend to that many latest tokens and
-    the first self_attn.window_sinks; an 8-bit pool (PagedKVCache of int8 or
+    the first self_attn.window_sinks (blocks of a multiple of 16 tokens); an 8-bit pool (PagedKVCache of int8 or
     float8_e4m3fn) is written with kernels.kv_write_q8. Both run the library-GEMM layer,
     whose attention order is its own (attn_order and gemm_rows do not apply).
     """

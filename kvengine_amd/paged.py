@@ -406,19 +406,22 @@ class ContiguousKVCache:
     Stored as a single block of max_seq_len tokens in the kernel layout, so the
     same attention and KV-write kernels serve it (block table [[0]]).
     `truncate` only moves the length; stale positions are never read.
+    room: tokens that the block has place for (default max_seq_len); windowed
+    attention wants a multiple of 16.
     """
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, max_seq_len: int,
-                 dtype: torch.dtype, device):
+                 dtype: torch.dtype, device, room: int | None = None):
         self.num_layers = num_layers
         self.num_kv_heads = num_kv_heads
         self.head_dim = head_dim
         self.max_seq_len = max_seq_len
         self.dtype = dtype
         self.device = torch.device(device)
-        self.k = torch.zeros((num_layers, 1, num_kv_heads, max_seq_len, head_dim), dtype=dtype,
+        self.room = max_seq_len if room is None else room
+        self.k = torch.zeros((num_layers, 1, num_kv_heads, self.room, head_dim), dtype=dtype,
                              device=self.device)
-        self.v = torch.zeros((num_layers, 1, num_kv_heads, head_dim, max_seq_len), dtype=dtype,
+        self.v = torch.zeros((num_layers, 1, num_kv_heads, head_dim, self.room), dtype=dtype,
                              device=self.device)
         self.tables = torch.zeros((1, 1), dtype=torch.int32, device=self.device)
         self.lens = torch.zeros(1, dtype=torch.int32, device=self.device)
@@ -430,8 +433,10 @@ class ContiguousKVCache:
     def for_model(cls, model, max_seq_len: int) -> "ContiguousKVCache":
         info = _model_info(model)
         p = next(model.parameters())
+        from .forward import windowed
+        room = -(-max_seq_len // 16) * 16 if windowed(model) else None
         return cls(info["num_layers"], info["num_key_value_heads"], info["head_dim"], max_seq_len,
-                   p.dtype, p.device)
+                   p.dtype, p.device, room)
 
     @property
     def length(self) -> int:
@@ -459,7 +464,7 @@ class ContiguousKVCache:
         self.lens.fill_(0)
 
     def device_kv(self) -> DeviceKV:
-        return DeviceKV(self.k, self.v, self.tables, self.lens, self.max_seq_len)
+        return DeviceKV(self.k, self.v, self.tables, self.lens, self.room)
 
     def reserve(self, n_tokens: int) -> None:
         if self._length + n_tokens > self.max_seq_len:

@@ -21,7 +21,7 @@ import torch
 
 from kvengine_amd import kernels
 from kvengine_amd.arch import TINY, TINY128
-from kvengine_amd.decode import greedy_paged, score_tokens
+from kvengine_amd.decode import greedy_own_cache, greedy_paged, score_tokens
 from kvengine_amd.forward import forward_hidden, forward_packed, forward_with_own_cache
 from kvengine_amd.model import build_model
 from kvengine_amd.paged import ContiguousKVCache, PagedKVCache
@@ -107,9 +107,10 @@ def test_a_windowed_model(arch, window, sinks, dtype, fused):
     pool = PagedKVCache.for_model(model, 16)
     got = passes(model, ids, pool.new_sequence("a"), [90, 91, 92, 97, 130])
     close(got, reference(model, ids[0]), dtype)
-    # the contiguous cache, one block of a multiple of 16 tokens
-    got = passes(model, ids, ContiguousKVCache.for_model(model, 160), [149])
-    close(got, reference(model, ids[0]), dtype)
+    # the contiguous cache, of any capacity
+    for room in (160, 151):
+        got = passes(model, ids, ContiguousKVCache.for_model(model, room), [149])
+        close(got, reference(model, ids[0]), dtype)
 
 
 @pytest.mark.parametrize("pool_dtype", Q8)
@@ -204,6 +205,14 @@ def test_speculative_decoding(pool_dtype, window, dtype):
     assert runs[0] == runs[1]
 
 
+def test_greedy_decoding_over_either_cache():
+    model = model_of(TINY, torch.float32, 9, 2)
+    ids = prompt(21).to(DEV)
+    a = greedy_own_cache(model, ids, max_new_tokens=14, eos_token_id=None)
+    b = greedy_paged(model, ids, PagedKVCache.for_model(model, 8), max_new_tokens=14, eos_token_id=None)
+    assert len(a.new_token_ids) == 14 and a.new_token_ids == b.new_token_ids
+
+
 def test_windows_set_between_calls_are_seen():
     """The same models and pools, other windows: captured iterations of the first call do not
     serve the second."""
@@ -268,8 +277,9 @@ def test_refusals():
             SpecEngine(*pair, k=2, slots=2, t_blocks=16, d_blocks=16)
     with pytest.raises(ValueError):
         PagedKVCache.for_model(plain, 16, block_size=8, dtype=torch.int8)
-    with pytest.raises(ValueError):
-        score_tokens(plain, prompt(1).to(DEV), PagedKVCache.for_model(plain, 4).new_sequence("s"))
+    for ids in (prompt(1), prompt(8).view(2, 4), prompt(4)[0]):
+        with pytest.raises(ValueError):
+            score_tokens(plain, ids.to(DEV), PagedKVCache.for_model(plain, 4).new_sequence("s"))
 
 
 @pytest.mark.parametrize("pool_dtype", Q8)
