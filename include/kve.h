@@ -285,6 +285,7 @@ int kve_kv_write_q8(const void* k_new, const void* v_new, int64_t src_token_stri
  * pool_dtype: dtype, KVE_DTYPE_I8 or KVE_DTYPE_E4M3 (k_scale, v_scale as above; else NULL)
  * block_size % 16 == 0, head_dim 64 or 128, max_ctx and num_q_heads / num_kv_heads * q_len at most 2^30,
  * scale > 0; q, pools, out and workspace 16-byte aligned
+ * sinks: any number of 0 and more (INT32_MAX: every key, as window 0)
  * workspace: kve_window_workspace_bytes(...) bytes (0: none needed), no initialisation
  */
 size_t kve_window_workspace_bytes(int num_seqs, int q_len, int num_q_heads, int num_kv_heads,

@@ -1083,7 +1083,8 @@ extern "C" int kve_paged_window_attn(const void* q, const void* k_layer, const v
   a.num_blocks = num_blocks;
   a.max_ctx = max_ctx;
   a.window = win;
-  a.sinks = sinks;
+  // (no more than there are keys: the walk rounds them up to whole steps in 32 bits)
+  a.sinks = std::min(sinks, max_ctx);
   a.row_groups = c.row_groups;
   a.chunk = c.chunk;
   a.splits = c.splits;
