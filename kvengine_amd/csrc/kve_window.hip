@@ -36,8 +36,8 @@
 // part costs a third of them; a prompt's outputs then lie 2.1e-3 from 64 bits instead of 1.6e-3,
 // which is the output's own rounding. fp32: fp32 products. 8 bits: codes are exact in
 // fp16, so the products are fp16's: q is scaled to the fp16 range by a power of two per row
-// (exact for bf16; fp32 as the sum of two fp16, 22 bits), P s_v by one per walk (11 bits of
-// it for bf16 queries, 22 for fp32). Sums, m and l are fp32.
+// (exact for bf16; fp32 as the sum of two fp16, 22 bits), P s_v by one per row that follows its
+// largest product (11 bits of it for bf16 queries, 22 for fp32). Sums, m and l are fp32.
 //
 // Values that a row must not see. A masked score is replaced, not added to, so that nothing
 // of its key remains. In V a masked infinity or NaN would be 0 * inf: steps that some
@@ -249,9 +249,8 @@ __device__ __forceinline__ float nonfinite_of(const uint8_t* p) {
 constexpr int kRingBytes = 64 * 1024;
 
 // How far a row's maximum may lag behind its scores (in powers of 2) before its state is
-// rescaled: P stays below 2^8 in fp32 and bf16, below 2^15 in fp16.
-template <bool F16>
-constexpr float kLag = F16 ? 1.0f : 8.0f;
+// rescaled: P stays below 2^8.
+constexpr float kLag = 8.0f;
 
 // QP: fp16 parts that q is taken as over 8-bit pools (1: bf16 queries, 2: fp32; else 1).
 // PP: 16-bit parts of P (fp32 pools: 1, whole).
@@ -479,27 +478,15 @@ __global__ __launch_bounds__(win_threads(SHARED)) __attribute__((amdgpu_waves_pe
     m[mt] = kNone;
     lsum[mt] = 0.0f;
   }
-  // 8-bit: acc is in units of ref 2^-14, ref a power of two that no s_v of a tile seen so far
-  // exceeds
-  float ref = kMinScale;
-  const auto raise_ref = [&](int i) {  // the batch that starts at step i has become the current one
-    const int k0 = tile_of(i) * 16;
-    const bool seen = k0 + 15 > w.p0 - a.window || k0 < a.sinks;
-    float top = seen && vsl < INFINITY ? vsl : 0.0f;
+  // 8-bit: a row's acc is in units of ref 2^-14, ref above every P s_v that it has met, in units
+  // of its present maximum. By row and from P, not from the scales of the walk's blocks: a
+  // block that a row does not see, or gives no weight, takes no bits from the others.
+  float ref[MT], per_ref[MT];  // per_ref = 2^14 / ref
 #pragma unroll
-    for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
-    top = max_across_groups(top);
-    if (top > ref) {  // (the same in every lane)
-      const float to = ldexpf(1.0f, min(__builtin_amdgcn_frexp_expf(top), 127)), f = ref / to;
-      ref = to;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) acc[mt][dt] *= f;
-      }
-    }
-  };
-  if (Q8B && n > 0) raise_ref(0);
+  for (int mt = 0; mt < MT; ++mt) {
+    ref[mt] = kMinScale;
+    per_ref[mt] = 0x1p14f / kMinScale;
+  }
 
   for (int i = 0; i < n; ++i) {
     if (n > BATCH && i % (BATCH / 2) == 0) {
@@ -508,7 +495,6 @@ __global__ __launch_bounds__(win_threads(SHARED)) __attribute__((amdgpu_waves_pe
           ids = ids1;
           ksl = ks1;
           vsl = vs1;
-          if (Q8B) raise_ref(i);
           if (i + BATCH < n) raw1 = read_table(i + BATCH);
         }
       } else if (i + BATCH / 2 < n) {
@@ -608,7 +594,7 @@ __global__ __launch_bounds__(win_threads(SHARED)) __attribute__((amdgpu_waves_pe
     float ks = 1.0f, vs = 1.0f;
     if constexpr (Q8B) {
       ks = __shfl(ksl, i % BATCH * NT + lg);
-      vs = __shfl(vsl, i % BATCH * NT + lg) * (0x1p14f / ref);
+      vs = __shfl(vsl, i % BATCH * NT + lg);
     }
     // seen whole by every row of the wave
     const bool whole = k0 + SK - 1 <= p0 && (k0 > p1 - a.window || k0 + SK <= a.sinks);
@@ -643,14 +629,35 @@ __global__ __launch_bounds__(win_threads(SHARED)) __attribute__((amdgpu_waves_pe
       float top = -INFINITY;
 #pragma unroll
       for (int x = 0; x < 4 * NT; ++x) top = fmaxf(top, sc[mt][x >> 2][x & 3]);
+      const float own = top;  // of the lane's keys, in 8 bits those of one tile
       top = max_across_groups(top * f);
-      const bool grow = top > m[mt] + kLag<Q8B>;
+      const bool grow = top > m[mt] + kLag;
       if (__any(grow)) {
         const float to = grow ? top : m[mt], al = __builtin_amdgcn_exp2f(m[mt] - to);
         m[mt] = to;
         lsum[mt] *= al;
+        if constexpr (Q8B) {
+          ref[mt] *= al;
+        } else {
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) acc[mt][dt] *= al;
+          for (int dt = 0; dt < DT; ++dt) acc[mt][dt] *= al;
+        }
+      }
+      float unit = 1.0f;
+      if constexpr (Q8B) {
+        // the lane's largest P s_v; P counts as 2^-100 at the least, which keeps s_v / ref in range
+        const float p = __builtin_amdgcn_exp2f(fmaf(own, f, -m[mt]));
+        const bool number = fabsf(vs) < INFINITY;  // (what is none goes its own way)
+        const float most = max_across_groups(p > 0.0f && number ? fabsf(vs) * fmaxf(p, 0x1p-100f) : 0.0f);
+        if (__any(grow || most >= ref[mt])) {
+          const float was = ref[mt];
+          ref[mt] = fminf(fmaxf(most >= was ? 2.0f * most : was, kMinScale), 0x1p127f);
+          per_ref[mt] = 0x1p14f / ref[mt];
+          const float al = was / ref[mt];
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) acc[mt][dt] *= al;
+        }
+        unit = p > 0.0f || !number ? vs * per_ref[mt] : 0.0f;
       }
       float x[4 * NT];
       float add = 0.0f;
@@ -663,7 +670,7 @@ __global__ __launch_bounds__(win_threads(SHARED)) __attribute__((amdgpu_waves_pe
       if constexpr (Q8B) {
         // (0 * s_v of a block whose scale is no number stays 0)
 #pragma unroll
-        for (int e = 0; e < 4 * NT; ++e) x[e] = whole || x[e] != 0.0f ? x[e] * vs : 0.0f;
+        for (int e = 0; e < 4 * NT; ++e) x[e] = whole || x[e] != 0.0f ? x[e] * unit : 0.0f;
       }
       if constexpr (F32) {
 #pragma unroll
@@ -773,7 +780,7 @@ __global__ __launch_bounds__(win_threads(SHARED)) __attribute__((amdgpu_waves_pe
     lsum[mt] = sum_across_groups(lsum[mt]);
     if constexpr (Q8B) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) acc[mt][dt] *= ref * 0x1p-14f;
+      for (int dt = 0; dt < DT; ++dt) acc[mt][dt] *= ref[mt] * 0x1p-14f;
     }
   }
 
