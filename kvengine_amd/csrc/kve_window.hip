@@ -31,13 +31,15 @@
 // as an operand of O^T = V^T P^T without leaving the lane. A direct load writes its 64 lanes'
 // 16 bytes one after another, so a fragment is read back from LDS without bank conflicts.
 //
-// Numbers. bf16: products in bf16, P as the sum of two bf16 (16 bits of it), but as one (8
-// bits) where a wave has two tiles: there matrix products bound the pass, and the second
-// part costs a third of them; a prompt's outputs then lie 2.1e-3 from 64 bits instead of 1.6e-3,
-// which is the output's own rounding. fp32: fp32 products. 8 bits: codes are exact in
-// fp16, so the products are fp16's: q is scaled to the fp16 range by a power of two per row
-// (exact for bf16; fp32 as the sum of two fp16, 22 bits), P s_v by one per row that follows its
-// largest product (11 bits of it for bf16 queries, 22 for fp32). Sums, m and l are fp32.
+// Numbers. bf16: products in bf16, P as the sum of two bf16 (16 bits of it; with one, 8 bits, a
+// prompt takes 160 us for 190, but its outputs lie 2.16e-3 from 64 bits instead of the 1.62e-3
+// that the output's own rounding makes). fp32: fp32 products. 8 bits: codes are exact in fp16, so
+// the products are fp16's: q is scaled to the fp16 range by a power of two per row (exact for
+// bf16; fp32 as the sum of two fp16, 22 bits), P s_v by a factor per row that follows its largest
+// product. For fp32 queries it has two fp16 (22 bits), for bf16 ones one (11 bits): outputs lie
+// 1.666e-3 from 64 bits either way at 1000 keys, 1.645e-3 and 1.643e-3 in 16 x 5 rows, and two cost
+// 4 % of a decode step (32 long histories 26.2 / 27.3 us) and 12 % of a prompt. Sums, m and l
+// are fp32.
 //
 // Values that a row must not see. A masked score is replaced, not added to, so that nothing
 // of its key remains. In V a masked infinity or NaN would be 0 * inf: steps that some
@@ -970,12 +972,10 @@ static void launch_walk(const WindowArgs& a, hipStream_t st) {
 
 template <Pool P, int QP, int PP, int D>
 static int launch_window(const WindowArgs& a, const WindowCfg& c, hipStream_t st) {
-  // bf16 pools: one part of P from two tiles a wave on
-  constexpr int PM = P == Pool::kBf16 ? 1 : PP;
   constexpr bool kTwo = P != Pool::kF32 && QP == 1;  // bf16 queries
   if (c.mt == 0) launch_walk<P, QP, PP, D, 1, false>(a, st);
   else if (c.mt == 1) launch_walk<P, QP, PP, D, 1, true>(a, st);
-  else if constexpr (kTwo) launch_walk<P, QP, PM, D, 2, true>(a, st);
+  else if constexpr (kTwo) launch_walk<P, QP, PP, D, 2, true>(a, st);
   if (c.splits > 1) {
     constexpr bool bf = P == Pool::kBf16 || (PoolOf<P, D>::Q8B && QP == 1);
     const int64_t rows = static_cast<int64_t>(a.B) * a.Hkv * a.G * a.Tq;
