@@ -912,8 +912,8 @@ __global__ __launch_bounds__(kMergeThreads) void window_merge_kernel(WindowArgs 
 
 // Waves that a launch should have before walks are cut: eight per compute unit.
 constexpr int kFillWaves = 2048;
-// Workgroups from which on a wave takes two tiles of rows.
-constexpr int kTwoTiles = 96;
+// Workgroups from which on a wave takes two tiles of rows: two for each compute unit.
+constexpr int kTwoTiles = 512;
 
 struct WindowCfg {
   int mt, rows, row_groups, chunk, splits;  // mt 0: up to 16 rows
@@ -927,16 +927,22 @@ struct WindowCfg {
 // histories in bf16 17.9 / 20.5 / 28.3, 32 under a window of 1024 14.8 / 19.2 / 17.7; where
 // all waves are done in two turns, the join costs more than it gains (1000 keys 9.5 us, 8.4
 // in one piece). Eight waves for four: 32 long 8-bit histories 28.3 -> 25.9 us.
-// Two tiles a wave halve the LDS reads per product and pay where the workgroups fill the chip
-// all the same (1 / 2 tiles, bf16: 4 x 4097 tokens 232 / 153 us, 48 x 9 28.0 / 24.9, 32 x 9
-// 19.5 / 20.6, 16 x 17 21.1 / 23.1, 4 x 33 14.7 / 18.4; 8-bit: 32 x 17 48.0 / 43.0, 16 x 17
-// 26.1 / 30.1); fp32 queries, bound by products or registers, keep one (prompt of 1025
-// 242 / 275 us).
+// Two tiles a wave halve the LDS reads per product and pay where workgroups of twice the rows
+// still fill the chip, two a compute unit, and few of their rows are empty. 1 / 2 tiles, window
+// 1024, 16 query heads of 128, by workgroups of 128 rows: prompts in bf16 152 18 / 32 us, 258 36 /
+// 40, 376 39 / 43, 516 55 / 51, 656 58 / 49, 1032 103 / 89, 2056 227 / 188; 8-bit 258 42 / 51, 376
+// 48 / 54, 516 71 / 60, 1032 123 / 105, 2056 270 / 212; 9 tokens a sequence in bf16 128 30 / 31, 192
+// 36 / 43, 384 57 / 59, 512 75 / 63, 1024 147 / 115 (at 96 alone, where one round of workgroups is as
+// long as the longest walk, 28 / 26). With 264 rows, which take 384 for
+// 320, 768 workgroups 84 / 93, with 520, 640 for 576, 640 workgroups 77 / 84. fp32 queries, bound by products or registers,
+// keep one (prompt of 1025 242 / 275 us).
 static WindowCfg window_cfg(int B, int Tq, int Hq, int Hkv, int D, int max_ctx, int window,
                             int sinks, int elem_bytes, bool f32) {
   WindowCfg c{};
   const int R = Hq / Hkv * Tq, sk = step_keys(elem_bytes, D);
-  const bool two = !f32 && R > 64 && static_cast<int64_t>(B) * Hkv * cdiv(R, 128) >= kTwoTiles;
+  const int t64 = cdiv(R, 64), t128 = cdiv(R, 128);  // workgroups of 64 rows, of 128
+  const bool two = !f32 && R > 64 && static_cast<int64_t>(B) * Hkv * t128 >= kTwoTiles &&
+                   2 * t128 <= t64 + t64 / 16;
   c.mt = R <= 16 ? 0 : two ? 2 : 1;
   c.rows = c.mt ? 64 * c.mt : 16;
   c.row_groups = cdiv(R, c.rows);
