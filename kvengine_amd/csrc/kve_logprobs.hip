@@ -238,12 +238,12 @@ __device__ __forceinline__ void select_largest(Select& sm, int n, int count, int
       if (above < n) found(above, mine);
     }
   } else {
-    uint64_t under = ~0ull;
+    uint64_t under = ~0ull;  // (also the key of a NaN at place 0: the first turn takes any)
     for (int x = 0; x < n; ++x) {
       uint64_t best = 0;
       for (int i = tid; i < count; i += kFinishThreads) {
         const uint64_t k = key(i);
-        if (k < under) best = umax64(best, k);
+        if (x == 0 || k < under) best = umax64(best, k);
       }
       best = max_across_groups_u64(row_reduce64(best, umax64));
       __syncthreads();
