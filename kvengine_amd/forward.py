@@ -131,16 +131,23 @@ def _window(attn) -> tuple[int | None, int]:
     return getattr(attn, "sliding_window", None), getattr(attn, "window_sinks", 0)
 
 
+def _attns(model):
+    """The attention module of each layer; none for a model without layers."""
+    for layer in getattr(getattr(model, "model", None), "layers", ()):
+        # (nn.Module's lookup of a submodule costs a microsecond a layer; a layer in a wrapper
+        # that forwards attributes has no such submodule)
+        attn = getattr(layer, "_modules", {}).get("self_attn")
+        yield getattr(layer, "self_attn", None) if attn is None else attn
+
+
 def windows(model) -> tuple:
     """(sliding_window, sinks) of each layer."""
-    return tuple(_window(layer.self_attn) for layer in model.model.layers)
+    return tuple(map(_window, _attns(model)))
 
 
 def windowed(model) -> bool:
     """Some layer of the model has a sliding window."""
-    # (nn.Module's lookup of a submodule costs a microsecond a layer)
-    return any(getattr(layer._modules["self_attn"], "sliding_window", None) is not None
-               for layer in model.model.layers)
+    return any(getattr(attn, "sliding_window", None) is not None for attn in _attns(model))
 
 
 def _q_heads(model, kv: DeviceKV) -> int:

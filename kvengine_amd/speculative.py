@@ -142,7 +142,7 @@ class _IterationGraphs:
         # tables were replaced since the capture gets new graphs; so does one
         # whose windows were set since, which the launches hold by value
         key = (id(target), id(draft), id(tp), id(dp), k, _addresses(target), _addresses(draft),
-               _windows(target), _windows(draft),
+               windows(target), windows(draft),
                tuple(None if t is None else t.data_ptr() for p in (tp, dp)
                      for t in (p.tables, p.lens, p.k, p.v, getattr(p, "k_scale", None),
                                getattr(p, "v_scale", None))))
@@ -263,11 +263,6 @@ def _addresses(model) -> int:
             if isinstance(t, torch.Tensor):
                 ptrs.append(t.data_ptr())
     return hash(tuple(ptrs))
-
-
-def _windows(model) -> tuple:
-    """windows() of a model with layers."""
-    return windows(model) if hasattr(model, "model") else ()
 
 
 def _feed(model, cache, ids: torch.Tensor) -> torch.Tensor:
