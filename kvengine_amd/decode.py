@@ -139,6 +139,10 @@ def score_tokens(model, input_ids: torch.Tensor, cache, top: int = 0):
     with and without a window, is what either costs."""
     if input_ids.dim() != 2 or input_ids.shape[0] != 1 or input_ids.shape[1] < 2:
         raise ValueError(f"input_ids {list(input_ids.shape)}: one text of two tokens or more")
+    w = lm_head_weight(model)
+    most = kernels.LOGPROBS_MAX_TOP if w is None else min(kernels.LOGPROBS_MAX_TOP, w.shape[0])
+    if not 0 <= top <= most:  # (before the cache takes the text)
+        raise ValueError(f"{top} alternatives, at most {most}")
     T = input_ids.shape[1]
     hidden = forward_with_own_cache(model, input_ids, cache, all_logits=True, return_hidden=True)[0]
     nxt = input_ids[0, 1:].to(device=hidden.device, dtype=torch.int32).contiguous()
