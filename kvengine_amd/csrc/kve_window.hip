@@ -914,6 +914,8 @@ __global__ __launch_bounds__(kMergeThreads) void window_merge_kernel(WindowArgs 
 constexpr int kFillWaves = 2048;
 // Workgroups from which on a wave takes two tiles of rows: two for each compute unit.
 constexpr int kTwoTiles = 512;
+// Tokens of history by whose whole numbers the cut of a walk follows max_ctx.
+constexpr int kCtxStep = 256;
 
 struct WindowCfg {
   int mt, rows, row_groups, chunk, splits;  // mt 0: up to 16 rows
@@ -946,18 +948,21 @@ static WindowCfg window_cfg(int B, int Tq, int Hq, int Hkv, int D, int max_ctx, 
   c.mt = R <= 16 ? 0 : two ? 2 : 1;
   c.rows = c.mt ? 64 * c.mt : 16;
   c.row_groups = cdiv(R, c.rows);
-  // the longest walk: the window of a workgroup's first query to its last
-  const int64_t keys =
-      std::min<int64_t>(max_ctx, static_cast<int64_t>(window) + cdiv(c.rows, Hq / Hkv) + 1);
-  int64_t steps = keys / sk + 2;
-  if (keys < max_ctx) steps += cdiv(std::min(sinks, max_ctx), sk);
+  // the longest walk: the window of a workgroup's first query to its last, and the sinks; or all keys
+  const int64_t in_window = (static_cast<int64_t>(window) + cdiv(c.rows, Hq / Hkv) + 1) / sk + 2 +
+                            (static_cast<int64_t>(sinks) + sk - 1) / sk;
+  // max_ctx decides where walks are cut by what it is in whole kCtxStep: a pass gives the same bits
+  // under every bound from one to the next
+  const int64_t in_all = static_cast<int64_t>(cdiv(max_ctx, kCtxStep)) * (kCtxStep / sk);
+  const int64_t longest = std::min(in_window, in_all);
   const int waves = c.mt == 0 ? kKeyWaves : 4;
   int64_t least = c.mt == 0 ? kKeyWaves : elem_bytes == 4 ? 1 : 4;
-  if (c.mt == 0 && steps <= 2 * kKeyWaves + 1) least = steps;
+  if (c.mt == 0 && (in_window <= 2 * kKeyWaves + 1 || in_all <= 2 * kKeyWaves)) least = longest;
   const int64_t units = static_cast<int64_t>(B) * Hkv * c.row_groups;
   const int64_t want = std::max<int64_t>(1, kFillWaves / waves / units);
-  int64_t chunk = std::max<int64_t>((steps + want - 1) / want, least);
+  int64_t chunk = std::max<int64_t>((longest + want - 1) / want, least);
   if (c.mt == 0) chunk = (chunk + kKeyWaves - 1) / kKeyWaves * kKeyWaves;
+  const int64_t steps = std::min<int64_t>(in_window, cdiv(max_ctx, sk));
   c.splits = static_cast<int>((steps + chunk - 1) / chunk);
   c.chunk = static_cast<int>(chunk);
   if (c.splits > 1) {

@@ -32,7 +32,9 @@ one reserve per pass), the graph commits and rolls back the device lengths and
 tables, and the host applies the same commits and truncates to its own
 bookkeeping afterwards. The context bucket keeps each pass's attention
 summation order (the automatic order depends on the bound only through whether
-it passes 896 tokens), so a replayed iteration gives the eager iteration's bits.
+it passes 896 tokens; that of windowed and 8-bit attention through the bound
+rounded up to 256 tokens, and not at all up to 1024), so a replayed iteration
+gives the eager iteration's bits.
 """
 
 from __future__ import annotations
@@ -46,7 +48,7 @@ import torch
 from . import kernels
 from .capture import no_gc
 from .decode import AUTO_EOS, _resolve_eos, _sync, argmax_rows
-from .forward import forward_hidden, windows
+from .forward import forward_hidden, windowed, windows
 from .model import lm_head_weight
 from .paged import PagedSequenceCache
 
@@ -96,7 +98,9 @@ class SpecDecodeResult:
 # Context bucket of the replayed iterations: the automatic attention order of a
 # pass depends on its bound only through whether it exceeds one unit record
 # (56 blocks of 16 tokens), so a bucket on the same side of that bound as every
-# pass's exact bound (start + tokens) sums every row as the eager pass does.
+# pass's exact bound (start + tokens) sums every row as the eager pass does. A
+# pass of windowed or 8-bit attention sums its rows alike under all bounds up to
+# 1024, and from one multiple of 256 to the next: CTX_STEP is the bucket's.
 ONE_UNIT_CTX = 896
 CTX_STEP = 256
 
@@ -123,6 +127,7 @@ class _IterationGraphs:
         self.stream = torch.cuda.Stream(device=dev)
         self.graphs: dict[tuple[int, int], torch.cuda.CUDAGraph] = {}
         self.t = self.d = self.target = self.draft = None  # bound for one call
+        self.by_step = False  # windowed or 8-bit attention: passes of one CTX_STEP only
 
     @staticmethod
     def usable(target, draft, t_cache, d_cache, propose) -> bool:
@@ -149,6 +154,8 @@ class _IterationGraphs:
         g = _GRAPHS.get(key)
         if g is None:
             g = _GRAPHS[key] = _IterationGraphs(t_cache.pool, k)
+            g.by_step = (windowed(target) or windowed(draft)
+                         or any(getattr(p, "k_scale", None) is not None for p in (tp, dp)))
             for obj in (target, draft, t_cache.pool, d_cache.pool):
                 weakref.finalize(obj, _GRAPHS.pop, key, None)
         g.target, g.draft, g.t, g.d = target, draft, t_cache, d_cache
@@ -166,7 +173,7 @@ class _IterationGraphs:
             return None
         if hi <= ONE_UNIT_CTX:
             return min(ONE_UNIT_CTX, cap)
-        if lo > ONE_UNIT_CTX:
+        if lo > ONE_UNIT_CTX and not (self.by_step and (lo - 1) // CTX_STEP != (hi - 1) // CTX_STEP):
             return min(-(-hi // CTX_STEP) * CTX_STEP, cap)
         return None
 
