@@ -72,7 +72,8 @@ class PagedKVCache:
     a multiple of 16 tokens, head_dim 64 or 128. Passes over it run through forward_hidden
     (greedy and speculative decoding, chains only); the batched engine needs a pool of the
     model's type. A block's scale only grows while the block holds rows, so tokens that a
-    rejected draft wrote may leave a coarser scale behind."""
+    rejected draft wrote may leave a coarser scale behind, and the accepted rows beside them
+    rounded to it: speculative decoding over such a pool need not give greedy decoding's tokens."""
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_blocks: int,
                  block_size: int, dtype: torch.dtype, device, max_seqs: int = 64,

@@ -286,7 +286,14 @@ def _feed(model, cache, ids: torch.Tensor) -> torch.Tensor:
 def speculative_greedy(target_model, draft_model, input_ids: torch.Tensor, target_cache,
                        draft_cache, k: int = 4, max_new_tokens: int = 32,
                        eos_token_id=AUTO_EOS, propose=None) -> SpecDecodeResult:
-    """Greedy speculative decoding; output equals greedy decoding of the target."""
+    """Greedy speculative decoding; output equals greedy decoding of the target, as far as the
+    passes' rounding does (a verify pass and one-token passes may part where two logits lie
+    within it).
+
+    Over 8-bit pools the two hold other codes: a block's scale covers every row that a pass wrote
+    into it, those of rejected drafts among them, and rows that are held are rounded again when it
+    grows (kernels.kv_write_q8). Each token is then the target's greedy choice over what the pool
+    held at its pass, not the token of greedy_paged over a pool of its own."""
     assert input_ids.dim() == 2 and input_ids.shape[0] == 1, "one request at a time"
     assert k >= 1, "k must be at least 1"
     assert target_cache.length == 0 and draft_cache.length == 0, "caches must be empty"
