@@ -260,7 +260,8 @@ int kve_sample_verify(const void* target, int64_t target_seq_stride, int64_t tar
  * block that holds rows already keeps its scale, or takes a larger one where a new row
  * needs it, and then the held rows' codes are rounded to it. Codes are the exact
  * quotients to the nearest, ties to even (E4M3: exact while every scale is a power of two).
- * NaN becomes 0; an infinity becomes the largest code and does not count for the scale.
+ * NaN becomes 0; an infinity becomes the largest code and does not count for the scale (in a
+ * block whose finite values are all zeros that scale is 0, and the infinity stands for 0 too).
  * Rows behind the pass's last keep their codes. A sequence's row may stand once in a
  * launch, and no two sequences of it may share a block that they write.
  * k_new, v_new, src_token_stride, dtype: as for kve_kv_write; block_size % 16 == 0,
@@ -279,12 +280,14 @@ int kve_kv_write_q8(const void* k_new, const void* v_new, int64_t src_token_stri
  * the queries' type or, with scales, an 8-bit one. The reference refuses models with a
  * window (forward.py:186-188) and has no such cache.
  * A key that a row does not see contributes nothing to it, whatever its K, V or scale
- * holds, and blocks that no query of the pass sees are not read (their table entries may
- * name anything). out: the shape and dtype of q; rows past q_lens and sequences that are
- * skipped keep what is there.
+ * holds or is being written there. Keys are read in aligned steps of 64 (32 in fp32 at
+ * head_dim 128), so blocks that no query of the pass sees are read where they share a step
+ * with one that is seen, and not elsewhere; their table entries may name anything (block 0
+ * is read for a number outside the pool). out: the shape and dtype of q; rows past q_lens and
+ * sequences that are skipped keep what is there.
  * pool_dtype: dtype, KVE_DTYPE_I8 or KVE_DTYPE_E4M3 (k_scale, v_scale as above; else NULL)
- * block_size % 16 == 0, head_dim 64 or 128, max_ctx and num_q_heads / num_kv_heads * q_len at most 2^30,
- * scale > 0; q, pools, out and workspace 16-byte aligned
+ * block_size % 16 == 0, head_dim 64 or 128, max_ctx at most 2^30, num_q_heads / num_kv_heads * q_len
+ * below it, scale > 0; q, pools, out and workspace 16-byte aligned
  * sinks: any number of 0 and more (INT32_MAX: every key, as window 0)
  * workspace: kve_window_workspace_bytes(...) bytes (0: none needed), no initialisation
  */

@@ -49,7 +49,7 @@ __device__ __forceinline__ float int8_code(float x, float s, float inv) {
 }
 
 // Codes of four values against a scale (inv of it), the first in the lowest byte. NaN
-// becomes 0 and an infinity the largest code.
+// becomes 0 and an infinity the largest code (0 where the scale is 0).
 template <Q8 Q>
 __device__ __forceinline__ uint32_t q8_codes(const float (&x)[4], float s, float inv) {
   float y[4];

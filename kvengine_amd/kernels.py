@@ -1162,7 +1162,8 @@ def kv_write_q8(k_new: torch.Tensor, v_new: torch.Tensor, k_layer: torch.Tensor,
     times its block's scale. A block written from its first row on takes the scale of its
     new rows (int8: largest / 127, e4m3: the least power of two that brings it to 448); one
     that holds rows keeps its scale or takes a larger one, and its rows follow. Codes are
-    to the nearest, ties to even; NaN becomes 0, an infinity the largest code. bs a
+    to the nearest, ties to even; NaN becomes 0, an infinity the largest code (of a block
+    whose finite values are all zeros, scale 0, it stands for 0). bs a
     multiple of 16. No two sequences of a call may write one block."""
     _need(k_new.dim() == 4 and k_new.shape == v_new.shape and k_new.is_cuda,
           "k_new/v_new must be [B, T, Hkv, D] on the GPU")
@@ -1245,9 +1246,10 @@ def paged_window_attn(q: torch.Tensor, k_layer: torch.Tensor, v_layer: torch.Ten
                       out: torch.Tensor | None = None) -> torch.Tensor:
     """paged_verify_attn under a sliding window: the query at position p sees the keys
     j <= p with j > p - window (itself and the window - 1 before it) or j < sinks. q
-    [B, T, Hq, D], pools and tables as there; blocks of a multiple of 16 tokens. Blocks
-    that no query of the pass sees are not read, so they may have been given away. Rows
-    past q_lens, and sequences that max_ctx does not cover, keep what out holds. The
+    [B, T, Hq, D], pools and tables as there; blocks of a multiple of 16 tokens. What a
+    query does not see adds nothing to it, whatever is or is being written there, so blocks
+    behind every window may have been given away (they are read where they share a step of 64
+    tokens with one that is seen). Rows past q_lens, and sequences that max_ctx does not cover, keep what out holds. The
     workspace is the call's own, so captured graphs share none."""
     _need(q.dim() == 4 and q.is_contiguous() and q.is_cuda, "q must be contiguous [B, T, Hq, D]")
     _need(k_layer.dim() == 4 and k_layer.dtype == q.dtype, "k layer must be [NB, Hkv, bs, D] of q's dtype")
@@ -1266,7 +1268,7 @@ def paged_q8_attn(q: torch.Tensor, k_layer: torch.Tensor, v_layer: torch.Tensor,
     """paged_verify_attn over an 8-bit pool (kv_write_q8: codes [NB, Hkv, bs, D] and
     [NB, Hkv, D, bs] of int8 or float8_e4m3fn, scales [NB, Hkv] float32), q bf16 or float32.
     window: None (every key up to the query's own) or paged_window_attn's, with its sinks;
-    the other arguments, what is not read and the result as there."""
+    the other arguments, what is not seen and the result as there."""
     _need(q.dim() == 4 and q.is_contiguous() and q.is_cuda, "q must be contiguous [B, T, Hq, D]")
     _need(k_layer.dim() == 4, "k layer must be [NB, Hkv, bs, D]")
     if window is not None and window < 1:
