@@ -16,8 +16,9 @@
 //
 // What bounds it: one decode step is launch and three dependent reads (length, block id, scale
 // and held codes): 32 sequences of 2 heads of 128 5.4 us. A prompt is bytes: 8 x 2049 tokens 9.0
-// us, 2.8 TB/s; a tile's reads, its maximum and its stores follow one another (18 with a workgroup
-// a tile, whose waves meet for the maximum and whose reads of V jump from token to token).
+// us, 2.8 TB/s; a tile's reads, its maximum and its stores follow one another in 4128 waves, four a
+// SIMD (110 registers at head_dim 128), of which the last 32 find no place beside the rest (18 with a
+// workgroup a tile, whose waves meet for the maximum and whose reads of V jump from token to token).
 
 #include "kve_q8.h"
 

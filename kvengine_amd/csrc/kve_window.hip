@@ -1,5 +1,5 @@
 // Attention over the paged cache with a sliding window and sinks, and over a cache held
-// in 8 bits (kve_paged_window_attn, kve_paged_q8_attn). The counterpart in the reference
+// in 8 bits (kve_paged_window_attn). The counterpart in the reference
 // is its gather and masked SDPA (kvengine/paged.py:315-331, forward.py:85-144), which knows
 // neither a window (it refuses such models) nor a quantised cache.
 //
@@ -46,14 +46,17 @@
 // row sees in part are taken without the non-finite values, which are then added to the rows
 // that do see them. Other steps are seen whole by every row. Half of a short walk's steps are
 // seen in part, so these are kept cheap: the ends that a step reaches are compared with constants,
-// and V is looked over before anything is dropped from it (182 -> 163 us at the prompt below, 18.6
-// -> 16.8 at 32 x 5).
+// and V is looked over before anything is dropped from it (a tenth of the time of a prompt and of
+// 32 x 5 tokens).
 //
 // What bounds it, at 16 query heads to 2 kv heads of 128 in bf16. A prompt of 4 x 4097 tokens under a
-// window of 1024: 154 us, 780 TFLOP/s, the matrix pipes busy 39 % and the vector units 52 % of the
-// time and LDS reads 41 %, hardly at once with two waves a SIMD. 32 x 5 new tokens, window 1024:
-// 12.6 us and 4.2 for the join, behind launch, tables and the first K/V. 32 int8 histories of 3000 to
-// 8128 tokens, one new token each: 22 us (3.9 TB/s) and 4. One token of 256 keys: 6.8 us.
+// window of 1024: 182 us in a run of calls, 660 TFLOP/s of the definition's products and half as
+// many again for P's second part, the matrix pipes busy 48 % and the vector units 52 % of the time
+// and LDS reads 34 %, hardly at once with two waves a SIMD. 32 x 5 new tokens, window 1024: 12.9 us
+// and 4.0 for the join, about 1.7 a step (LDS reads, products, softmax, products in series, for
+// one of the four waves has no rows there and one half a tile) behind launch, tables and the first
+// K/V. 32 int8 histories of 3000 to 8128 tokens, one new token each: 22.7 us (3.8 TB/s) and 4. One
+// token of 256 keys: 6.8 us.
 
 #include "kve_gemm.h"
 #include "kve_q8.h"
@@ -277,7 +280,7 @@ __global__ __launch_bounds__(win_threads(SHARED)) __attribute__((amdgpu_waves_pe
   const int tid = threadIdx.x, l = tid & 63, lr = l & 15, lg = l >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   // The last rows of all sequences come first: their walks are the longest, and what is left
-  // at the end is short (prompt of 4 x 4097 tokens 167 -> 160 us).
+  // at the end is short (4 % of a prompt of 4 x 4097 tokens).
   int u = blockIdx.x;
   const int c = u % a.splits;
   u /= a.splits;
@@ -935,9 +938,9 @@ struct WindowCfg {
 // 40, 376 39 / 43, 516 55 / 51, 656 58 / 49, 1032 103 / 89, 2056 227 / 188; 8-bit 258 42 / 51, 376
 // 48 / 54, 516 71 / 60, 1032 123 / 105, 2056 270 / 212; 9 tokens a sequence in bf16 128 30 / 31, 192
 // 36 / 43, 384 57 / 59, 512 75 / 63, 1024 147 / 115 (at 96 alone, where one round of workgroups is as
-// long as the longest walk, 28 / 26). With 264 rows, which take 384 for
-// 320, 768 workgroups 84 / 93, with 520, 640 for 576, 640 workgroups 77 / 84. fp32 queries, bound by products or registers,
-// keep one (prompt of 1025 242 / 275 us).
+// long as the longest walk, 28 / 26). With 264 rows, which take 384 for 320, 768 workgroups 84 / 93,
+// with 520, 640 for 576, 640 workgroups 77 / 84. fp32 queries, bound by products or registers, keep
+// one (prompt of 1025 242 / 275 us). So many workgroups are never cut.
 static WindowCfg window_cfg(int B, int Tq, int Hq, int Hkv, int D, int max_ctx, int window,
                             int sinks, int elem_bytes, bool f32) {
   WindowCfg c{};
