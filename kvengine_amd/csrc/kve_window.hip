@@ -918,7 +918,7 @@ constexpr int kFillWaves = 2048;
 // Workgroups from which on a wave takes two tiles of rows: two for each compute unit.
 constexpr int kTwoTiles = 512;
 // Tokens of history by whose whole numbers the cut of a walk follows max_ctx.
-constexpr int kCtxStep = 256;
+constexpr int kCtxStep = 256, kCtxLeast = 1024;
 
 struct WindowCfg {
   int mt, rows, row_groups, chunk, splits;  // mt 0: up to 16 rows
@@ -956,7 +956,9 @@ static WindowCfg window_cfg(int B, int Tq, int Hq, int Hkv, int D, int max_ctx, 
                             (static_cast<int64_t>(sinks) + sk - 1) / sk;
   // max_ctx decides where walks are cut by what it is in whole kCtxStep: a pass gives the same bits
   // under every bound from one to the next
-  const int64_t in_all = static_cast<int64_t>(cdiv(max_ctx, kCtxStep)) * (kCtxStep / sk);
+  // (one sequence in bf16, as replayed iterations are, also under every bound up to kCtxLeast)
+  const int bound = B == 1 && !f32 ? std::max(max_ctx, kCtxLeast) : max_ctx;
+  const int64_t in_all = static_cast<int64_t>(cdiv(bound, kCtxStep)) * (kCtxStep / sk);
   const int64_t longest = std::min(in_window, in_all);
   const int waves = c.mt == 0 ? kKeyWaves : 4;
   int64_t least = c.mt == 0 ? kKeyWaves : elem_bytes == 4 ? 1 : 4;

@@ -38,6 +38,16 @@ def test_one_order_between_multiples_of_256(T):
         assert common, (T, end)
 
 
+@pytest.mark.parametrize("T,Hkv", [(5, 2), (40, 8), (101, 8), (201, 8)])
+def test_one_order_under_every_bound_up_to_1024(T, Hkv):
+    """Also where so many rows share a walk that it is cut in few chunks."""
+    common = None
+    for ctx in (T, 256, 300, 512, 600, 700, 896, 1000, 1024):
+        got = lengths(max(ctx, T), T, BF16, Hq=8 * Hkv, Hkv=Hkv, pool=BF16)
+        common = got if common is None else common & got
+    assert common
+
+
 @pytest.mark.parametrize("window,sinks", [(0, 0), (800, 300), (1000, 0), (5000, 4)])
 def test_one_token_in_one_piece_up_to_1024(window, sinks):
     for ctx in (1, 64, 500, 896, 897, 960, 1000, 1023, 1024):
