@@ -94,7 +94,7 @@ __device__ __forceinline__ uint32_t q8_rescale(uint32_t w, float s0, float s) {
       r |= (static_cast<uint32_t>(static_cast<int>(fmin(fmax(rint(v), -127.0), 127.0))) & 0xffu)
            << (8 * i);
     else
-      y[i] = static_cast<float>(fmin(fmax(v, -448.0), 448.0));
+      y[i] = static_cast<float>(v == v ? fmin(fmax(v, -448.0), 448.0) : v);  // (a NaN stays)
   }
   if constexpr (Q == Q8::kInt8) {
     return r;
